@@ -1,14 +1,19 @@
-"""Single-kernel entry points (HIP build): run ONE training kernel on torch CUDA tensors.
+"""Entry points of single kernels and operators (HIP build) on torch CUDA tensors.
 
-The training loop never goes through these - it drives the kernels from C++ -
-they exist so that every hot kernel can be checked against a plain NumPy /
-PyTorch reference in isolation:
+Each of these runs ONE training kernel.  The training loop never goes through them - it
+drives the kernels from C++ - they exist so that every hot kernel can be checked against a
+plain NumPy / PyTorch reference in isolation:
 
 * :func:`hist_build`      - gradient histogram of a row list (LDS packed 64-bit atomics), feature-tile records
 * :func:`lines_hist_build` - the same through the fused growth kernel's root pass over 128-byte row lines
 * :func:`partition_rows`  - stable split of a row list by ``bin <= threshold``
 * :func:`split_scan`      - best split of one leaf histogram (wave prefix scan + fp64 gain)
 * :func:`pack_gradients`  - the (g, h) -> packed int64 quantisation used by the histograms
+
+and the operators that the prediction and refitting of whole ensembles are made of, for use on any tensors:
+
+* :func:`embedding`, :func:`embedding_grad`   - row lookup by token with scaling, its gradient by sorted tokens
+* :func:`gated_scan`, :func:`gated_scan_grad` - gated linear recurrence over long sequences and its gradients
 
 Without a GPU every function raises ``LightGBMError``.
 """
@@ -20,6 +25,8 @@ from typing import Any, Dict, Tuple
 import numpy as np
 
 from .. import _lib
+from .lookup import embedding, embedding_grad
+from .recurrence import gated_scan, gated_scan_grad
 
 TILE = 32
 BINS = 256

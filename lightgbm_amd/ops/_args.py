@@ -1,0 +1,102 @@
+"""Checks and layouts shared by the row lookup and the gated recurrence."""
+from __future__ import annotations
+
+import ctypes
+
+from .. import _lib
+from .._lib import LightGBMError
+
+_core = None
+_TYPE_CODES = {}
+_FLOATS = ("bfloat16", "float16", "float32", "float64")
+
+
+def core():
+    """The HIP core; raises where there is none."""
+    global _core
+    if _core is None:
+        lib, hip = _lib.load()
+        if not hip:
+            raise LightGBMError("lightgbm_amd.ops needs the HIP build and a visible GPU")
+        _core = lib
+    return _core
+
+
+def type_code(dtype) -> int:
+    """0..3 for bf16, fp16, fp32, fp64; -1 for every other type."""
+    if not _TYPE_CODES:
+        import torch
+        _TYPE_CODES.update({getattr(torch, name): i for i, name in enumerate(_FLOATS)})
+    return _TYPE_CODES.get(dtype, -1)
+
+
+def fail(what: str):
+    raise LightGBMError(what)
+
+
+def need_tensor(op: str, name: str, t):
+    import torch
+    if not isinstance(t, torch.Tensor):
+        fail(f"{op}: {name} has to be a torch tensor, got {type(t).__name__}")
+    if t.requires_grad and torch.is_grad_enabled():
+        fail(f"{op}: {name} requires grad, and nothing is recorded here: call it under torch.no_grad() and take the gradient from {op}_grad")
+    return t
+
+
+def need_type(op: str, name: str, t) -> int:
+    code = type_code(t.dtype)
+    if code < 0:
+        fail(f"{op}: {name} has to be bfloat16, float16, float32 or float64, got {t.dtype}")
+    return code
+
+
+def need_device(op: str, first, *others):
+    """All tensors on one GPU; returns its index."""
+    device = first.device
+    for t in others:
+        if t is not None and t.device != device:
+            fail(f"{op}: tensors on {device} and {t.device}")
+    if device.type != "cuda":
+        fail(f"{op}: needs tensors on the GPU, got {device}")
+    return device.index
+
+
+def stream_of(device: int) -> int:
+    import torch
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def launch(fn, args: bytes) -> None:
+    if fn(args, None) != 0:
+        _lib.check(-1)
+
+
+def workspace_bytes(fn, args: bytes) -> int:
+    n = ctypes.c_int64()
+    if fn(args, ctypes.byref(n)) != 0:
+        _lib.check(-1)
+    return n.value
+
+
+def two_dims(shape, *strides):
+    """Merges neighbouring dimensions that every stride tuple walks evenly.  Returns (sizes, [strides, ...]) of two
+    dimensions, or None if more are left."""
+    sizes, kept = [], [[] for _ in strides]
+    for d, n in enumerate(shape):
+        if n == 1:
+            continue
+        if sizes and all(k[-1] == n * s[d] for k, s in zip(kept, strides)):
+            sizes[-1] *= n
+            for k, s in zip(kept, strides):
+                k[-1] = s[d]
+        else:
+            sizes.append(n)
+            for k, s in zip(kept, strides):
+                k.append(s[d])
+    if len(sizes) > 2:
+        return None
+    while len(sizes) < 2:
+        sizes.insert(0, 1)
+        for k in kept:
+            k.insert(0, 0)
+    return sizes, kept

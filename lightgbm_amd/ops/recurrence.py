@@ -1,0 +1,156 @@
+"""Gated linear recurrence over the steps of a batch of sequences, and its gradients (``csrc/hip/recurrence.hip``).
+
+    states[:, t] = gate[:, t] * states[:, t - 1] + w * x[:, t]        w = 1, or 1 - gate (``mix=True``)
+
+Staged scores of a boosted ensemble are the recurrence over its trees without a gate (a running sum), those of a random
+forest its mixed form with gates ``(k - 1) / k`` (a running mean); recurrent layers of sequence models have a gate per
+channel or head.  Everything runs on torch's current stream of the tensors' device, can be captured into a HIP graph,
+and gives the same bits every time.
+"""
+from __future__ import annotations
+
+import struct
+
+from ._args import core, fail, launch, need_device, need_tensor, need_type, stream_of, workspace_bytes
+
+_SCAN = struct.Struct("20q")
+_SCAN_GRAD = struct.Struct("29q")
+
+
+def _wide(t):
+    import torch
+    return torch.float64 if t.dtype == torch.float64 else torch.float32
+
+
+def _rows(t):
+    """``t`` with a sequence step's channels next to each other."""
+    return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _check(op: str, x, code: int, gate, lengths, ends):
+    """Checks what forward and backward share; returns (gate, gate type code, groups)."""
+    import torch
+    b, t, d = x.shape
+    gate_code = groups = 0
+    if gate is not None:
+        need_tensor(op, "gate", gate)
+        gate_code = need_type(op, "gate", gate)
+        if gate_code != code and not (gate_code == 2 and code < 2):
+            fail(f"{op}: a gate of {gate.dtype} for values of {x.dtype}; it has to be of that type or, for 16-bit values, float32")
+        if gate.dim() != 3 or gate.shape[0] not in (1, b) or gate.shape[1] != t:
+            fail(f"{op}: the gate has to be [{b} or 1, {t}, groups], got {tuple(gate.shape)}")
+        groups = gate.shape[2]
+        if d and (groups < 1 or d % groups):
+            fail(f"{op}: the width {d} is not a multiple of the gate's {groups} groups")
+        gate = _rows(gate)
+    for name, end in ends:
+        if end is not None:
+            need_tensor(op, name, end)
+            if end.dtype != _wide(x) or end.shape != (b, d):
+                fail(f"{op}: {name} has to be {_wide(x)} [{b}, {d}], got {end.dtype} {tuple(end.shape)}")
+    if lengths is not None:
+        need_tensor(op, "lengths", lengths)
+        if lengths.dtype != torch.int32 or lengths.shape != (b,):
+            fail(f"{op}: lengths have to be int32 [{b}], got {lengths.dtype} {tuple(lengths.shape)}")
+    return gate, gate_code, groups
+
+
+def _address(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _contiguous(t):
+    return None if t is None else t.contiguous()
+
+
+def _gate_steps(gate, batch: int):
+    """Elements between the gates of neighbouring sequences and steps."""
+    if gate is None:
+        return 0, 0
+    return (gate.stride(0) if gate.shape[0] == batch else 0), gate.stride(1)
+
+
+def gated_scan(x, gate=None, state=None, *, mix: bool = False, lengths=None):
+    """All states of the recurrence: ``(states [batch, steps, width], last [batch, width])``.
+
+    ``x``: [batch, steps, width] of bf16, fp16, fp32 or fp64.  ``gate``: [batch or 1, steps, groups] of ``x``'s type or
+    float32, where channel ``d`` takes the gate of group ``d // (width / groups)``; ``None`` is a gate of one.  ``state``:
+    the state before the first step (zeros if not given).  ``lengths``: int32 [batch]; behind a sequence's length (clamped to
+    0 .. steps) the states are zero, ``last`` is the state after its last step, and what stands in ``x`` and ``gate`` there
+    is not used.  States are carried in float32 (float64 for fp64), which is also the type of ``state`` and ``last``: feeding
+    ``last`` back in continues a sequence, step by step or in pieces.
+    """
+    import torch
+    need_tensor("gated_scan", "x", x)
+    code = need_type("gated_scan", "x", x)
+    if x.dim() != 3:
+        fail(f"gated_scan: x has to be [batch, steps, width], got {tuple(x.shape)}")
+    gate, gate_code, groups = _check("gated_scan", x, code, gate, lengths, (("state", state),))
+    if mix and gate is None:
+        fail("gated_scan: the mixed form needs a gate")
+    device = need_device("gated_scan", x, gate, state, lengths)
+    lib = core()
+    x, state, lengths = _rows(x), _contiguous(state), _contiguous(lengths)
+    b, t, d = x.shape
+    states = torch.empty((b, t, d), dtype=x.dtype, device=x.device)
+    last = torch.empty((b, d), dtype=_wide(x), device=x.device)
+    if last.numel():
+        fn = lib.lga_hip_gated_scan
+        gate_b, gate_t = _gate_steps(gate, b)
+
+        def pack(work: int) -> bytes:
+            return _SCAN.pack(x.data_ptr(), _address(gate) if t else 0, _address(state), _address(lengths), states.data_ptr(), last.data_ptr(), work,
+                              stream_of(device), device, b, t, d, x.stride(0), x.stride(1), gate_b, gate_t, groups, code, gate_code, bool(mix))
+        need = workspace_bytes(fn, pack(0))
+        work = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+        launch(fn, pack(_address(work)))
+    return states, last
+
+
+def gated_scan_grad(grad_states, states, gate=None, state=None, *, x=None, grad_last=None, mix: bool = False, lengths=None):
+    """Gradients of :func:`gated_scan`: ``(grad_x, grad_state, grad_gate)``.
+
+    ``states`` is what the forward pass gave back; ``gate``, ``state``, ``mix`` and ``lengths`` are what it got, and ``x``
+    too if it was the mixed form.  ``grad_states`` and ``grad_last`` are the gradients of its two results (``grad_last`` may
+    be left out).  ``grad_x`` has the type of ``states``, ``grad_state`` is float32 (float64), ``grad_gate`` has the gate's
+    type and shape - summed over the channels and sequences that shared a gate - and is ``None`` without one.  Behind a
+    sequence's length all of them are zero.
+    """
+    import torch
+    need_tensor("gated_scan_grad", "grad_states", grad_states)
+    need_tensor("gated_scan_grad", "states", states)
+    code = need_type("gated_scan_grad", "states", states)
+    if states.dim() != 3:
+        fail(f"gated_scan_grad: states have to be [batch, steps, width], got {tuple(states.shape)}")
+    for name, like in (("grad_states", grad_states), ("x", x)):
+        if like is not None:
+            need_tensor("gated_scan_grad", name, like)
+            if like.dtype != states.dtype or like.shape != states.shape:
+                fail(f"gated_scan_grad: {name} has to be {states.dtype} {tuple(states.shape)} as the states, got {like.dtype} {tuple(like.shape)}")
+    gate, gate_code, groups = _check("gated_scan_grad", states, code, gate, lengths, (("state", state), ("grad_last", grad_last)))
+    if mix and (gate is None or x is None):
+        fail("gated_scan_grad: the mixed form needs the gate and x")
+    device = need_device("gated_scan_grad", states, grad_states, x, gate, state, grad_last, lengths)
+    lib = core()
+    grad_states, states, x = _rows(grad_states), _rows(states), _rows(x) if mix else None
+    state, grad_last, lengths = _contiguous(state), _contiguous(grad_last), _contiguous(lengths)
+    b, t, d = states.shape
+    grad_x = torch.empty((b, t, d), dtype=states.dtype, device=states.device)
+    grad_state = torch.empty((b, d), dtype=_wide(states), device=states.device)
+    grad_gate = None if gate is None else torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
+    if grad_state.numel():
+        fn = lib.lga_hip_gated_scan_grad
+        gate_b, gate_t = _gate_steps(gate, b)
+        x_b, x_t = (x.stride(0), x.stride(1)) if mix else (0, 0)
+
+        def pack(work: int) -> bytes:
+            return _SCAN_GRAD.pack(grad_states.data_ptr(), states.data_ptr(), _address(gate) if t else 0, _address(state), _address(x),
+                                   _address(grad_last), _address(lengths), grad_x.data_ptr(), grad_state.data_ptr(), _address(grad_gate), work,
+                                   stream_of(device), device, b, t, d, grad_states.stride(0), grad_states.stride(1), states.stride(0),
+                                   states.stride(1), x_b, x_t, gate_b, gate_t, groups, 0 if gate is None else gate.shape[0], code, gate_code, bool(mix))
+        need = workspace_bytes(fn, pack(0))
+        work = torch.empty(need, dtype=torch.uint8, device=states.device) if need else None
+        launch(fn, pack(_address(work)))
+    elif grad_gate is not None:
+        grad_gate.zero_()
+    return grad_x, grad_state, grad_gate

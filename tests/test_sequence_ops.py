@@ -1,0 +1,619 @@
+"""Row lookup and gated recurrence (lightgbm_amd.ops): the formulas in 64 bits, the refusals, and their use together.
+
+Tolerances count roundings.  u(T) = eps(T) / 2 is the relative error of one rounding to T; sums and states are held in
+W (fp32, for fp64 fp64).  A sum of n terms, in any order, is off by at most (n - 1) u(W) times the sum of their absolute
+values.  In the recurrence a term passes at most two roundings a step (one in the product of the gates, one in the sum,
+whichever way the steps are grouped) and a handful at the ends, so a state is off by at most (2 t + 10) u(W) times the
+same recurrence over absolute values.  1.01 covers the products of these errors, `_TINY` what underflows.
+"""
+import itertools
+
+import numpy as np
+import pytest
+import torch
+
+from lightgbm_amd import LightGBMError, ops
+
+gpu = pytest.mark.gpu
+TYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32, "f64": torch.float64}
+_TINY = {torch.bfloat16: 1e-38, torch.float16: 2.0**-25, torch.float32: 1e-38, torch.float64: 1e-300}
+
+
+def u(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def wide(dtype):
+    return torch.float64 if dtype == torch.float64 else torch.float32
+
+
+def rng(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def normal(g, shape, dtype):
+    return torch.randn(shape, generator=g, dtype=torch.float64).to(dtype)
+
+
+def within(got, want, bound, dtype):
+    """|got - want| <= bound + the rounding to dtype, element by element."""
+    got = got.detach().double().cpu()
+    allowed = 1.01 * (bound + u(dtype) * want.abs()) + _TINY[dtype]
+    off = (got - want).abs()
+    assert got.shape == want.shape
+    bad = ~(off <= allowed)
+    assert not bad.any(), (int(bad.sum()), off[bad].max().item(), allowed[bad].min().item(), torch.nonzero(bad)[0].tolist())
+
+
+# -- oracles, on the CPU in 64 bits -----------------------------------------------------------------------------------
+
+def lookup_oracle(table, ids, scale):
+    t = torch.cat([table.double().cpu(), torch.zeros((1, table.shape[1]), dtype=torch.float64)])
+    i = ids.long().cpu()
+    i = torch.where((i >= 0) & (i < table.shape[0]), i, torch.full_like(i, table.shape[0]))
+    return t[i] * scale
+
+
+def lookup_grad_oracle(grad, ids, rows, scale):
+    """(sums, sums of absolute values, tokens of every row)."""
+    i = ids.long().cpu().reshape(-1)
+    g = grad.double().cpu().reshape(i.numel(), grad.shape[-1])
+    ok = (i >= 0) & (i < rows)
+    out, mag = torch.zeros((rows, g.shape[1]), dtype=torch.float64), torch.zeros((rows, g.shape[1]), dtype=torch.float64)
+    out.index_add_(0, i[ok], g[ok])
+    mag.index_add_(0, i[ok], g[ok].abs())
+    n = torch.zeros(rows, dtype=torch.float64).index_add_(0, i[ok], torch.ones(int(ok.sum()), dtype=torch.float64))
+    return out * scale, mag * abs(scale), n
+
+
+def _gates(gate, b, t, d):
+    if gate is None:
+        return torch.ones((b, t, d), dtype=torch.float64)
+    a = gate.double().cpu()
+    return a.repeat_interleave(d // a.shape[2], dim=2).expand(b, t, d)
+
+
+def scan_oracle(x, gate, state, mix, lengths):
+    """(states, last, bound of the states, bound of the last)."""
+    b, t, d = x.shape
+    a, xs = _gates(gate, b, t, d), x.double().cpu()
+    n = torch.full((b,), t) if lengths is None else lengths.cpu().long().clamp(0, t)
+    h = torch.zeros((b, d), dtype=torch.float64) if state is None else state.double().cpu()
+    s = h.abs()
+    states, mags = torch.zeros((b, t, d), dtype=torch.float64), torch.zeros((b, t, d), dtype=torch.float64)
+    for k in range(t):
+        live = (k < n).reshape(b, 1)
+        w = (1 - a[:, k]) * xs[:, k] if mix else xs[:, k]
+        h = torch.where(live, a[:, k] * h + w, h)
+        s = torch.where(live, a[:, k].abs() * s + w.abs(), s)
+        states[:, k] = torch.where(live, h, torch.zeros_like(h))
+        mags[:, k] = torch.where(live, s, torch.zeros_like(s))
+    e = u(wide(x.dtype))
+    steps = torch.arange(t, dtype=torch.float64).reshape(1, t, 1)
+    return states, h, (2 * steps + 12) * e * mags, (2 * t + 12) * e * s
+
+
+def scan_grad_oracle(dh, states, gate, state, x, dlast, mix, lengths):
+    """(grad_x, grad_state, grad_gate) and their bounds."""
+    b, t, d = states.shape
+    a = _gates(gate, b, t, d)
+    n = torch.full((b,), t) if lengths is None else lengths.cpu().long().clamp(0, t)
+    zero = torch.zeros((b, d), dtype=torch.float64)
+    e = zero if dlast is None else dlast.double().cpu()
+    s = e.abs()
+    first = zero if state is None else state.double().cpu()
+    hs, g = states.double().cpu(), dh.double().cpu()
+    gx, gx_b = torch.zeros((b, t, d), dtype=torch.float64), torch.zeros((b, t, d), dtype=torch.float64)
+    da, da_b = gx.clone(), gx.clone()
+    for k in reversed(range(t)):
+        live = (k < n).reshape(b, 1)
+        c, cs = e + g[:, k], s + g[:, k].abs()
+        before = hs[:, k - 1] if k else first
+        if mix:
+            xv = x.double().cpu()[:, k]
+            w, slope, mag = 1 - a[:, k], before - xv, before.abs() + xv.abs()
+        else:
+            w, slope, mag = torch.ones_like(c), before, before.abs()
+        gx[:, k], gx_b[:, k] = torch.where(live, w * c, zero), torch.where(live, w.abs() * cs, zero)
+        da[:, k], da_b[:, k] = torch.where(live, c * slope, zero), torch.where(live, cs * mag, zero)
+        e, s = torch.where(live, a[:, k] * c, e), torch.where(live, a[:, k].abs() * cs, s)
+    r = u(wide(states.dtype))
+    back = (t - torch.arange(t, dtype=torch.float64)).reshape(1, t, 1)
+    out = [(gx, (2 * back + 12) * r * gx_b), (e, (2 * t + 12) * r * s)]
+    if gate is None:
+        return out + [None]
+    groups = gate.shape[2]
+    terms = d // groups * (b if gate.shape[0] < b else 1)
+
+    def shared(v):
+        v = v.reshape(b, t, groups, d // groups).sum(3)
+        return v.sum(0, keepdim=True) if gate.shape[0] < b else v
+    return out + [(shared(da), (2 * back + 14 + terms) * r * shared(da_b))]
+
+
+# -- row lookup -------------------------------------------------------------------------------------------------------
+
+def make_ids(g, shape, rows, dtype=torch.int64, pad=0.1, kind="uniform"):
+    if kind == "one":
+        ids = torch.full(shape, max(0, rows - 1), dtype=dtype)
+    elif kind == "few":
+        ids = (torch.rand(shape, generator=g, dtype=torch.float64) ** 6 * rows).to(dtype)
+    else:
+        ids = torch.randint(0, max(rows, 1), shape, generator=g, dtype=dtype)
+    out = torch.rand(shape, generator=g) < pad
+    wrong = torch.tensor([-1, rows, -2**31, 2**31 - 1])[torch.randint(0, 4, shape, generator=g)]
+    return torch.where(out, wrong.to(dtype), ids)
+
+
+LOOKUPS = [((1,), 1, 1), ((0,), 5, 8), ((7,), 3, 5), ((64,), 100, 8), ((257,), 33, 64), ((3, 5), 10, 129), ((2, 3, 4), 50, 256),
+           ((1000,), 7, 1), ((513,), 1000, 3), ((130,), 64, 1024), ((65,), 40, 2050), ((5,), 4, 4096), ((40, 300), 90, 1), ((33, 65), 90, 7)]
+
+
+@gpu
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("shape,rows,width", LOOKUPS)
+def test_lookup_is_the_scaled_row(shape, rows, width, name):
+    g = rng(rows * 7 + width)
+    table = normal(g, (rows, width), TYPES[name])
+    for dtype, scale in ((torch.int64, 1.0), (torch.int32, 0.3)):
+        ids = make_ids(g, shape, rows, dtype)
+        got = ops.embedding(table.cuda(), ids.cuda(), scale=scale)
+        assert got.dtype == table.dtype and got.is_contiguous()
+        want = lookup_oracle(table, ids, scale)
+        within(got, want, 3 * u(wide(table.dtype)) * want.abs(), table.dtype)
+        if scale == 1.0:
+            assert torch.equal(got.double().cpu(), want)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f64"])
+def test_lookup_reads_strided_tables_and_ids_in_place(name):
+    g = rng(3)
+    big = normal(g, (40, 6, 72), TYPES[name]).cuda()
+    ids = make_ids(g, (70, 130), 40, torch.int32).cuda()
+    for table in (big[:, 2, :64], big[:, 0, 1:62], big.transpose(1, 2)[:, :, 3], big[3:4, 0].expand(40, 72), big[::2, 1, 8:24]):
+        for i in (ids.t(), ids[::2, ::3], ids[:, 5], ids.t()[4:, 1:], ids.reshape(10, 7, 130).permute(2, 0, 1), ids[:1].expand(9, 130)):
+            got = ops.embedding(table, i, scale=0.7)
+            want = lookup_oracle(table, i, 0.7)
+            within(got, want, 3 * u(wide(table.dtype)) * want.abs(), table.dtype)
+
+
+@gpu
+def test_lookup_passes_on_infinities_and_nan_of_named_rows_only():
+    table = torch.ones((4, 16))
+    table[1], table[2], table[3] = float("inf"), float("nan"), -float("inf")
+    got = ops.embedding(table.cuda(), torch.tensor([0, 1, 2, 3, -1, 4]).cuda(), scale=-2.0).cpu()
+    assert torch.equal(got[:, 0].nan_to_num(7.0, 8.0, 9.0), torch.tensor([-2.0, 9.0, 7.0, 8.0, 0.0, 0.0]))
+
+
+@gpu
+def test_lookup_of_offsets_behind_32_bits():
+    table = torch.zeros((70000, 32768), dtype=torch.bfloat16, device="cuda")        # 2.3e9 elements
+    table[-1] = 3.0
+    table[65536] = 5.0
+    ids = torch.tensor([69999, 65536, 0, 69999], dtype=torch.int32, device="cuda")
+    got = ops.embedding(table, ids)
+    assert got.float().mean(1).tolist() == [3.0, 5.0, 0.0, 3.0]
+    many = ids.repeat(17500)
+    out = ops.embedding(table, many)                                                   # and as many out
+    assert out[-4:].float().mean(1).tolist() == [3.0, 5.0, 0.0, 3.0] and out[65538].float().sum() == 0
+
+
+GRADS = [((0,), 5, 8, "uniform"), ((1,), 1, 1, "uniform"), ((9,), 0, 4, "uniform"), ((40,), 1, 7, "one"), ((300,), 5000, 40, "uniform"),
+         ((2000,), 300, 33, "few"), ((5000,), 60, 1, "uniform"), ((4097,), 70000, 3, "uniform"), ((20000,), 40, 64, "one"), ((30000,), 3000, 130, "few"),
+         ((70, 300), 900, 1, "uniform"), ((33000,), 257, 2, "few"), ((12, 90, 11), 65537, 8, "uniform"), ((50001,), 70001, 16, "few"),
+         ((100000,), 20, 1, "one"), ((70001,), 300, 1, "few")]
+
+
+@gpu
+@pytest.mark.parametrize("shape,rows,width,kind", GRADS)
+@pytest.mark.parametrize("name,out", [("bf16", "bf16"), ("bf16", "f32"), ("f16", "f16"), ("f32", "f32"), ("f64", "f64")])
+def test_lookup_gradient_is_the_sum_over_the_tokens_of_a_row(shape, rows, width, kind, name, out):
+    g = rng(rows + width)
+    grad = normal(g, (*shape, width), TYPES[name])
+    for dtype, pad, scale in ((torch.int64, 0.1, 1.0), (torch.int32, 0.0, -0.3)):
+        ids = make_ids(g, shape, rows, dtype, pad, kind)
+        got = ops.embedding_grad(grad.cuda(), ids.cuda(), rows, scale=scale, dtype=TYPES[out])
+        again = ops.embedding_grad(grad.cuda(), ids.cuda(), rows, scale=scale, dtype=TYPES[out])
+        assert got.dtype == TYPES[out] and got.shape == (rows, width) and torch.equal(got, again)
+        want, mag, n = lookup_grad_oracle(grad, ids, rows, scale)
+        within(got, want, (n + 4).reshape(-1, 1) * u(wide(TYPES[name])) * mag, TYPES[out])
+        assert not got[(n == 0).to("cuda")].any()
+
+
+@gpu
+def test_lookup_gradient_reads_expanded_and_strided_gradients_in_place():
+    g = rng(11)
+    ids = make_ids(g, (500, 60), 400, torch.int32)
+    per_row = normal(g, (500, 1, 3), torch.float32)
+    wide_grad = normal(g, (60, 500, 8), torch.float32)
+    for ids_view, grad in ((ids, per_row.expand(500, 60, 3)), (ids.t(), per_row.transpose(0, 1).expand(60, 500, 3)), (ids.t(), wide_grad[:, :, 2:7]),
+                           (ids, wide_grad.transpose(0, 1)), (ids[::2, 3:7], wide_grad[3:7, ::2, 1].t().unsqueeze(2))):
+        got = ops.embedding_grad(_on_gpu(grad), _on_gpu(ids_view), 400, scale=2.0)
+        want, mag, n = lookup_grad_oracle(grad, ids_view, 400, 2.0)
+        within(got, want, (n + 4).reshape(-1, 1) * u(torch.float32) * mag, torch.float32)
+
+
+def _on_gpu(t):
+    """A copy on the GPU with the same strides."""
+    size = 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    flat = torch.as_strided(t, (size,), (1,), t.storage_offset()).cuda()
+    return torch.as_strided(flat, t.shape, t.stride())
+
+
+@gpu
+def test_lookup_gradient_equals_differences_of_the_lookup():
+    g = rng(5)
+    table, ids = normal(g, (30, 6), torch.float64).cuda(), make_ids(g, (200,), 30).cuda()
+    weight = normal(g, (200, 6), torch.float64).cuda()
+    grad = ops.embedding_grad(weight, ids, 30, scale=0.5)
+    for v, k in itertools.product((0, 7, 29), (0, 5)):
+        up, down = table.clone(), table.clone()
+        up[v, k] += 0.5
+        down[v, k] -= 0.5
+        diff = (ops.embedding(up, ids, 0.5) * weight).sum() - (ops.embedding(down, ids, 0.5) * weight).sum()
+        # linear in the table: the difference is the gradient, up to the roundings of two sums of 1200 terms of about 1
+        assert abs(diff.item() - grad[v, k].item()) <= 1200 * 1200 * 8 * u(torch.float64)
+
+
+# -- recurrence -------------------------------------------------------------------------------------------------------
+
+def make_scan(g, b, t, d, name, gate_name, groups, gate_batch, state, lengths):
+    x = normal(g, (b, t, d), TYPES[name])
+    gate = None
+    if groups:
+        a = torch.sigmoid(normal(g, (gate_batch, t, groups), torch.float64) + 1.5)
+        pick = torch.rand((gate_batch, t, groups), generator=g)
+        a = torch.where(pick < 0.02, torch.zeros_like(a), torch.where(pick > 0.98, torch.ones_like(a), a))
+        a = torch.where((pick > 0.5) & (pick < 0.55), -a, a)
+        gate = a.to(TYPES[gate_name])
+    w = wide(TYPES[name])
+    first = normal(g, (b, d), w) if state else None
+    n = None
+    if lengths:
+        n = torch.randint(0, t + 1, (b,), generator=g, dtype=torch.int32)
+        n[0], n[-1] = (t, 0) if b > 1 else (max(0, t - 1), max(0, t - 1))
+        if b > 3:
+            n[1], n[2] = t + 5, -3        # clamped
+    return x, gate, first, n
+
+
+#        batch steps width  type  gate  groups gate_batch mix state lengths
+SCANS = [(1, 1, 1, "f32", "f32", 1, 1, False, False, False),
+         (3, 1, 64, "bf16", "f32", 64, 3, False, True, False),
+         (2, 1, 130, "f16", "f16", 130, 1, True, True, True),
+         (2, 2, 5, "f64", "f64", 5, 2, True, True, False),
+         (4, 7, 33, "bf16", "bf16", 33, 4, True, True, True),
+         (1, 16, 64, "f32", "f32", 0, 0, False, True, False),
+         (5, 17, 128, "bf16", "f32", 8, 5, False, True, True),
+         (2, 65, 1, "f32", "f32", 1, 1, False, True, True),
+         (1, 128, 300, "f64", "f64", 1, 1, True, False, False),
+         (3, 129, 96, "f16", "f32", 3, 1, True, True, True),
+         (1, 500, 451, "f64", "f64", 0, 0, False, False, False),
+         (2, 513, 16, "bf16", "bf16", 16, 2, False, True, False),
+         (7, 1000, 3, "f32", "f32", 3, 7, False, True, True),
+         (1, 2049, 515, "f32", "f32", 5, 1, False, True, False),
+         (4, 300, 256, "bf16", "f32", 256, 4, True, True, True),
+         (2, 4097, 66, "f16", "f16", 66, 2, False, False, True),
+         (1, 20000, 40, "f32", "f32", 40, 1, True, True, False),
+         (65, 40, 24, "bf16", "bf16", 24, 1, False, True, True),
+         (3, 700, 128, "f64", "f64", 4, 3, True, True, True)]
+
+
+@gpu
+@pytest.mark.parametrize("case", SCANS, ids=lambda c: "-".join(map(str, c)))
+def test_recurrence_and_its_gradients_follow_the_formula(case):
+    b, t, d, name, gate_name, groups, gate_batch, mix, with_state, with_lengths = case
+    g = rng(t * 31 + d)
+    x, gate, state, lengths = make_scan(g, b, t, d, name, gate_name, groups, gate_batch, with_state, with_lengths)
+    to = lambda v: None if v is None else v.cuda()
+    states, last = ops.gated_scan(to(x), to(gate), to(state), mix=mix, lengths=to(lengths))
+    again = ops.gated_scan(to(x), to(gate), to(state), mix=mix, lengths=to(lengths))
+    assert torch.equal(states, again[0]) and torch.equal(last, again[1])
+    assert states.dtype == x.dtype and last.dtype == wide(x.dtype) and states.is_contiguous()
+    want, want_last, bound, bound_last = scan_oracle(x, gate, state, mix, lengths)
+    within(states, want, bound, x.dtype)
+    within(last, want_last, bound_last, last.dtype)
+
+    dh, dlast = normal(g, (b, t, d), x.dtype), normal(g, (b, d), wide(x.dtype)) if with_state else None
+    got = ops.gated_scan_grad(to(dh), states, to(gate), to(state), x=to(x), grad_last=to(dlast), mix=mix, lengths=to(lengths))
+    again = ops.gated_scan_grad(to(dh), states, to(gate), to(state), x=to(x), grad_last=to(dlast), mix=mix, lengths=to(lengths))
+    expect = scan_grad_oracle(dh, states.cpu(), gate, state, x, dlast, mix, lengths)
+    for value, same, oracle, dtype in zip(got, again, expect, (x.dtype, wide(x.dtype), None if gate is None else gate.dtype)):
+        if oracle is None:
+            assert value is None
+            continue
+        assert value.dtype == dtype and torch.equal(value, same)
+        within(value, *oracle, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["bf16", "f32"])
+def test_recurrence_reads_strided_tensors_in_place(name):
+    g = rng(9)
+    big = normal(g, (6, 50, 3, 72), TYPES[name])
+    gates = torch.sigmoid(normal(g, (6, 50, 3, 72), TYPES[name]))
+    to = _on_gpu
+    for x, gate in ((big[:, :, 1, :64], gates[:, :, 2, 4:68]), (big[:, :, 0, 1:62], gates[:1, :, 0, 3:4]), (big[::2, 10:, 2], gates[::2, 10:, 1]),
+                    (big.transpose(0, 1)[:, :, 1], gates.transpose(0, 1)[:, :, 0, :8]), (big[:1, :, 0].expand(4, 50, 72), gates[:1, :, 0].expand(4, 50, 72)),
+                    (big[:, :, :, 5], gates[:, :, :, 6]), (big.permute(0, 3, 1, 2)[:, :, :, 1], gates.permute(0, 3, 1, 2)[:, :, :, 1])):
+        x_g, gate_g = to(x), to(gate)
+        states, last = ops.gated_scan(x_g, gate_g, mix=True)
+        want, want_last, bound, bound_last = scan_oracle(x, gate, None, True, None)
+        within(states, want, bound, x.dtype)
+        within(last, want_last, bound_last, last.dtype)
+        dh = normal(g, x.shape, x.dtype)
+        got = ops.gated_scan_grad(dh.cuda().transpose(0, 1).contiguous().transpose(0, 1), states, gate_g, x=x_g, mix=True)
+        for value, oracle, dtype in zip(got, scan_grad_oracle(dh, states.cpu(), gate, None, x, None, True, None), (x.dtype, wide(x.dtype), gate.dtype)):
+            within(value, *oracle, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("t,d", [(40, 64), (300, 128), (1500, 37)])
+def test_what_stands_behind_a_length_reaches_nothing(t, d):
+    g = rng(t)
+    x, gate, state, _ = make_scan(g, 4, t, d, "f32", "f32", d, 4, True, False)
+    n = torch.tensor([0, 1, t // 2, t], dtype=torch.int32)
+    dh, dlast = normal(g, (4, t, d), torch.float32), normal(g, (4, d), torch.float32)
+    behind = (torch.arange(t).reshape(1, t, 1) >= n.reshape(4, 1, 1)).expand(4, t, d)
+    results = []
+    for junk in (0.0, float("nan"), float("inf"), -3e38):
+        fill = lambda v: torch.where(behind, torch.full_like(v, junk), v).cuda()
+        states, last = ops.gated_scan(fill(x), fill(gate), state.cuda(), lengths=n.cuda(), mix=True)
+        assert not states[behind.cuda()].any()
+        got = ops.gated_scan_grad(fill(dh), fill(states.cpu()), fill(gate), state.cuda(), x=fill(x), grad_last=dlast.cuda(), mix=True, lengths=n.cuda())
+        assert not got[0][behind.cuda()].any() and not got[2][behind.cuda()].any()
+        assert torch.equal(last[0].cpu(), state[0]) and torch.equal(got[1][0].cpu(), dlast[0])
+        results.append((states, last, *got))
+    for other in results[1:]:
+        assert all(torch.equal(p, q) for p, q in zip(results[0], other))
+
+
+@gpu
+def test_a_gate_of_zero_starts_anew_and_infinities_stay_where_they_are():
+    x = torch.ones((2, 600, 64))
+    gate = torch.full((2, 600, 64), 0.5)
+    x[0, 100] = float("inf")
+    x[1, 70, 3] = float("nan")
+    states, last = ops.gated_scan(x.cuda(), gate.cuda())
+    states = states.cpu()
+    assert torch.isfinite(states[0, :100]).all() and torch.isinf(states[0, 100:]).all()
+    nan = torch.isnan(states[1])
+    assert nan[70:, 3].all() and int(nan.sum()) == 530
+    long = ops.gated_scan(torch.ones((1, 3000, 8)).cuda(), torch.zeros((1, 3000, 1)).cuda(), torch.full((1, 8), 1e30).cuda())[0]
+    assert torch.equal(long.cpu(), torch.ones((1, 3000, 8)))
+
+
+@gpu
+@pytest.mark.parametrize("mix", [False, True])
+def test_pieces_and_single_steps_continue_a_sequence(mix):
+    g = rng(21)
+    x, gate, state, _ = make_scan(g, 3, 400, 96, "bf16", "f32", 96, 3, True, False)
+    x, gate, state = x.cuda(), gate.cuda(), state.cuda()
+    whole, last = ops.gated_scan(x, gate, state, mix=mix)
+    want, want_last, bound, bound_last = scan_oracle(x, gate, state, mix, None)
+    h, pieces = state, []
+    for at in [0, 1, 2, 3, 50, 51, 180, 399]:
+        end = {0: 1, 1: 2, 2: 3, 3: 50, 50: 51, 51: 180, 180: 399, 399: 400}[at]
+        part, h = ops.gated_scan(x[:, at:end], gate[:, at:end], h, mix=mix)
+        pieces.append(part)
+    within(torch.cat(pieces, 1), want, bound, torch.bfloat16)
+    within(h, want_last, bound_last, torch.float32)
+    within(whole, want, bound, torch.bfloat16)
+
+
+@gpu
+def test_gradients_of_the_recurrence_equal_differences():
+    g = rng(2)
+    b, t, d = 2, 70, 6
+    x, gate, state, _ = make_scan(g, b, t, d, "f64", "f64", 3, 1, True, False)
+    n = torch.tensor([70, 41], dtype=torch.int32).cuda()
+    x, gate, state = x.cuda(), gate.cuda(), state.cuda()
+    weight, weight_last = normal(g, (b, t, d), torch.float64).cuda(), normal(g, (b, d), torch.float64).cuda()
+
+    def loss(x, gate, state):
+        states, last = ops.gated_scan(x, gate, state, mix=True, lengths=n)
+        return ((states * weight).sum() + (last * weight_last).sum()).item()
+    states, _ = ops.gated_scan(x, gate, state, mix=True, lengths=n)
+    grads = ops.gated_scan_grad(weight, states, gate, state, x=x, grad_last=weight_last, mix=True, lengths=n)
+    step = 1e-4
+    for which, (value, grad) in enumerate(zip((x, state, gate), grads)):
+        for at in range(0, value.numel(), max(1, value.numel() // 17)):
+            moved = []
+            for sign in (1, -1):
+                copy = value.clone()
+                copy.view(-1)[at] += sign * step
+                args = [x, gate, state]
+                args[(0, 2, 1)[which]] = copy
+                moved.append(loss(*args))
+            # values about 10, summed over 840 terms: 1e-9 from roundings over 2e-4, 1e-8 (cubic term) from the step
+            assert abs((moved[0] - moved[1]) / (2 * step) - grad.view(-1)[at].item()) <= 1e-4
+
+
+@gpu
+def test_recurrence_of_offsets_behind_32_bits():
+    t, d = 66000, 32768                                             # 2.16e9 values, 4.3 GB
+    x = torch.zeros((1, t, d), dtype=torch.bfloat16, device="cuda")
+    x[0, 3], x[0, -2] = 1.0, 2.0
+    gate = torch.ones((1, t, 1), dtype=torch.bfloat16, device="cuda")
+    states, last = ops.gated_scan(x, gate)
+    assert torch.equal(last, torch.full_like(last, 3.0))
+    for at, want in ((2, 0.0), (3, 1.0), (t - 3, 1.0), (t - 2, 3.0), (t - 1, 3.0)):
+        assert states[0, at].eq(want).all()
+    grad_x, grad_state, grad_gate = ops.gated_scan_grad(x, states, gate)
+    assert grad_state.eq(3.0).all() and grad_x[0, t - 1].eq(0).all() and grad_x[0, t - 2].eq(2).all() and grad_x[0, 0].eq(3).all()
+    # da[t] = sum over the channels of c[t] h[t-1]: 32768 of 2 * 1 at t - 2, none where either is zero
+    assert grad_gate[0, t - 2, 0].item() == 65536.0 and grad_gate[0, 3, 0].item() == 0.0 and grad_gate[0, t - 1, 0].item() == 0.0
+
+
+# -- streams, graphs, empties -----------------------------------------------------------------------------------------
+
+def _everything(seed, t=300, d=96):
+    g = rng(seed)
+    ids = make_ids(g, (2, t), 700, torch.int64, kind="few").cuda()
+    table = normal(g, (700, d), torch.bfloat16).cuda()
+    gate = torch.sigmoid(normal(g, (2, t, d), torch.float32)).cuda()
+    dh = normal(g, (2, t, d), torch.bfloat16).cuda()
+    return ids, table, gate, dh
+
+
+def _chain(ids, table, gate, dh):
+    """Lookup, recurrence and both gradients, as a training step runs them."""
+    x = ops.embedding(table, ids, scale=2.0)
+    states, last = ops.gated_scan(x, gate, mix=True)
+    grad_x, grad_state, grad_gate = ops.gated_scan_grad(dh, states, gate, x=x, mix=True)
+    grad_table = ops.embedding_grad(grad_x, ids, table.shape[0], scale=2.0, dtype=torch.float32)
+    return x, states, last, grad_x, grad_state, grad_gate, grad_table
+
+
+@gpu
+@pytest.mark.parametrize("t,d", [(1, 64), (60, 96), (300, 96), (2500, 130)])
+def test_a_training_step_of_all_four_follows_the_formulas(t, d):
+    ids, table, gate, dh = _everything(t, t, d)
+    x, states, last, grad_x, grad_state, grad_gate, grad_table = _chain(ids, table, gate, dh)
+    want = lookup_oracle(table, ids, 2.0)
+    assert torch.equal(x.double().cpu(), want)
+    want, want_last, bound, bound_last = scan_oracle(x, gate, None, True, None)
+    within(states, want, bound, torch.bfloat16)
+    for value, oracle, dtype in zip((grad_x, grad_state, grad_gate), scan_grad_oracle(dh, states.cpu(), gate.cpu(), None, x.cpu(), None, True, None),
+                                    (torch.bfloat16, torch.float32, torch.float32)):
+        within(value, *oracle, dtype)
+    want, mag, n = lookup_grad_oracle(grad_x, ids, 700, 2.0)
+    within(grad_table, want, (n + 4).reshape(-1, 1) * u(torch.float32) * mag, torch.float32)
+
+
+@gpu
+def test_captured_graphs_replay_and_share_nothing():
+    steps = [_everything(1), _everything(2, 2500, 130)]
+    want = [[v.clone() for v in _chain(*s)] for s in steps]
+    graphs, outs, inputs = [], [], []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for s in steps:
+            _chain(*s)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for s in steps:
+        still = [torch.zeros_like(v) for v in s]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = _chain(*still)
+        graphs.append(graph)
+        outs.append(out)
+        inputs.append(still)
+    streams = [torch.cuda.Stream() for _ in steps]
+    for replay in range(4):
+        for k, s in enumerate(steps):
+            for dst, src in zip(inputs[k], s):
+                dst.copy_(src)
+        torch.cuda.synchronize()
+        for k in range(len(steps)):             # both at once
+            with torch.cuda.stream(streams[k]):
+                graphs[k].replay()
+        eager = _chain(*steps[replay % 2])
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(eager, want[replay % 2]))
+        for k in range(len(steps)):
+            assert all(torch.equal(p, q) for p, q in zip(outs[k], want[k])), (replay, k)
+            for v in outs[k]:
+                v.zero_()
+
+
+@gpu
+def test_two_streams_and_threads_at_once():
+    import threading
+    steps = [_everything(k, 400 + 37 * k, 64 + 32 * k) for k in range(4)]
+    want = [[v.clone() for v in _chain(*s)] for s in steps]
+    torch.cuda.synchronize()
+    got = [None] * len(steps)
+
+    def work(k):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(5):
+                got[k] = _chain(*steps[k])
+        stream.synchronize()
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(len(steps))]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    for a, b in zip(got, want):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@gpu
+def test_empty_tensors():
+    dev = "cuda"
+    assert ops.embedding(torch.ones((0, 4), device=dev), torch.tensor([0, 1], device=dev)).eq(0).all()
+    assert ops.embedding(torch.ones((3, 0), device=dev), torch.tensor([0, 1], device=dev)).shape == (2, 0)
+    assert ops.embedding_grad(torch.ones((0, 4), device=dev), torch.zeros(0, dtype=torch.int32, device=dev), 3).eq(0).all()
+    state = torch.full((2, 5), 3.0, device=dev)
+    states, last = ops.gated_scan(torch.ones((2, 0, 5), device=dev), torch.ones((2, 0, 5), device=dev), state)
+    assert states.shape == (2, 0, 5) and torch.equal(last, state)
+    gx, gs, gg = ops.gated_scan_grad(states, states, torch.ones((2, 0, 5), device=dev), state, grad_last=2 * state)
+    assert gx.shape == (2, 0, 5) and torch.equal(gs, 2 * state) and gg.shape == (2, 0, 5)
+    for shape in ((0, 7, 5), (2, 7, 0)):
+        x = torch.ones(shape, device=dev)
+        states, last = ops.gated_scan(x, torch.ones((1, 7, 1), device=dev), mix=True)
+        gx, gs, gg = ops.gated_scan_grad(x, states, torch.ones((1, 7, 1), device=dev), x=x, mix=True)
+        assert states.shape == gx.shape == shape and gg.shape == (1, 7, 1) and not gg.any()
+
+
+# -- refusals (no GPU needed: arguments are looked at first) ---------------------------------------------------------
+
+_X, _I = torch.ones((2, 3, 4)), torch.zeros(3, dtype=torch.int64)
+REFUSED = {
+    "table is no tensor": lambda: ops.embedding(np.ones((2, 3)), _I),
+    "table of whole numbers": lambda: ops.embedding(torch.ones((2, 3), dtype=torch.int32), _I),
+    "table of one dimension": lambda: ops.embedding(torch.ones(3), _I),
+    "ids of floats": lambda: ops.embedding(torch.ones((2, 3)), torch.zeros(3)),
+    "ids of bytes": lambda: ops.embedding(torch.ones((2, 3)), torch.zeros(3, dtype=torch.uint8)),
+    "table on the CPU": lambda: ops.embedding(torch.ones((2, 3)), _I),
+    "table with autograd": lambda: ops.embedding(torch.ones((2, 3), requires_grad=True), _I),
+    "gradient of another shape": lambda: ops.embedding_grad(torch.ones((4, 3)), _I, 5),
+    "gradient without a width": lambda: ops.embedding_grad(torch.ones(3), _I, 5),
+    "negative rows": lambda: ops.embedding_grad(torch.ones((3, 2)), _I, -1),
+    "too many rows": lambda: ops.embedding_grad(torch.ones((3, 2)), _I, 2**31),
+    "half a row": lambda: ops.embedding_grad(torch.ones((3, 2)), _I, 1.5),
+    "narrower result": lambda: ops.embedding_grad(torch.ones((3, 2)), _I, 5, dtype=torch.bfloat16),
+    "wider result": lambda: ops.embedding_grad(torch.ones((3, 2)), _I, 5, dtype=torch.float64),
+    "gradient on the CPU": lambda: ops.embedding_grad(torch.ones((3, 2)), _I, 5),
+    "x of two dimensions": lambda: ops.gated_scan(torch.ones((2, 3))),
+    "x of whole numbers": lambda: ops.gated_scan(_X.long()),
+    "gate of another batch": lambda: ops.gated_scan(_X, torch.ones((3, 3, 4))),
+    "gate of other steps": lambda: ops.gated_scan(_X, torch.ones((2, 2, 4))),
+    "gate of three groups": lambda: ops.gated_scan(_X, torch.ones((2, 3, 3))),
+    "gate without groups": lambda: ops.gated_scan(_X, torch.ones((2, 3, 0))),
+    "gate of two dimensions": lambda: ops.gated_scan(_X, torch.ones((2, 3))),
+    "gate of 64 bits": lambda: ops.gated_scan(_X, torch.ones((2, 3, 4), dtype=torch.float64)),
+    "gate of 16 bits": lambda: ops.gated_scan(_X, torch.ones((2, 3, 4), dtype=torch.bfloat16)),
+    "state of 16 bits": lambda: ops.gated_scan(_X.bfloat16(), None, torch.ones((2, 4), dtype=torch.bfloat16)),
+    "state of another shape": lambda: ops.gated_scan(_X, None, torch.ones((2, 3))),
+    "lengths of 64 bits": lambda: ops.gated_scan(_X, lengths=torch.ones(2, dtype=torch.int64)),
+    "lengths of another batch": lambda: ops.gated_scan(_X, lengths=torch.ones(3, dtype=torch.int32)),
+    "mixed form without a gate": lambda: ops.gated_scan(_X, mix=True),
+    "x on the CPU": lambda: ops.gated_scan(_X),
+    "x with autograd": lambda: ops.gated_scan(_X.clone().requires_grad_()),
+    "gradient of another type": lambda: ops.gated_scan_grad(_X.bfloat16(), _X),
+    "gradient of other steps": lambda: ops.gated_scan_grad(_X[:, :2], _X),
+    "x of another shape": lambda: ops.gated_scan_grad(_X, _X, torch.ones((2, 3, 4)), x=_X[:1], mix=True),
+    "mixed gradient without x": lambda: ops.gated_scan_grad(_X, _X, torch.ones((2, 3, 4)), mix=True),
+    "last gradient of another shape": lambda: ops.gated_scan_grad(_X, _X, grad_last=torch.ones((2, 3))),
+    "states on the CPU": lambda: ops.gated_scan_grad(_X, _X),
+}
+
+
+@pytest.mark.parametrize("what", REFUSED)
+def test_refused(what):
+    with pytest.raises(LightGBMError):
+        REFUSED[what]()
+
+
+@gpu
+def test_tensors_of_different_devices_are_refused():
+    with pytest.raises(LightGBMError, match="tensors on"):
+        ops.embedding(torch.ones((2, 3)).cuda(), _I)
+    with pytest.raises(LightGBMError, match="tensors on"):
+        ops.gated_scan(_X.cuda(), torch.ones((2, 3, 4)))

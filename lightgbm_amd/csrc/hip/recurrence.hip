@@ -3,6 +3,12 @@
 // and its gradients.  With e[t] = a[t] c[t] the gradient c[t] of h[t] follows the same recurrence backwards:
 //   c[t] = dh[t] + e[t+1],  e[t] = a[t] c[t];   dx = w c,  da = c (h[t-1] - (mixed) x),  dstate = e[0].
 // Behind a sequence's length the state is kept and nothing is read: whatever stands there cannot reach a result.
+//
+// A run of steps is an affine map h -> A h + H, and maps compose associatively: (A, H) after (A', H') is
+// (A A', A H' + H).  The steps are cut into chunks of kSteps that one lane holds in registers, kSlots chunks make a tile
+// (one workgroup, 64 channel packs wide).  A tile folds its chunks through LDS, hands its map to the tiles behind it
+// through memory, folds the maps before it, and then walks its chunks again from the exact state before each: every
+// value is read once and written once.  All folds run in the order of the steps, so results do not depend on timing.
 #include "recurrence.hpp"
 #include "device.hpp"
 #include "seq_types.hpp"
@@ -13,74 +19,365 @@ namespace lga {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kLanes = 64;          // channel packs of a tile
+constexpr int kSteps = 16;          // steps a lane holds
+constexpr int kMaxSlots = 8;        // chunks of a tile
+constexpr int kCheckpoint = 32;     // every 32nd tile hands on the state itself, so that no tile folds more than 31 maps
+constexpr uint64_t kEmpty = ~0ull;  // a word nobody has written yet: a NaN that publish() never stores
 
 enum GateKind { kNoGate, kOwnGate, kSharedGate };
 
-// One lane walks a sequence's channel through all steps.
-template <typename T, typename G, GateKind K>
-__global__ __launch_bounds__(kThreads) void scan_walk_kernel(ScanArgs a) {
-  typedef Wide<T> W;
-  const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (c >= a.batch * a.width) return;
-  const int64_t b = c / a.width, d = c - b * a.width;
-  const T* x = (const T*)a.x + b * a.x_b + d;
-  const G* gate = K == kNoGate ? nullptr : (const G*)a.gate + b * a.gate_b + d / (a.width / a.groups);
-  T* out = (T*)a.states + b * a.steps * a.width + d;
-  const int64_t len = a.lengths ? std::min<int64_t>(((const int32_t*)a.lengths)[b], a.steps) : a.steps;
-  W h = a.state ? ((const W*)a.state)[c] : (W)0;
-  int64_t t = 0;
-  for (; t < len; ++t) {
-    W v = (W)x[t * a.x_t];
-    if constexpr (K == kNoGate) {
-      h += v;
-    } else {
-      const W g = (W)gate[t * a.gate_t];
-      if (a.mix) v *= (W)1 - g;
-      h = fma_wide(g, h, v);
-    }
-    out[t * a.width] = (T)h;
-  }
-  for (; t < a.steps; ++t) out[t * a.width] = (T)(W)0;
-  ((W*)a.last)[c] = h;
+__device__ __forceinline__ float smallest(float) { return 1.40129846e-45f; }
+__device__ __forceinline__ double smallest(double) { return 4.9406564584124654e-324; }
+__device__ __forceinline__ float abs_of(float x) { return __builtin_fabsf(x); }
+__device__ __forceinline__ double abs_of(double x) { return __builtin_fabs(x); }
+__device__ __forceinline__ float sign_of(float m, float s) { return __builtin_copysignf(m, s); }
+__device__ __forceinline__ double sign_of(double m, double s) { return __builtin_copysign(m, s); }
+
+// A product of gates that has underflowed although none of them is zero stays just above zero: an infinite state must
+// come out of it as infinite as out of the single steps, not as 0 * inf = NaN.
+template <typename W> __device__ __forceinline__ W kept(W product, bool any_zero) {
+  return product == 0 && !any_zero ? sign_of(smallest(product), product) : product;
 }
 
-template <typename T, typename G, GateKind K>
-__global__ __launch_bounds__(kThreads) void scan_grad_walk_kernel(ScanGradArgs a) {
+template <typename W> struct Map { W a, h; };
+
+// `later` after `first`
+template <typename W> __device__ __forceinline__ Map<W> after(const Map<W>& later, const Map<W>& first) {
+  return {kept(later.a * first.a, later.a == 0 || first.a == 0), fma_wide(later.a, first.h, later.h)};
+}
+
+// Words that tiles hand to one another.  Each is written once, whole, and read with agent scope until it is there: the
+// value itself is the flag.
+__device__ __forceinline__ void put_word(uint64_t* p, uint64_t v) {
+  __hip_atomic_store(p, v == kEmpty ? 0x7ff8000000000000ull : v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t get_word(const uint64_t* p) {
+  uint64_t v;
+  while ((v = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) == kEmpty) __builtin_amdgcn_s_sleep(1);
+  return v;
+}
+// fp32: one word (a low, h high).  A NaN pair that reads as kEmpty becomes another NaN pair.
+__device__ __forceinline__ void publish(uint64_t* p, const Map<float>& m) {
+  const uint64_t v = (uint64_t)__float_as_uint(m.a) | (uint64_t)__float_as_uint(m.h) << 32;
+  __hip_atomic_store(p, v == kEmpty ? 0x7fc000007fc00000ull : v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void fetch(const uint64_t* p, Map<float>& m) {
+  const uint64_t v = get_word(p);
+  m.a = __uint_as_float((uint32_t)v);
+  m.h = __uint_as_float((uint32_t)(v >> 32));
+}
+// fp64: two words
+__device__ __forceinline__ void publish(uint64_t* p, const Map<double>& m) {
+  put_word(p, (uint64_t)__double_as_longlong(m.a));
+  put_word(p + 1, (uint64_t)__double_as_longlong(m.h));
+}
+__device__ __forceinline__ void fetch(const uint64_t* p, Map<double>& m) {
+  m.a = __longlong_as_double((int64_t)get_word(p));
+  m.h = __longlong_as_double((int64_t)get_word(p + 1));
+}
+template <typename W> constexpr int kMapWords = sizeof(W) / 4;
+
+__global__ __launch_bounds__(kThreads) void fill_words_kernel(uint64_t* __restrict__ p, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) p[i] = kEmpty;
+}
+
+// How the steps are cut, for both directions.  Channels are counted in packs of V over all sequences.
+struct Cut {
+  int64_t packs;      // batch * width / V
+  int64_t pack_rows;  // workgroups side by side: packs / lanes, rounded up
+  int64_t tiles;      // workgroups one behind the other
+  int lanes, slots;   // of a workgroup
+};
+
+// Workspace of a cut into several tiles, in words: [0] tickets, then the tiles' maps, then the checkpoints' states.
+template <typename W> __host__ __device__ inline int64_t map_words(const Cut& k, int v) { return k.tiles * k.pack_rows * k.lanes * v * kMapWords<W>; }
+template <typename W> inline int64_t work_words(const Cut& k, int v) {
+  return k.tiles < 2 ? 0 : 8 + map_words<W>(k, v) + (k.tiles / kCheckpoint + 1) * k.pack_rows * k.lanes * v * kMapWords<W>;
+}
+
+// Which tile a workgroup is.  Several tiles: by ticket, in the order in which workgroups really start, so that whatever a
+// tile waits for belongs to a workgroup that already runs (and waits for earlier ones only).
+__device__ __forceinline__ void take_tile(const Cut& k, uint64_t* work, int64_t& tile, int64_t& row) {
+  int64_t ticket = blockIdx.x;
+  if (k.tiles > 1) {
+    __shared__ uint32_t taken;
+    if (threadIdx.x == 0) taken = __hip_atomic_fetch_add((uint32_t*)work, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;   // starts at 2^32 - 1
+    __syncthreads();
+    ticket = taken;
+  }
+  tile = ticket / k.pack_rows;
+  row = ticket - tile * k.pack_rows;
+}
+
+// The state before this lane's chunk, given the chunk's own map.  `first`: the state before the first tile.
+// Returns it in `carry`.
+template <typename W, int V>
+__device__ __forceinline__ void carry_in(const Cut& k, uint64_t* work, int64_t tile, int64_t row, int lane, int slot, const Map<W> (&own)[V], const W (&first)[V],
+                                         W (&carry)[V]) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  Map<W>(*maps)[V] = (Map<W>(*)[V])lds;                       // [slots][lanes]
+  Map<W>(*parts)[V] = maps + k.slots * k.lanes;               // partial folds of the tiles before this one
+  const int at = slot * k.lanes + lane;
+  for (int v = 0; v < V; ++v) maps[at][v] = own[v];
+  __syncthreads();
+  Map<W> mine[V];                                             // the chunks of this tile before this one
+  for (int v = 0; v < V; ++v) mine[v] = {1, 0};
+  for (int s = 0; s < slot; ++s)
+    for (int v = 0; v < V; ++v) mine[v] = after(maps[s * k.lanes + lane][v], mine[v]);
+  for (int v = 0; v < V; ++v) carry[v] = first[v];
+  if (k.tiles > 1) {
+    const int64_t stride = k.pack_rows * k.lanes * V * kMapWords<W>;
+    uint64_t* tile_maps = work + 8 + (row * k.lanes + lane) * V * kMapWords<W>;
+    uint64_t* checkpoints = tile_maps + k.tiles * stride;
+    if (slot == k.slots - 1 && tile + 1 < k.tiles)
+      for (int v = 0; v < V; ++v) publish(tile_maps + tile * stride + v * kMapWords<W>, after(own[v], mine[v]));
+    const int64_t from = tile / kCheckpoint * kCheckpoint;    // first tile behind the last checkpoint
+    const int before = (int)(tile - from), share = (before + k.slots - 1) / k.slots;
+    Map<W> part[V];
+    for (int v = 0; v < V; ++v) part[v] = {1, 0};
+    for (int p = slot * share; p < min(before, (slot + 1) * share); ++p)
+      for (int v = 0; v < V; ++v) {
+        Map<W> m;
+        fetch(tile_maps + (from + p) * stride + v * kMapWords<W>, m);
+        part[v] = after(m, part[v]);
+      }
+    for (int v = 0; v < V; ++v) parts[at][v] = part[v];
+    if (from > 0)
+      for (int v = 0; v < V; ++v) {
+        Map<W> m;
+        fetch(checkpoints + (from / kCheckpoint - 1) * stride + v * kMapWords<W>, m);
+        carry[v] = m.h;
+      }
+    __syncthreads();
+    if (before)
+      for (int s = 0; s * share < before; ++s)
+        for (int v = 0; v < V; ++v) {
+          const Map<W> m = parts[s * k.lanes + lane][v];
+          carry[v] = fma_wide(m.a, carry[v], m.h);
+        }
+    if (slot == k.slots - 1 && (tile + 1) % kCheckpoint == 0 && tile + 1 < k.tiles)
+      for (int v = 0; v < V; ++v) {
+        const Map<W> m = after(own[v], mine[v]);
+        publish(checkpoints + tile / kCheckpoint * stride + v * kMapWords<W>, Map<W>{0, fma_wide(m.a, carry[v], m.h)});
+      }
+  }
+  for (int v = 0; v < V; ++v) carry[v] = fma_wide(mine[v].a, carry[v], mine[v].h);
+}
+
+template <typename G, GateKind K, int V> struct GateRow {
+  const G* base = nullptr;
+  int64_t step = 0;
+  int64_t group[V];
+  __device__ __forceinline__ GateRow(int64_t gate, int64_t b, int64_t gate_b, int64_t gate_t, int64_t d, int64_t per) {
+    if constexpr (K != kNoGate) {
+      base = (const G*)gate + b * gate_b + (K == kOwnGate ? d : 0);
+      step = gate_t;
+      for (int v = 0; v < V; ++v) group[v] = K == kSharedGate ? (d + v) / per : v;
+    }
+  }
+  __device__ __forceinline__ Pack<G, V> load(int64_t t) const {
+    Pack<G, V> g;
+    if constexpr (K == kOwnGate) g = load_pack<G, V>(base + t * step);
+    else if constexpr (K == kSharedGate)
+      for (int v = 0; v < V; ++v) g.v[v] = base[t * step + group[v]];
+    return g;
+  }
+};
+
+template <typename T, int V> __device__ __forceinline__ Pack<T, V> constant(float x) {
+  Pack<T, V> p;
+  for (int v = 0; v < V; ++v) p.v[v] = (T)x;
+  return p;
+}
+
+__device__ __forceinline__ int64_t length_of(int64_t lengths, int64_t b, int64_t steps) {
+  if (!lengths) return steps;
+  return max((int64_t)0, min((int64_t)((const int32_t*)lengths)[b], steps));
+}
+
+template <typename T, typename G, GateKind K, int V, int L>
+__global__ __launch_bounds__(kLanes* kMaxSlots) void scan_kernel(ScanArgs a, Cut k) {
   typedef Wide<T> W;
-  const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (c >= a.batch * a.width) return;
-  const int64_t b = c / a.width, d = c - b * a.width;
+  int64_t tile, row;
+  take_tile(k, (uint64_t*)a.work, tile, row);
+  const int lane = threadIdx.x % k.lanes, slot = threadIdx.x / k.lanes;
+  const int64_t pack = row * k.lanes + lane;
+  const bool live = pack < k.packs;
+  const int64_t c = live ? pack * V : 0, b = c / a.width, d = c - b * a.width;
+  const int64_t t0 = (tile * k.slots + slot) * L, len = live ? length_of(a.lengths, b, a.steps) : 0;
+  const T* x = (const T*)a.x + b * a.x_b + d;
+  const GateRow<G, K, V> gate(a.gate, b, a.gate_b, a.gate_t, d, K == kSharedGate ? a.width / a.groups : 1);
+  Pack<T, V> xs[L];
+  Pack<G, V> gs[L];
+  if (__all(t0 + L <= len)) {
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+      xs[j] = load_pack<T, V>(x + (t0 + j) * a.x_t);
+      gs[j] = gate.load(t0 + j);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+      xs[j] = constant<T, V>(0);
+      gs[j] = constant<G, V>(1);
+      if (t0 + j < len) {
+        xs[j] = load_pack<T, V>(x + (t0 + j) * a.x_t);
+        gs[j] = gate.load(t0 + j);
+      }
+    }
+  }
+  W h[V], first[V];
+  for (int v = 0; v < V; ++v) first[v] = a.state && live ? ((const W*)a.state)[c + v] : (W)0;
+  if (k.tiles > 1 || k.slots > 1) {
+    Map<W> own[V];
+    W least[V];
+    for (int v = 0; v < V; ++v) own[v] = {1, 0}, least[v] = 1;
+#pragma unroll
+    for (int j = 0; j < L; ++j)
+      for (int v = 0; v < V; ++v) {
+        W in = (W)xs[j].v[v];
+        if constexpr (K == kNoGate) {
+          own[v].h += in;
+        } else {
+          const W g = (W)gs[j].v[v];
+          if (a.mix) in *= (W)1 - g;
+          own[v].h = fma_wide(g, own[v].h, in);
+          own[v].a *= g;
+          least[v] = min(least[v], abs_of(g));
+        }
+      }
+    for (int v = 0; v < V; ++v) own[v].a = kept(own[v].a, least[v] == 0);
+    carry_in<W, V>(k, (uint64_t*)a.work, tile, row, lane, slot, own, first, h);
+  } else {
+    for (int v = 0; v < V; ++v) h[v] = first[v];
+  }
+  if (!live) return;
+  T* out = (T*)a.states + b * a.steps * a.width + d;
+#pragma unroll
+  for (int j = 0; j < L; ++j) {
+    const int64_t t = t0 + j;
+    Pack<T, V> o;
+    for (int v = 0; v < V; ++v) {
+      W in = (W)xs[j].v[v];
+      if constexpr (K == kNoGate) {
+        h[v] += in;
+      } else {
+        const W g = (W)gs[j].v[v];
+        if (a.mix) in *= (W)1 - g;
+        h[v] = fma_wide(g, h[v], in);
+      }
+      o.v[v] = t < len ? (T)h[v] : (T)(W)0;
+    }
+    if (t < a.steps) store_pack<T, V>(out + t * a.width, o);
+  }
+  if (tile == k.tiles - 1 && slot == k.slots - 1)
+    for (int v = 0; v < V; ++v) ((W*)a.last)[c + v] = h[v];
+}
+
+// Backwards: step r of a chunk is step steps - 1 - r of the sequence.
+template <typename T, typename G, GateKind K, int V, int L>
+__global__ __launch_bounds__(kLanes* kMaxSlots) void scan_grad_kernel(ScanGradArgs a, Cut k, uint64_t* work, int64_t slopes) {
+  typedef Wide<T> W;
+  int64_t tile, row;
+  take_tile(k, work, tile, row);
+  const int lane = threadIdx.x % k.lanes, slot = threadIdx.x / k.lanes;
+  const int64_t pack = row * k.lanes + lane;
+  const bool live = pack < k.packs;
+  const int64_t c = live ? pack * V : 0, b = c / a.width, d = c - b * a.width;
+  const int64_t t0 = a.steps - 1 - (tile * k.slots + slot) * L, len = live ? length_of(a.lengths, b, a.steps) : 0;
   const T* dh = (const T*)a.grad_states + b * a.g_b + d;
   const T* hs = (const T*)a.states + b * a.h_b + d;
-  const T* x = a.mix ? (const T*)a.x + b * a.x_b + d : nullptr;
-  const G* gate = K == kNoGate ? nullptr : (const G*)a.gate + b * a.gate_b + d / (a.width / a.groups);
-  T* dx = (T*)a.grad_x + b * a.steps * a.width + d;
-  W* slope = (W*)a.work + b * a.steps * a.width + d;        // the gate's gradient, value by value
-  const int64_t len = a.lengths ? std::max<int64_t>(0, std::min<int64_t>(((const int32_t*)a.lengths)[b], a.steps)) : a.steps;
-  W e = a.grad_last ? ((const W*)a.grad_last)[c] : (W)0;
-  int64_t t = a.steps;
-  for (; t > len; --t) {
-    dx[(t - 1) * a.width] = (T)(W)0;
-    if (K != kNoGate) slope[(t - 1) * a.width] = 0;
-  }
-  for (; t > 0; --t) {
-    const W cc = (W)dh[(t - 1) * a.g_t] + e;
-    W v = cc;
-    if constexpr (K == kNoGate) {
-      e = cc;
-    } else {
-      const W g = (W)gate[(t - 1) * a.gate_t];
-      W before = t > 1 ? (W)hs[(t - 2) * a.h_t] : (a.state ? ((const W*)a.state)[c] : (W)0);
-      if (a.mix) {
-        before -= (W)x[(t - 1) * a.x_t];
-        v *= (W)1 - g;
+  const T* x = (const T*)a.x + b * a.x_b + d;
+  const GateRow<G, K, V> gate(a.gate, b, a.gate_b, a.gate_t, d, K == kSharedGate ? a.width / a.groups : 1);
+  Pack<T, V> gs[L], before[L], xs[L];
+  Pack<G, V> as[L];
+  if (__all(t0 < len && t0 - L >= 0)) {
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+      gs[j] = load_pack<T, V>(dh + (t0 - j) * a.g_t);
+      as[j] = gate.load(t0 - j);
+      if constexpr (K != kNoGate) {
+        before[j] = load_pack<T, V>(hs + (t0 - j - 1) * a.h_t);
+        if (a.mix) xs[j] = load_pack<T, V>(x + (t0 - j) * a.x_t);
       }
-      slope[(t - 1) * a.width] = cc * before;
-      e = g * cc;
     }
-    dx[(t - 1) * a.width] = (T)v;
+  } else {
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+      const int64_t t = t0 - j;
+      gs[j] = before[j] = xs[j] = constant<T, V>(0);
+      as[j] = constant<G, V>(1);
+      if (t >= 0 && t < len) {
+        gs[j] = load_pack<T, V>(dh + t * a.g_t);
+        as[j] = gate.load(t);
+        if constexpr (K != kNoGate) {
+          if (t > 0) before[j] = load_pack<T, V>(hs + (t - 1) * a.h_t);
+          if (a.mix) xs[j] = load_pack<T, V>(x + t * a.x_t);
+        }
+      }
+    }
   }
-  ((W*)a.grad_state)[c] = e;
+  W e[V], first[V];
+  for (int v = 0; v < V; ++v) first[v] = a.grad_last && live ? ((const W*)a.grad_last)[c + v] : (W)0;
+  if (k.tiles > 1 || k.slots > 1) {
+    Map<W> own[V];
+    W least[V];
+    for (int v = 0; v < V; ++v) own[v] = {1, 0}, least[v] = 1;
+#pragma unroll
+    for (int j = 0; j < L; ++j)
+      for (int v = 0; v < V; ++v) {
+        own[v].h += (W)gs[j].v[v];
+        if constexpr (K != kNoGate) {
+          const W g = (W)as[j].v[v];
+          own[v].h *= g;
+          own[v].a *= g;
+          least[v] = min(least[v], abs_of(g));
+        }
+      }
+    for (int v = 0; v < V; ++v) own[v].a = kept(own[v].a, least[v] == 0);
+    carry_in<W, V>(k, work, tile, row, lane, slot, own, first, e);
+  } else {
+    for (int v = 0; v < V; ++v) e[v] = first[v];
+  }
+  if (!live) return;
+  T* dx = (T*)a.grad_x + b * a.steps * a.width + d;
+  G* da = (G*)a.grad_gate + b * a.steps * a.width + d;
+  W* slope = (W*)slopes + b * a.steps * a.width + d;
+#pragma unroll
+  for (int j = 0; j < L; ++j) {
+    const int64_t t = t0 - j;
+    Pack<T, V> o;
+    Pack<G, V> og;
+    Pack<W, V> os;
+    for (int v = 0; v < V; ++v) {
+      const W cc = (W)gs[j].v[v] + e[v];
+      W value = cc;
+      if constexpr (K == kNoGate) {
+        e[v] = cc;
+      } else {
+        const W g = (W)as[j].v[v];
+        W from = t == 0 ? (a.state ? ((const W*)a.state)[c + v] : (W)0) : (W)before[j].v[v];
+        if (a.mix) {
+          from -= (W)xs[j].v[v];
+          value *= (W)1 - g;
+        }
+        os.v[v] = t < len ? cc * from : (W)0;
+        og.v[v] = (G)os.v[v];
+        e[v] = g * cc;
+      }
+      o.v[v] = t < len ? (T)value : (T)(W)0;
+    }
+    if (t >= 0) {
+      store_pack<T, V>(dx + t * a.width, o);
+      if constexpr (K != kNoGate) {
+        if (slopes) store_pack<W, V>(slope + t * a.width, os);
+        else store_pack<G, V>(da + t * a.width, og);
+      }
+    }
+  }
+  if (tile == k.tiles - 1 && slot == k.slots - 1)
+    for (int v = 0; v < V; ++v) ((W*)a.grad_state)[c + v] = e[v];
 }
 
 // grad_gate[q][t][g] = sum of the slopes of the sequences and channels that share the gate, in a fixed order:
@@ -108,41 +405,43 @@ __global__ __launch_bounds__(kThreads) void gate_sum_kernel(const W* __restrict_
   }
 }
 
-unsigned lanes(int64_t n) { return (unsigned)((n + kThreads - 1) / kThreads); }
+bool aligned(int64_t address, int64_t bytes) { return address % bytes == 0; }
 
-template <typename T, typename G> void run_scan(const ScanArgs& a) {
-  const dim3 grid(lanes(a.batch * a.width)), block(kThreads);
-  const hipStream_t s = (hipStream_t)a.stream;
-  if (!a.gate) hipLaunchKernelGGL((scan_walk_kernel<T, G, kNoGate>), grid, block, 0, s, a);
-  else if (a.groups == a.width) hipLaunchKernelGGL((scan_walk_kernel<T, G, kOwnGate>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((scan_walk_kernel<T, G, kSharedGate>), grid, block, 0, s, a);
-  LGA_HIP_CHECK(hipGetLastError());
+// Two channels a lane where every row of every tensor starts at a multiple of both.
+template <typename A> bool even_rows(const A& a) {
+  const int64_t size = a.type == kF64 ? 8 : a.type == kF32 ? 4 : 2, gate = a.gate_type == kF64 ? 8 : a.gate_type == kF32 ? 4 : 2;
+  if (a.type == kF64 || a.width % 2 || a.x_b % 2 || a.x_t % 2 || !aligned(a.x, 2 * size)) return false;
+  return !a.gate || a.groups != a.width || (a.gate_b % 2 == 0 && a.gate_t % 2 == 0 && aligned(a.gate, 2 * gate));
+}
+bool two_wide(const ScanArgs& a) { return even_rows(a); }
+bool two_wide(const ScanGradArgs& a) {
+  const int64_t size = a.type == kF32 ? 8 : 4;
+  return even_rows(a) && a.g_b % 2 == 0 && a.g_t % 2 == 0 && a.h_b % 2 == 0 && a.h_t % 2 == 0 && aligned(a.grad_states, size) && aligned(a.states, size);
 }
 
-template <typename T, typename G> void run_scan_grad(const ScanGradArgs& a) {
-  typedef Wide<T> W;
-  const dim3 grid(lanes(a.batch * a.width)), block(kThreads);
-  const hipStream_t s = (hipStream_t)a.stream;
-  if (!a.gate) hipLaunchKernelGGL((scan_grad_walk_kernel<T, G, kNoGate>), grid, block, 0, s, a);
-  else if (a.groups == a.width) hipLaunchKernelGGL((scan_grad_walk_kernel<T, G, kOwnGate>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((scan_grad_walk_kernel<T, G, kSharedGate>), grid, block, 0, s, a);
-  LGA_HIP_CHECK(hipGetLastError());
-  if (a.gate && a.steps) {
-    const int64_t sums = a.gate_batch * a.steps * a.groups;
-    hipLaunchKernelGGL((gate_sum_kernel<W, G>), dim3((unsigned)std::min<int64_t>(sums, 1 << 20)), block, 0, s, (const W*)a.work, (G*)a.grad_gate,
-                       a.batch, a.steps, a.width, a.groups, a.gate_batch);
-    LGA_HIP_CHECK(hipGetLastError());
-  }
+Cut cut_steps(int64_t batch, int64_t steps, int64_t width, int v, int per_lane) {
+  Cut k;
+  k.packs = batch * width / v;
+  k.lanes = kLanes;
+  while (k.lanes > 1 && k.lanes / 2 >= k.packs) k.lanes /= 2;
+  const int64_t chunks = std::max<int64_t>(1, (steps + per_lane - 1) / per_lane);
+  k.slots = 1;
+  while (k.slots < kMaxSlots && k.slots < chunks) k.slots *= 2;
+  k.tiles = (chunks + k.slots - 1) / k.slots;
+  if (k.tiles == 1 && k.slots == 1) k.lanes = k.packs >= kThreads ? kThreads : k.lanes;
+  k.pack_rows = (k.packs + k.lanes - 1) / k.lanes;
+  if (k.tiles * k.pack_rows > 2147483647LL) throw std::runtime_error("gated_scan: the tensor is too large");
+  return k;
 }
 
 template <typename A> void check_args(const A& a) {
   if (a.batch < 0 || a.steps < 0 || a.width < 0) throw std::runtime_error("gated_scan: a negative size");
-  if (a.batch * a.width > 2147483647LL * 64 || a.steps > 2147483647LL) throw std::runtime_error("gated_scan: the tensor is too large");
+  if (a.steps > 2147483647LL) throw std::runtime_error("gated_scan: the tensor is too large");
   if (a.gate && (a.groups <= 0 || a.width % a.groups)) throw std::runtime_error("gated_scan: the width is not a multiple of the gate's groups");
 }
 
 // type and gate_type -> template arguments
-template <typename F> void by_types(int64_t type, int64_t gate_type, bool gate, F f) {
+template <typename F> auto by_types(int64_t type, int64_t gate_type, bool gate, F f) {
   if (!gate) gate_type = type;
   if (type == kBf16 && gate_type == kBf16) return f((__bf16)0, (__bf16)0);
   if (type == kBf16 && gate_type == kF32) return f((__bf16)0, (float)0);
@@ -153,26 +452,93 @@ template <typename F> void by_types(int64_t type, int64_t gate_type, bool gate, 
   throw std::runtime_error("gated_scan: unknown pair of types");
 }
 
+template <int N> struct Const { static constexpr int value = N; };
+
+// f(gate kind, channels a lane, steps a lane)
+template <bool Two, typename A, typename F> void by_shape(const A& a, F f) {
+  auto with_kind = [&](auto kind) {
+    if constexpr (Two) {
+      if (two_wide(a)) return a.steps <= 1 ? f(kind, Const<2>(), Const<1>()) : f(kind, Const<2>(), Const<kSteps>());
+    }
+    return a.steps <= 1 ? f(kind, Const<1>(), Const<1>()) : f(kind, Const<1>(), Const<kSteps>());
+  };
+  if (!a.gate) with_kind(Const<kNoGate>());
+  else if (a.groups == a.width) with_kind(Const<kOwnGate>());
+  else with_kind(Const<kSharedGate>());
+}
+
+template <typename W> size_t fold_bytes(const Cut& k, int v) { return k.tiles * k.slots == 1 ? 0 : 2 * k.slots * k.lanes * v * sizeof(Map<W>); }
+
+template <typename W> void clear_work(const Cut& k, int v, uint64_t* work, hipStream_t s) {
+  const int64_t n = work_words<W>(k, v);
+  if (!n) return;
+  hipLaunchKernelGGL(fill_words_kernel, dim3((unsigned)std::min<int64_t>((n + kThreads - 1) / kThreads, 2048)), dim3(kThreads), 0, s, work, n);
+  LGA_HIP_CHECK(hipGetLastError());
+}
+
+bool sums_gates(const ScanGradArgs& a) { return a.gate && (a.groups != a.width || a.gate_batch != a.batch); }
+
 }  // namespace
 
-int64_t scan_workspace(const ScanArgs& a) { return 0; }
+int64_t scan_workspace(const ScanArgs& a) {
+  check_args(a);
+  const int v = two_wide(a) ? 2 : 1;
+  const Cut k = cut_steps(a.batch, a.steps, a.width, v, a.steps <= 1 ? 1 : kSteps);
+  return 8 * (a.type == kF64 ? work_words<double>(k, v) : work_words<float>(k, v));
+}
 
 void gated_scan(const ScanArgs& a) {
   check_args(a);
   if (a.batch * a.width == 0) return;
   DeviceScope scope(a.device);
-  by_types(a.type, a.gate_type, a.gate != 0, [&](auto t, auto g) { run_scan<decltype(t), decltype(g)>(a); });
+  by_types(a.type, a.gate_type, a.gate != 0, [&](auto tt, auto gg) {
+    typedef decltype(tt) T;
+    typedef decltype(gg) G;
+    by_shape<sizeof(T) < 8>(a, [&](auto kind, auto v, auto l) {
+      constexpr int V = decltype(v)::value, L = decltype(l)::value;
+      const Cut k = cut_steps(a.batch, a.steps, a.width, V, L);
+      clear_work<Wide<T>>(k, V, (uint64_t*)a.work, (hipStream_t)a.stream);
+      hipLaunchKernelGGL((scan_kernel<T, G, (GateKind)decltype(kind)::value, V, L>), dim3((unsigned)(k.tiles * k.pack_rows)), dim3(k.lanes * k.slots),
+                         fold_bytes<Wide<T>>(k, V), (hipStream_t)a.stream, a, k);
+      LGA_HIP_CHECK(hipGetLastError());
+    });
+  });
 }
 
 int64_t scan_grad_workspace(const ScanGradArgs& a) {
-  return a.gate ? a.batch * a.steps * a.width * (a.type == kF64 ? 8 : 4) : 0;
+  check_args(a);
+  const int v = two_wide(a) ? 2 : 1;
+  const Cut k = cut_steps(a.batch, a.steps, a.width, v, a.steps <= 1 ? 1 : kSteps);
+  const int64_t slopes = sums_gates(a) ? a.batch * a.steps * a.width * (a.type == kF64 ? 8 : 4) : 0;
+  return 8 * (a.type == kF64 ? work_words<double>(k, v) : work_words<float>(k, v)) + slopes;
 }
 
 void gated_scan_grad(const ScanGradArgs& a) {
   check_args(a);
   if (a.batch * a.width == 0) return;
   DeviceScope scope(a.device);
-  by_types(a.type, a.gate_type, a.gate != 0, [&](auto t, auto g) { run_scan_grad<decltype(t), decltype(g)>(a); });
+  by_types(a.type, a.gate_type, a.gate != 0, [&](auto tt, auto gg) {
+    typedef decltype(tt) T;
+    typedef decltype(gg) G;
+    typedef Wide<T> W;
+    const hipStream_t s = (hipStream_t)a.stream;
+    by_shape<sizeof(T) < 8>(a, [&](auto kind, auto v, auto l) {
+      constexpr int V = decltype(v)::value, L = decltype(l)::value;
+      const Cut k = cut_steps(a.batch, a.steps, a.width, V, L);
+      uint64_t* work = (uint64_t*)a.work;
+      clear_work<W>(k, V, work, s);
+      const int64_t slopes = sums_gates(a) ? (int64_t)(work + work_words<W>(k, V)) : 0;
+      hipLaunchKernelGGL((scan_grad_kernel<T, G, (GateKind)decltype(kind)::value, V, L>), dim3((unsigned)(k.tiles * k.pack_rows)), dim3(k.lanes * k.slots),
+                         fold_bytes<W>(k, V), s, a, k, work, slopes);
+      LGA_HIP_CHECK(hipGetLastError());
+      if (slopes) {
+        const int64_t sums = a.gate_batch * a.steps * a.groups;
+        hipLaunchKernelGGL((gate_sum_kernel<W, G>), dim3((unsigned)std::min<int64_t>(sums, 1 << 20)), dim3(kThreads), 0, s, (const W*)slopes, (G*)a.grad_gate,
+                           a.batch, a.steps, a.width, a.groups, a.gate_batch);
+        LGA_HIP_CHECK(hipGetLastError());
+      }
+    });
+  });
 }
 
 }  // namespace lga

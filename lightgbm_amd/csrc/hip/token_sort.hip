@@ -1,0 +1,268 @@
+// Stable radix sort of tokens by id.  A pass counts the digits of every tile (LDS counters), turns the counts into the
+// places where a tile's runs begin, and scatters: a wave ranks its keys digit by digit with ballots (lanes of one digit
+// find each other in `bits` of them), the tile is put in order in LDS and written out run by run.  Integers only, so the
+// order never depends on timing.
+#include "token_sort.hpp"
+#include "device.hpp"
+#include <algorithm>
+
+namespace lga {
+
+namespace {
+
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kItems = kSortTile / kThreads;    // keys a lane holds
+constexpr int kMaxBits = 8, kBins = 1 << kMaxBits;
+
+struct Pass {
+  TokenGrid grid;
+  TokenTiles tiles;
+  const uint32_t* keys_in;      // null: first pass, keys come from the grid
+  const void* payload_in;
+  int64_t v0, v1;               // first pass: payload (i, j) is at i * v0 + j * v1; payload_in null: the token's number
+  int shift, bits;
+};
+
+__device__ __forceinline__ uint32_t grid_key(const TokenGrid& g, int64_t i, int64_t j) {
+  if (i >= g.n0 || j >= g.n1) return (uint32_t)g.rows;
+  const int64_t at = i * g.s0 + j * g.s1;
+  const int64_t id = g.ids64 ? ((const int64_t*)g.ids)[at] : (int64_t)((const int32_t*)g.ids)[at];
+  return id >= 0 && id < g.rows ? (uint32_t)id : (uint32_t)g.rows;
+}
+
+// Item q of tile b is token (i, j) with j running fastest.
+__device__ __forceinline__ void item_place(const Pass& p, int64_t b, int q, int64_t& i, int64_t& j) {
+  const int64_t ti = b / p.tiles.across, tj = b - ti * p.tiles.across;
+  i = ti * (kSortTile >> p.tiles.shift1) + (q >> p.tiles.shift1);
+  j = (tj << p.tiles.shift1) + (q & ((1 << p.tiles.shift1) - 1));
+}
+// The same items walked along the axis on which ids are neighbours: returns the item number.
+__device__ __forceinline__ int ids_order(const Pass& p, int n) {
+  if (p.grid.s1 <= p.grid.s0 || p.tiles.shift1 == 12) return n;
+  const int shift0 = 12 - p.tiles.shift1;
+  return ((n & ((1 << shift0) - 1)) << p.tiles.shift1) | (n >> shift0);
+}
+
+__global__ __launch_bounds__(kThreads) void sort_count_kernel(Pass p, uint32_t* __restrict__ counts) {
+  __shared__ uint32_t bin[kBins];
+  const int64_t b = blockIdx.x;
+  for (int d = threadIdx.x; d < kBins; d += kThreads) bin[d] = 0;
+  __syncthreads();
+  const uint32_t mask = (1u << p.bits) - 1;
+#pragma unroll 4
+  for (int k = 0; k < kItems; ++k) {
+    const int n = k * kThreads + threadIdx.x;
+    uint32_t key;
+    if (p.keys_in) {
+      key = p.keys_in[b * kSortTile + n];
+    } else {
+      int64_t i, j;
+      item_place(p, b, ids_order(p, n), i, j);
+      key = grid_key(p.grid, i, j);
+    }
+    atomicAdd(&bin[(key >> p.shift) & mask], 1u);
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < (1 << p.bits); d += kThreads) counts[(int64_t)d * p.tiles.blocks + b] = bin[d];
+}
+
+// Counts of one digit over the tiles -> where each tile's run of that digit begins among all of that digit; their sum.
+__global__ __launch_bounds__(kThreads) void sort_offsets_kernel(uint32_t* __restrict__ counts, uint32_t* __restrict__ totals, int64_t blocks) {
+  __shared__ uint32_t wave_sum[kWaves];
+  uint32_t* row = counts + (int64_t)blockIdx.x * blocks;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t before = 0;
+  for (int64_t base = 0; base < blocks; base += kThreads * 4) {
+    uint32_t v[4], sum = 0;
+    for (int k = 0; k < 4; ++k) {
+      const int64_t at = base + threadIdx.x * 4 + k;
+      v[k] = at < blocks ? row[at] : 0;
+      sum += v[k];
+    }
+    uint32_t scan = sum;
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t o = __shfl_up(scan, d);
+      if (lane >= d) scan += o;
+    }
+    if (lane == 63) wave_sum[wave] = scan;
+    __syncthreads();
+    uint32_t at = before + scan - sum, all = 0;
+    for (int w = 0; w < kWaves; ++w) {
+      if (w < wave) at += wave_sum[w];
+      all += wave_sum[w];
+    }
+    for (int k = 0; k < 4; ++k) {
+      const int64_t i = base + threadIdx.x * 4 + k;
+      if (i < blocks) row[i] = at;
+      at += v[k];
+    }
+    before += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) totals[blockIdx.x] = before;
+}
+
+// P: what is carried with a key (uint32 or uint64 words).
+template <typename P>
+__global__ __launch_bounds__(kThreads) void sort_scatter_kernel(Pass p, const uint32_t* __restrict__ offsets, const uint32_t* __restrict__ totals,
+                                                                uint32_t* __restrict__ keys_out, P* __restrict__ payload_out) {
+  __shared__ uint32_t skey[kSortTile];
+  __shared__ P spay[kSortTile];
+  __shared__ uint32_t count[kWaves][kBins];     // keys of a digit in a wave, then those in the waves before
+  __shared__ uint32_t local[kBins], global[kBins], wave_sum[kWaves][2];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int64_t b = blockIdx.x;
+  const uint32_t mask = (1u << p.bits) - 1;
+  uint32_t key[kItems], rank[kItems];
+  P pay[kItems];
+  for (int d = t; d < kWaves * kBins; d += kThreads) (&count[0][0])[d] = 0;
+  if (!p.keys_in) {
+    for (int k = 0; k < kItems; ++k) {
+      const int q = ids_order(p, k * kThreads + t);
+      int64_t i, j;
+      item_place(p, b, q, i, j);
+      skey[q] = grid_key(p.grid, i, j);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const int q = wave * (kSortTile / kWaves) + k * 64 + lane;
+    if (p.keys_in) {
+      key[k] = p.keys_in[b * kSortTile + q];
+      pay[k] = ((const P*)p.payload_in)[b * kSortTile + q];
+    } else {
+      key[k] = skey[q];
+      int64_t i, j;
+      item_place(p, b, q, i, j);
+      if (!p.payload_in) pay[k] = (P)(i * p.grid.n1 + j);
+      else pay[k] = key[k] < (uint32_t)p.grid.rows ? ((const P*)p.payload_in)[i * p.v0 + j * p.v1] : (P)0;
+    }
+  }
+  // ranks among the wave's keys of the same digit
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const uint32_t digit = (key[k] >> p.shift) & mask;
+    uint64_t same = ~0ull;
+    for (int bit = 0; bit < p.bits; ++bit) {
+      const bool one = (digit >> bit) & 1;
+      const uint64_t ones = __ballot(one);
+      same &= one ? ones : ~ones;
+    }
+    volatile uint32_t* const mine = &count[wave][digit];     // other lanes of the wave write it between two keys
+    const uint32_t before = *mine;
+    const int lower = __popcll(same & ((1ull << lane) - 1));
+    rank[k] = before + (uint32_t)lower;
+    if (lower == 0) *mine = before + (uint32_t)__popcll(same);
+  }
+  __syncthreads();
+  // one lane a digit: keys of the digit in the waves before, in the tile, in the digits below (of the tile and of all)
+  {
+    uint32_t in_tile = 0;
+    for (int w = 0; w < kWaves; ++w) {
+      const uint32_t c = count[w][t];
+      count[w][t] = in_tile;
+      in_tile += c;
+    }
+    const uint32_t total = t < (1 << p.bits) ? totals[t] : 0u;
+    uint32_t a = in_tile, g = total;
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t oa = __shfl_up(a, d), og = __shfl_up(g, d);
+      if (lane >= d) a += oa, g += og;
+    }
+    if (lane == 63) wave_sum[wave][0] = a, wave_sum[wave][1] = g;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) a += wave_sum[w][0], g += wave_sum[w][1];
+    local[t] = a - in_tile;
+    global[t] = t < (1 << p.bits) ? g - total + offsets[(int64_t)t * p.tiles.blocks + b] : 0u;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const uint32_t digit = (key[k] >> p.shift) & mask;
+    const uint32_t at = local[digit] + count[wave][digit] + rank[k];
+    skey[at] = key[k];
+    spay[at] = pay[k];
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int k = 0; k < kItems; ++k) {
+    const uint32_t n = k * kThreads + t, ky = skey[n], digit = (ky >> p.shift) & mask;
+    const uint32_t to = global[digit] + n - local[digit];
+    keys_out[to] = ky;
+    payload_out[to] = spay[n];
+  }
+}
+
+static_assert(kBins == kThreads, "one lane a digit");
+
+int bit_length(int64_t v) {
+  int n = 0;
+  while (v > 0) ++n, v >>= 1;
+  return std::max(n, 1);
+}
+
+struct Layout {
+  int64_t keys[2], payload[2], counts, totals, bytes;
+};
+Layout layout(const TokenTiles& t, int payload) {
+  Layout l;
+  int64_t at = 0;
+  auto take = [&](int64_t n) { const int64_t here = at; at += (n + 255) / 256 * 256; return here; };
+  for (int k = 0; k < 2; ++k) {
+    l.keys[k] = take(t.count * 4);
+    l.payload[k] = take(t.count * payload);
+  }
+  l.counts = take(t.blocks * kBins * 4);
+  l.totals = take(kBins * 4);
+  l.bytes = at;
+  return l;
+}
+
+template <typename P> void scatter(const Pass& p, const uint32_t* counts, const uint32_t* totals, uint32_t* keys, void* payload, hipStream_t s) {
+  hipLaunchKernelGGL(sort_scatter_kernel<P>, dim3((unsigned)p.tiles.blocks), dim3(kThreads), 0, s, p, counts, totals, keys, (P*)payload);
+  LGA_HIP_CHECK(hipGetLastError());
+}
+
+}  // namespace
+
+TokenTiles token_tiles(const TokenGrid& g) {
+  TokenTiles t;
+  // sides: as many tokens along axis 0 as there are, up to 64 (256 bytes of int32 ids where they are neighbours)
+  int shift0 = 0;
+  while (shift0 < 6 && (1LL << shift0) < g.n0) ++shift0;
+  t.shift1 = 12 - shift0;
+  t.across = (g.n1 + (1LL << t.shift1) - 1) >> t.shift1;
+  t.blocks = ((g.n0 + (1LL << shift0) - 1) >> shift0) * t.across;
+  t.count = t.blocks * kSortTile;
+  if (t.count > 4294967295LL - kSortTile) throw std::runtime_error("embedding_grad: too many tokens");
+  return t;
+}
+
+int64_t token_sort_workspace(const TokenGrid& g, int payload) { return layout(token_tiles(g), payload).bytes; }
+
+SortedTokens token_sort(const TokenGrid& g, const void* values, int64_t v0, int64_t v1, int payload, void* workspace, hipStream_t s) {
+  const TokenTiles tiles = token_tiles(g);
+  const Layout l = layout(tiles, payload);
+  char* w = (char*)workspace;
+  const int bits = bit_length(g.rows), passes = (bits + kMaxBits - 1) / kMaxBits, each = (bits + passes - 1) / passes;
+  uint32_t *counts = (uint32_t*)(w + l.counts), *totals = (uint32_t*)(w + l.totals);
+  Pass p{g, tiles, nullptr, values, v0, v1, 0, each};
+  for (int k = 0; k < passes; ++k) {
+    p.shift = k * each;
+    p.bits = std::min(each, bits - p.shift);
+    uint32_t* keys = (uint32_t*)(w + l.keys[k & 1]);
+    void* pay = w + l.payload[k & 1];
+    hipLaunchKernelGGL(sort_count_kernel, dim3((unsigned)tiles.blocks), dim3(kThreads), 0, s, p, counts);
+    LGA_HIP_CHECK(hipGetLastError());
+    hipLaunchKernelGGL(sort_offsets_kernel, dim3(1u << p.bits), dim3(kThreads), 0, s, counts, totals, tiles.blocks);
+    LGA_HIP_CHECK(hipGetLastError());
+    if (payload == 8) scatter<uint64_t>(p, counts, totals, keys, pay, s);
+    else scatter<uint32_t>(p, counts, totals, keys, pay, s);
+    p.keys_in = keys;
+    p.payload_in = pay;
+  }
+  return {p.keys_in, p.payload_in, tiles.count};
+}
+
+}  // namespace lga

@@ -16,18 +16,80 @@ __device__ __forceinline__ int64_t load_id(const void* ids, int64_t at, int ids6
   return ids64 ? reinterpret_cast<const int64_t*>(ids)[at] : (int64_t)reinterpret_cast<const int32_t*>(ids)[at];
 }
 
-// One lane per element of the output, for every width and alignment.
+constexpr int kNarrow = 16;      // rows of up to this many values go through a tile of tokens
+
+// Rows of more than kNarrow values: `group` lanes copy a row in packs of V.
+template <typename T, int V>
+__global__ __launch_bounds__(kThreads) void lookup_rows_kernel(const T* __restrict__ table, const void* __restrict__ ids, T* __restrict__ out,
+                                                               int64_t rows, int64_t width, int64_t table_stride, int64_t n1, int64_t s0,
+                                                               int64_t s1, int ids64, int64_t tokens, int group, Wide<T> scale) {
+  typedef Wide<T> W;
+  const int64_t token = (int64_t)blockIdx.x * (kThreads / group) + threadIdx.x / group;
+  if (token >= tokens) return;
+  const uint32_t i = (uint32_t)token / (uint32_t)n1, j = (uint32_t)token - i * (uint32_t)n1;
+  const int64_t id = load_id(ids, i * s0 + j * s1, ids64);
+  const bool named = id >= 0 && id < rows;
+  const T* from = table + (named ? id * table_stride : 0);
+  T* to = out + token * width;
+  const int step = group * V;
+  int64_t c = (int64_t)(threadIdx.x % group) * V;
+  constexpr int kAhead = 4;
+  for (; c + (kAhead - 1) * step < width; c += kAhead * step) {
+    Pack<T, V> x[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (named) x[u] = load_pack<T, V>(from + c + u * step);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      for (int v = 0; v < V; ++v) x[u].v[v] = named ? (T)((W)x[u].v[v] * scale) : (T)(W)0;
+      store_pack<T, V>(to + c + u * step, x[u]);
+    }
+  }
+  for (; c < width; c += step) {
+    Pack<T, V> x;
+    if (named) x = load_pack<T, V>(from + c);
+    for (int v = 0; v < V; ++v) x.v[v] = named ? (T)((W)x.v[v] * scale) : (T)(W)0;
+    store_pack<T, V>(to + c, x);
+  }
+}
+
+// Narrow rows: a workgroup takes a tile of tokens, reads its ids along the axis on which they are neighbours, and writes
+// along the axis on which the results are.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void lookup_elements_kernel(const T* __restrict__ table, const void* __restrict__ ids, T* __restrict__ out,
-                                                                   int64_t rows, int64_t width, int64_t table_stride, int64_t n1, int64_t s0,
-                                                                   int64_t s1, int ids64, int64_t total, Wide<T> scale) {
-  for (int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x; e < total; e += (int64_t)gridDim.x * kThreads) {
-    const int64_t token = e / width, col = e - token * width;
-    const int64_t i = token / n1, j = token - i * n1;
-    const int64_t id = load_id(ids, i * s0 + j * s1, ids64);
-    Wide<T> v = 0;
-    if (id >= 0 && id < rows) v = (Wide<T>)table[id * table_stride + col] * scale;
-    out[e] = (T)v;
+__global__ __launch_bounds__(kThreads) void lookup_tile_kernel(const T* __restrict__ table, const void* __restrict__ ids, T* __restrict__ out, int64_t rows,
+                                                               int width, int64_t table_stride, TokenGrid grid, TokenTiles tiles, Wide<T> scale) {
+  __shared__ int32_t id_of[kSortTile];
+  const int shift1 = tiles.shift1, side1 = 1 << shift1, shift0 = 12 - shift1;
+  const int64_t ti = blockIdx.x / tiles.across, i0 = ti << shift0, j0 = (blockIdx.x - ti * tiles.across) << shift1;
+  const bool along0 = grid.s0 < grid.s1;
+#pragma unroll 8
+  for (int n = threadIdx.x; n < kSortTile; n += kThreads) {
+    const int i = along0 ? n & ((1 << shift0) - 1) : n >> shift1, j = along0 ? n >> shift0 : n & (side1 - 1);
+    int32_t id = -1;
+    if (i0 + i < grid.n0 && j0 + j < grid.n1) {
+      const int64_t v = load_id(ids, (i0 + i) * grid.s0 + (j0 + j) * grid.s1, grid.ids64);
+      if (v >= 0 && v < rows) id = (int32_t)v;
+    }
+    id_of[tile_slot(i << shift1 | j)] = id;
+  }
+  __syncthreads();
+  const int live1 = (int)min((int64_t)side1, grid.n1 - j0), live0 = (int)min((int64_t)1 << shift0, grid.n0 - i0);
+  if (width == 1) {
+#pragma unroll 8
+    for (int n = threadIdx.x; n < kSortTile; n += kThreads) {
+      const int i = n >> shift1, j = n & (side1 - 1);
+      if (i >= live0 || j >= live1) continue;
+      const int32_t id = id_of[tile_slot(n)];
+      out[(i0 + i) * grid.n1 + j0 + j] = id >= 0 ? (T)((Wide<T>)table[id * table_stride] * scale) : (T)(Wide<T>)0;
+    }
+    return;
+  }
+  const int line = live1 * width, total = live0 * line;
+#pragma unroll 4
+  for (int n = threadIdx.x; n < total; n += kThreads) {
+    const int i = n / line, e = n - i * line, j = e / width;
+    const int32_t id = id_of[tile_slot(i << shift1 | j)];
+    out[((i0 + i) * grid.n1 + j0) * width + e] = id >= 0 ? (T)((Wide<T>)table[id * table_stride + e - j * width] * scale) : (T)(Wide<T>)0;
   }
 }
 
@@ -85,6 +147,97 @@ __global__ __launch_bounds__(kThreads) void lookup_grad_owned_kernel(const T* __
   if (col < width)
     for (int r = 0; r < kOwnRows; ++r)
       if (first + r < rows) out[(first + r) * width + col] = (O)(acc[r][t] * scale);
+}
+
+// Few rows, many tokens: every wave keeps sums of the whole table in LDS and adds its tokens to them one wave of 64 at a
+// time; the waves' sums are added up in order afterwards.  LDS instructions of one wave run in their order, and no two lanes
+// of one add share an address, so the order of additions is fixed:  tag[row] = lane, read back, tells whether all rows of
+// the 64 differ (whichever of two lanes is read back, one of them sees the other); if not, lanes of one row find each other
+// with ballots and take turns.
+constexpr int kPrivateItems = 16;     // tokens a lane holds
+
+// A step: 64 x kPrivateItems tokens; lanes along axis 0, items along axis 1 or (few tokens there) along axis 0 too.
+template <typename T>
+__global__ __launch_bounds__(64) void lookup_grad_private_kernel(const T* __restrict__ grad, TokenGrid grid, int64_t g0, int64_t g1, int width, int row_bits,
+                                                                 int items_along0, int64_t lines, int64_t steps, Wide<T>* __restrict__ parts) {
+  typedef Wide<T> W;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  W* sums = (W*)lds;
+  const int rows = (int)grid.rows, values = rows * width, lane = threadIdx.x;
+  volatile uint8_t* tag = (volatile uint8_t*)(sums + values);
+  for (int k = lane; k < values; k += 64) sums[k] = 0;
+  __syncthreads();
+  for (int64_t step = blockIdx.x; step < steps; step += gridDim.x) {
+    const int64_t si = step / lines, line = step - si * lines;
+    const int64_t i0 = si * 64 * (items_along0 ? kPrivateItems : 1) + lane, j0 = items_along0 ? line : line * kPrivateItems;
+    const int64_t item_i = items_along0 ? 64 : 0, item_j = items_along0 ? 0 : 1;
+    int32_t row[kPrivateItems];
+#pragma unroll
+    for (int u = 0; u < kPrivateItems; ++u) {
+      const int64_t i = i0 + u * item_i, j = j0 + u * item_j;
+      row[u] = -1;
+      if (i < grid.n0 && j < grid.n1) {
+        const int64_t id = load_id(grid.ids, i * grid.s0 + j * grid.s1, grid.ids64);
+        if (id >= 0 && id < rows) row[u] = (int32_t)id;
+      }
+    }
+    T g[kPrivateItems];
+#pragma unroll
+    for (int u = 0; u < kPrivateItems; ++u) g[u] = row[u] >= 0 ? grad[(i0 + u * item_i) * g0 + (j0 + u * item_j) * g1] : (T)0.f;
+    uint8_t seen[kPrivateItems];
+#pragma unroll
+    for (int u = 0; u < kPrivateItems; ++u) {
+      seen[u] = (uint8_t)lane;
+      if (row[u] >= 0) {
+        tag[row[u]] = (uint8_t)lane;
+        seen[u] = tag[row[u]];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kPrivateItems; ++u) {
+      int turn = 0, turns = 1;
+      if (__any(seen[u] != (uint8_t)lane)) {       // two lanes share a row
+        uint64_t same = __ballot(row[u] >= 0);
+        for (int bit = 0; bit < row_bits; ++bit) {
+          const bool one = row[u] >> bit & 1;
+          const uint64_t ones = __ballot(one);
+          same &= one ? ones : ~ones;
+        }
+        turn = __popcll(same & ((1ull << lane) - 1));
+        turns = row[u] >= 0 ? __popcll(same) : 1;
+        for (int d = 32; d; d >>= 1) turns = max(turns, __shfl_xor(turns, d));
+      }
+      for (int k = 0; k < turns; ++k)
+        if (row[u] >= 0 && turn == k) {
+          W* at = sums + row[u] * width;
+          unsafeAtomicAdd(at, (W)g[u]);
+          for (int c = 1; c < width; ++c) unsafeAtomicAdd(at + c, (W)grad[(i0 + u * item_i) * g0 + (j0 + u * item_j) * g1 + c]);
+        }
+    }
+  }
+  __syncthreads();
+  for (int k = lane; k < values; k += 64) parts[(int64_t)blockIdx.x * values + k] = sums[k];
+}
+
+// out = scale * the waves' sums, 64 values side by side, the waves in kThreads / 64 parts.
+template <typename W, typename O>
+__global__ __launch_bounds__(kThreads) void lookup_grad_total_kernel(const W* __restrict__ parts, O* __restrict__ out, int64_t values, int waves, W scale) {
+  constexpr int kParts = kThreads / 64;
+  __shared__ W of_part[kParts][64];
+  const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
+  const int64_t at = (int64_t)blockIdx.x * 64 + lane;
+  const int each = (waves + kParts - 1) / kParts, from = part * each, to = min(waves, from + each);
+  W sum = 0;
+  if (at < values) {
+#pragma unroll 8
+    for (int w = from; w < to; ++w) sum += parts[(int64_t)w * values + at];
+  }
+  of_part[part][lane] = sum;
+  __syncthreads();
+  if (part == 0 && at < values) {
+    for (int k = 1; k < kParts; ++k) sum += of_part[k][lane];
+    out[at] = (O)(sum * scale);
+  }
 }
 
 // Sorted path.  The sorted tokens are cut into pieces of equal length.  A run (the tokens of one row) that lies within a
@@ -193,7 +346,7 @@ __global__ __launch_bounds__(kThreads) void lookup_grad_runs_kernel(Runs r, cons
   }
 }
 
-constexpr int kNarrow = 16, kNarrowItems = 8, kNarrowPiece = kThreads * kNarrowItems;
+constexpr int kNarrowItems = 8, kNarrowPiece = kThreads * kNarrowItems;
 
 // Rows of up to kNarrow values: a workgroup takes a piece, a lane 8 neighbouring tokens; a segmented scan over the lanes
 // carries a run's sum on.  kValues: the payload is the gradient itself (rows of one value).
@@ -298,7 +451,7 @@ __global__ __launch_bounds__(kThreads) void lookup_grad_join_kernel(Runs r, O* _
   __shared__ W parts[kParts][64];
   const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
   const int64_t each = (chain + kParts - 1) / kParts, from = part * each, to = min(chain, from + each);
-  for (int64_t base = 0; base < r.width; base += 64) {
+  for (int64_t base = (int64_t)blockIdx.y * 64; base < r.width; base += (int64_t)gridDim.y * 64) {
     const int64_t col = base + lane;
     W sum = 0;
     if (col < r.width) {
@@ -317,16 +470,41 @@ __global__ __launch_bounds__(kThreads) void lookup_grad_join_kernel(Runs r, O* _
   }
 }
 
+template <typename T, int V> void launch_rows(const LookupArgs& a, int64_t tokens) {
+  int group = 64;
+  while (group > 1 && group / 2 * V >= a.width) group /= 2;
+  hipLaunchKernelGGL((lookup_rows_kernel<T, V>), dim3((unsigned)((tokens * group + kThreads - 1) / kThreads)), dim3(kThreads), 0, (hipStream_t)a.stream,
+                     (const T*)a.table, (const void*)a.ids, (T*)a.out, a.rows, a.width, a.table_stride, a.n1, a.s0, a.s1, (int)a.ids64, tokens, group,
+                     (Wide<T>)a.scale);
+}
+
 template <typename T> void run_lookup(const LookupArgs& a) {
-  const int64_t total = a.n0 * a.n1 * a.width;
-  const int blocks = (int)std::min<int64_t>((total + kThreads - 1) / kThreads, 1 << 20);
-  hipLaunchKernelGGL(lookup_elements_kernel<T>, dim3(blocks), dim3(kThreads), 0, (hipStream_t)a.stream, (const T*)a.table, (const void*)a.ids,
-                     (T*)a.out, a.rows, a.width, a.table_stride, a.n1, a.s0, a.s1, (int)a.ids64, total, (Wide<T>)a.scale);
+  const int64_t tokens = a.n0 * a.n1, size = sizeof(T);
+  if (a.width <= kNarrow) {
+    TokenGrid grid;
+    grid.ids64 = (int)a.ids64;
+    grid.n0 = a.n0, grid.n1 = a.n1, grid.s0 = a.s0, grid.s1 = a.s1;
+    grid.rows = a.rows;
+    const TokenTiles tiles = token_tiles(grid);
+    hipLaunchKernelGGL(lookup_tile_kernel<T>, dim3((unsigned)tiles.blocks), dim3(kThreads), 0, (hipStream_t)a.stream, (const T*)a.table, (const void*)a.ids,
+                       (T*)a.out, a.rows, (int)a.width, a.table_stride, grid, tiles, (Wide<T>)a.scale);
+  } else {
+    int64_t v = 16 / size;
+    while (v > 1 && (a.width % v || a.table_stride % v || a.table % (v * size))) v /= 2;
+    if (v == 1) launch_rows<T, 1>(a, tokens);
+    else if (v == 2) launch_rows<T, 2>(a, tokens);
+    else if constexpr (sizeof(T) <= 4) {
+      if (v == 4) launch_rows<T, 4>(a, tokens);
+      else if constexpr (sizeof(T) == 2) launch_rows<T, 8>(a, tokens);
+    }
+  }
   LGA_HIP_CHECK(hipGetLastError());
 }
 
 // Up to this many tokens every workgroup looks through all ids for its own rows; above, they are sorted.
 constexpr int64_t kOwnedTokens = 2048;
+// LDS a wave may take for sums of the whole table.
+constexpr int64_t kPrivateLds = 65536;
 
 struct GradPlan {
   TokenGrid grid;
@@ -374,6 +552,37 @@ GradPlan plan_grad(const LookupGradArgs& a) {
 
 bool owned(const LookupGradArgs& a) { return a.n0 * a.n1 <= kOwnedTokens; }
 
+// Few rows and many tokens: sums of the whole table in a wave's share of LDS.
+struct PrivatePlan {
+  TokenGrid grid;
+  int64_t g0, g1, lines, steps;
+  int items_along0, waves = 0, lds = 0;      // waves 0: not this way
+};
+
+PrivatePlan plan_private(const LookupGradArgs& a) {
+  PrivatePlan p;
+  const int64_t wide = a.type == kF64 ? 8 : 4, tokens = a.n0 * a.n1, lds = a.rows * (a.width * wide + 1);
+  if (a.width > kNarrow || lds > kPrivateLds || tokens < 16 * a.rows) return p;
+  p.grid.ids = (const void*)a.ids;
+  p.grid.ids64 = (int)a.ids64;
+  p.grid.rows = a.rows;
+  p.grid.n0 = a.n0, p.grid.n1 = a.n1, p.grid.s0 = a.s0, p.grid.s1 = a.s1;
+  p.g0 = a.g0, p.g1 = a.g1;
+  if (a.n1 > 1 && (a.n0 == 1 || a.s1 < a.s0)) {      // lanes along the axis on which ids are neighbours
+    std::swap(p.grid.n0, p.grid.n1);
+    std::swap(p.grid.s0, p.grid.s1);
+    std::swap(p.g0, p.g1);
+  }
+  p.items_along0 = p.grid.n1 < kPrivateItems / 2;
+  p.lines = p.items_along0 ? p.grid.n1 : (p.grid.n1 + kPrivateItems - 1) / kPrivateItems;
+  const int64_t side0 = p.items_along0 ? 64 * kPrivateItems : 64;
+  p.steps = (p.grid.n0 + side0 - 1) / side0 * p.lines;
+  p.lds = (int)((lds + 15) / 16 * 16);
+  const int64_t fit = 256 * std::min<int64_t>(8, std::max<int64_t>(1, 163840 / p.lds));
+  p.waves = (int)std::max<int64_t>(1, std::min({fit, p.steps, tokens / std::max<int64_t>(1024, 2 * a.rows)}));
+  return p;
+}
+
 template <typename T, typename O, int V> void launch_runs(const LookupGradArgs& a, const GradPlan& p, const Runs& r, Wide<T>* head, Wide<T>* tail) {
   const int64_t zero_blocks = (a.rows + kZeroRows * (kThreads / 64) - 1) / (kZeroRows * (kThreads / 64));
   const int64_t run_blocks = (p.pieces * p.group + kThreads - 1) / kThreads;
@@ -389,6 +598,20 @@ template <typename T, typename O> void run_lookup_grad(const LookupGradArgs& a) 
     const dim3 grid((unsigned)((a.rows + kOwnRows - 1) / kOwnRows), (unsigned)((a.width + kThreads - 1) / kThreads));
     hipLaunchKernelGGL((lookup_grad_owned_kernel<T, O>), grid, dim3(kThreads), 0, s, (const T*)a.grad, (const void*)a.ids, (O*)a.out, a.rows, a.width,
                        a.n0 * a.n1, a.n1, a.s0, a.s1, a.g0, a.g1, (int)a.ids64, (W)a.scale);
+    LGA_HIP_CHECK(hipGetLastError());
+    return;
+  }
+  const PrivatePlan few = plan_private(a);
+  if (few.waves) {
+    W* parts = (W*)a.work;
+    const int64_t values = a.rows * a.width;
+    int bits = 1;
+    while (a.rows >> bits) ++bits;
+    hipLaunchKernelGGL(lookup_grad_private_kernel<T>, dim3(few.waves), dim3(64), few.lds, s, (const T*)a.grad, few.grid, few.g0, few.g1, (int)a.width, bits,
+                       few.items_along0, few.lines, few.steps, parts);
+    LGA_HIP_CHECK(hipGetLastError());
+    hipLaunchKernelGGL((lookup_grad_total_kernel<W, O>), dim3((unsigned)((values + 63) / 64)), dim3(kThreads), 0, s, parts, (O*)a.out, values, few.waves,
+                       (W)a.scale);
     LGA_HIP_CHECK(hipGetLastError());
     return;
   }
@@ -418,7 +641,7 @@ template <typename T, typename O> void run_lookup_grad(const LookupGradArgs& a) 
     }
   }
   LGA_HIP_CHECK(hipGetLastError());
-  hipLaunchKernelGGL((lookup_grad_join_kernel<W, O>), dim3((unsigned)p.pieces), dim3(kThreads), 0, s, r, (O*)a.out, head, tail, p.piece_tokens, (W)a.scale);
+  hipLaunchKernelGGL((lookup_grad_join_kernel<W, O>), dim3((unsigned)p.pieces, (unsigned)std::min<int64_t>((a.width + 63) / 64, 8)), dim3(kThreads), 0, s, r, (O*)a.out, head, tail, p.piece_tokens, (W)a.scale);
   LGA_HIP_CHECK(hipGetLastError());
 }
 
@@ -446,6 +669,8 @@ void lookup(const LookupArgs& a) {
 int64_t lookup_grad_workspace(const LookupGradArgs& a) {
   check_sizes(a.rows, a.width, a.n0, a.n1);
   if (owned(a)) return 0;
+  const PrivatePlan few = plan_private(a);
+  if (few.waves) return few.waves * a.rows * a.width * (a.type == kF64 ? 8 : 4);
   const GradPlan p = plan_grad(a);
   return p.sort_bytes + 2 * p.parts_bytes;
 }

@@ -121,7 +121,7 @@ __global__ __launch_bounds__(kThreads) void sort_scatter_kernel(Pass p, const ui
       const int q = ids_order(p, k * kThreads + t);
       int64_t i, j;
       item_place(p, b, q, i, j);
-      skey[q] = grid_key(p.grid, i, j);
+      skey[tile_slot(q)] = grid_key(p.grid, i, j);
     }
   }
   __syncthreads();
@@ -132,7 +132,7 @@ __global__ __launch_bounds__(kThreads) void sort_scatter_kernel(Pass p, const ui
       key[k] = p.keys_in[b * kSortTile + q];
       pay[k] = ((const P*)p.payload_in)[b * kSortTile + q];
     } else {
-      key[k] = skey[q];
+      key[k] = skey[tile_slot(q)];
       int64_t i, j;
       item_place(p, b, q, i, j);
       if (!p.payload_in) pay[k] = (P)(i * p.grid.n1 + j);

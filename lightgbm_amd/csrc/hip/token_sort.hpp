@@ -22,6 +22,10 @@ struct TokenTiles {
 };
 TokenTiles token_tiles(const TokenGrid& g);
 
+// Where item q of a tile stands in LDS: tiles are written along one axis and read along the other, and this way neither
+// walk meets a bank twice.
+__device__ __forceinline__ int tile_slot(int q) { return (q & ~63) | ((q ^ (q >> 6)) & 63); }
+
 // Bytes of workspace of a sort with `payload` bytes a token.
 int64_t token_sort_workspace(const TokenGrid& g, int payload);
 

@@ -156,8 +156,9 @@ __global__ __launch_bounds__(kThreads) void lookup_grad_owned_kernel(const T* __
 // with ballots and take turns.
 constexpr int kPrivateItems = 16;     // tokens a lane holds
 
-// A step: 64 x kPrivateItems tokens; lanes along axis 0, items along axis 1 or (few tokens there) along axis 0 too.
-template <typename T>
+// A step: 64 x kPrivateItems tokens; lanes along axis 0, items along axis 1 or (few tokens there) along axis 0 too.  A step
+// is loaded while the one before is added up.  kWhole: a lane's gradients of a step are neighbours and loaded as packs.
+template <typename T, typename I, bool kWhole>
 __global__ __launch_bounds__(64) void lookup_grad_private_kernel(const T* __restrict__ grad, TokenGrid grid, int64_t g0, int64_t g1, int width, int row_bits,
                                                                  int items_along0, int64_t lines, int64_t steps, Wide<T>* __restrict__ parts) {
   typedef Wide<T> W;
@@ -167,23 +168,45 @@ __global__ __launch_bounds__(64) void lookup_grad_private_kernel(const T* __rest
   volatile uint8_t* tag = (volatile uint8_t*)(sums + values);
   for (int k = lane; k < values; k += 64) sums[k] = 0;
   __syncthreads();
-  for (int64_t step = blockIdx.x; step < steps; step += gridDim.x) {
+  const int64_t item_i = items_along0 ? 64 : 0, item_j = items_along0 ? 0 : 1;
+  auto place = [&](int64_t step, int64_t& i0, int64_t& j0) {
     const int64_t si = step / lines, line = step - si * lines;
-    const int64_t i0 = si * 64 * (items_along0 ? kPrivateItems : 1) + lane, j0 = items_along0 ? line : line * kPrivateItems;
-    const int64_t item_i = items_along0 ? 64 : 0, item_j = items_along0 ? 0 : 1;
-    int32_t row[kPrivateItems];
+    i0 = si * 64 * (items_along0 ? kPrivateItems : 1) + lane;
+    j0 = items_along0 ? line : line * kPrivateItems;
+  };
+  auto load = [&](int64_t step, I (&id)[kPrivateItems], T (&g)[kPrivateItems]) {
+    int64_t i0, j0;
+    place(step, i0, j0);
 #pragma unroll
     for (int u = 0; u < kPrivateItems; ++u) {
       const int64_t i = i0 + u * item_i, j = j0 + u * item_j;
-      row[u] = -1;
-      if (i < grid.n0 && j < grid.n1) {
-        const int64_t id = load_id(grid.ids, i * grid.s0 + j * grid.s1, grid.ids64);
-        if (id >= 0 && id < rows) row[u] = (int32_t)id;
+      id[u] = -1;
+      if (i < grid.n0 && j < grid.n1) id[u] = ((const I*)grid.ids)[i * grid.s0 + j * grid.s1];
+    }
+    if (kWhole && i0 < grid.n0 && j0 + kPrivateItems <= grid.n1) {
+      constexpr int kPack = 16 / sizeof(T);
+#pragma unroll
+      for (int u = 0; u < kPrivateItems; u += kPack) {
+        const Pack<T, kPack> x = load_pack<T, kPack>(grad + i0 * g0 + j0 + u);
+#pragma unroll
+        for (int v = 0; v < kPack; ++v) g[u + v] = x.v[v];
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < kPrivateItems; ++u) {
+        const int64_t i = i0 + u * item_i, j = j0 + u * item_j;
+        g[u] = i < grid.n0 && j < grid.n1 ? grad[i * g0 + j * g1] : (T)0.f;
       }
     }
-    T g[kPrivateItems];
+  };
+  int32_t row[kPrivateItems];
+  I next_id[kPrivateItems];
+  T g[kPrivateItems], next_g[kPrivateItems];
+  load(blockIdx.x, next_id, next_g);
+  for (int64_t step = blockIdx.x; step < steps; step += gridDim.x) {
 #pragma unroll
-    for (int u = 0; u < kPrivateItems; ++u) g[u] = row[u] >= 0 ? grad[(i0 + u * item_i) * g0 + (j0 + u * item_j) * g1] : (T)0.f;
+    for (int u = 0; u < kPrivateItems; ++u) row[u] = next_id[u] >= 0 && next_id[u] < rows ? (int32_t)next_id[u] : -1, g[u] = next_g[u];
+    if (step + gridDim.x < steps) load(step + gridDim.x, next_id, next_g);
     uint8_t seen[kPrivateItems];
 #pragma unroll
     for (int u = 0; u < kPrivateItems; ++u) {
@@ -211,7 +234,12 @@ __global__ __launch_bounds__(64) void lookup_grad_private_kernel(const T* __rest
         if (row[u] >= 0 && turn == k) {
           W* at = sums + row[u] * width;
           unsafeAtomicAdd(at, (W)g[u]);
-          for (int c = 1; c < width; ++c) unsafeAtomicAdd(at + c, (W)grad[(i0 + u * item_i) * g0 + (j0 + u * item_j) * g1 + c]);
+          if (width > 1) {
+            int64_t i0, j0;
+            place(step, i0, j0);
+            const T* more = grad + (i0 + u * item_i) * g0 + (j0 + u * item_j) * g1;
+            for (int c = 1; c < width; ++c) unsafeAtomicAdd(at + c, (W)more[c]);
+          }
         }
     }
   }
@@ -529,7 +557,7 @@ GradPlan plan_grad(const LookupGradArgs& a) {
   }
   p.values = a.width == 1 && size >= 4;
   p.payload = p.values ? (int)size : 4;
-  const TokenTiles tiles = token_tiles(p.grid);
+  const TokenTiles tiles = sort_tiles(p.grid);
   p.vec = 1;
   p.group = 64;
   if (a.width <= kNarrow) {
@@ -557,6 +585,7 @@ struct PrivatePlan {
   TokenGrid grid;
   int64_t g0, g1, lines, steps;
   int items_along0, waves = 0, lds = 0;      // waves 0: not this way
+  bool whole = false;
 };
 
 PrivatePlan plan_private(const LookupGradArgs& a) {
@@ -577,6 +606,8 @@ PrivatePlan plan_private(const LookupGradArgs& a) {
   p.lines = p.items_along0 ? p.grid.n1 : (p.grid.n1 + kPrivateItems - 1) / kPrivateItems;
   const int64_t side0 = p.items_along0 ? 64 * kPrivateItems : 64;
   p.steps = (p.grid.n0 + side0 - 1) / side0 * p.lines;
+  const int64_t pack = a.type == kF64 ? 2 : a.type == kF32 ? 4 : 8;
+  p.whole = !p.items_along0 && a.width == 1 && p.g1 == 1 && p.g0 % pack == 0 && a.grad % 16 == 0;
   p.lds = (int)((lds + 15) / 16 * 16);
   const int64_t fit = 256 * std::min<int64_t>(8, std::max<int64_t>(1, 163840 / p.lds));
   p.waves = (int)std::max<int64_t>(1, std::min({fit, p.steps, tokens / std::max<int64_t>(1024, 2 * a.rows)}));
@@ -607,8 +638,12 @@ template <typename T, typename O> void run_lookup_grad(const LookupGradArgs& a) 
     const int64_t values = a.rows * a.width;
     int bits = 1;
     while (a.rows >> bits) ++bits;
-    hipLaunchKernelGGL(lookup_grad_private_kernel<T>, dim3(few.waves), dim3(64), few.lds, s, (const T*)a.grad, few.grid, few.g0, few.g1, (int)a.width, bits,
-                       few.items_along0, few.lines, few.steps, parts);
+    auto run = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(few.waves), dim3(64), few.lds, s, (const T*)a.grad, few.grid, few.g0, few.g1, (int)a.width, bits, few.items_along0,
+                         few.lines, few.steps, parts);
+    };
+    if (a.ids64) few.whole ? run(lookup_grad_private_kernel<T, int64_t, true>) : run(lookup_grad_private_kernel<T, int64_t, false>);
+    else few.whole ? run(lookup_grad_private_kernel<T, int32_t, true>) : run(lookup_grad_private_kernel<T, int32_t, false>);
     LGA_HIP_CHECK(hipGetLastError());
     hipLaunchKernelGGL((lookup_grad_total_kernel<W, O>), dim3((unsigned)((values + 63) / 64)), dim3(kThreads), 0, s, parts, (O*)a.out, values, few.waves,
                        (W)a.scale);

@@ -11,7 +11,6 @@ namespace lga {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kItems = kSortTile / kThreads;    // keys a lane holds
 constexpr int kMaxBits = 8, kBins = 1 << kMaxBits;
 
 struct Pass {
@@ -21,7 +20,9 @@ struct Pass {
   const void* payload_in;
   int64_t v0, v1;               // first pass: payload (i, j) is at i * v0 + j * v1; payload_in null: the token's number
   int shift, bits;
+  bool few;                     // few tiles: no kernel of its own for the offsets
 };
+constexpr int64_t kFewTiles = 128;
 
 __device__ __forceinline__ uint32_t grid_key(const TokenGrid& g, int64_t i, int64_t j) {
   if (i >= g.n0 || j >= g.n1) return (uint32_t)g.rows;
@@ -33,17 +34,19 @@ __device__ __forceinline__ uint32_t grid_key(const TokenGrid& g, int64_t i, int6
 // Item q of tile b is token (i, j) with j running fastest.
 __device__ __forceinline__ void item_place(const Pass& p, int64_t b, int q, int64_t& i, int64_t& j) {
   const int64_t ti = b / p.tiles.across, tj = b - ti * p.tiles.across;
-  i = ti * (kSortTile >> p.tiles.shift1) + (q >> p.tiles.shift1);
+  i = ti * (1 << (p.tiles.bits - p.tiles.shift1)) + (q >> p.tiles.shift1);
   j = (tj << p.tiles.shift1) + (q & ((1 << p.tiles.shift1) - 1));
 }
 // The same items walked along the axis on which ids are neighbours: returns the item number.
 __device__ __forceinline__ int ids_order(const Pass& p, int n) {
-  if (p.grid.s1 <= p.grid.s0 || p.tiles.shift1 == 12) return n;
-  const int shift0 = 12 - p.tiles.shift1;
+  if (p.grid.s1 <= p.grid.s0 || p.tiles.shift1 == p.tiles.bits) return n;
+  const int shift0 = p.tiles.bits - p.tiles.shift1;
   return ((n & ((1 << shift0) - 1)) << p.tiles.shift1) | (n >> shift0);
 }
 
+template <int kItems>
 __global__ __launch_bounds__(kThreads) void sort_count_kernel(Pass p, uint32_t* __restrict__ counts) {
+  constexpr int kTile = kItems * kThreads;
   __shared__ uint32_t bin[kBins];
   const int64_t b = blockIdx.x;
   for (int d = threadIdx.x; d < kBins; d += kThreads) bin[d] = 0;
@@ -54,7 +57,7 @@ __global__ __launch_bounds__(kThreads) void sort_count_kernel(Pass p, uint32_t* 
     const int n = k * kThreads + threadIdx.x;
     uint32_t key;
     if (p.keys_in) {
-      key = p.keys_in[b * kSortTile + n];
+      key = p.keys_in[b * kTile + n];
     } else {
       int64_t i, j;
       item_place(p, b, ids_order(p, n), i, j);
@@ -102,12 +105,13 @@ __global__ __launch_bounds__(kThreads) void sort_offsets_kernel(uint32_t* __rest
   if (threadIdx.x == 0) totals[blockIdx.x] = before;
 }
 
-// P: what is carried with a key (uint32 or uint64 words).
-template <typename P>
+// P: what is carried with a key (uint32 or uint64 words).  `offsets` are still counts where there are few tiles.
+template <typename P, int kItems>
 __global__ __launch_bounds__(kThreads) void sort_scatter_kernel(Pass p, const uint32_t* __restrict__ offsets, const uint32_t* __restrict__ totals,
                                                                 uint32_t* __restrict__ keys_out, P* __restrict__ payload_out) {
-  __shared__ uint32_t skey[kSortTile];
-  __shared__ P spay[kSortTile];
+  constexpr int kTile = kItems * kThreads;
+  __shared__ uint32_t skey[kTile];
+  __shared__ P spay[kTile];
   __shared__ uint32_t count[kWaves][kBins];     // keys of a digit in a wave, then those in the waves before
   __shared__ uint32_t local[kBins], global[kBins], wave_sum[kWaves][2];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
@@ -127,10 +131,10 @@ __global__ __launch_bounds__(kThreads) void sort_scatter_kernel(Pass p, const ui
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
-    const int q = wave * (kSortTile / kWaves) + k * 64 + lane;
+    const int q = wave * (kTile / kWaves) + k * 64 + lane;
     if (p.keys_in) {
-      key[k] = p.keys_in[b * kSortTile + q];
-      pay[k] = ((const P*)p.payload_in)[b * kSortTile + q];
+      key[k] = p.keys_in[b * kTile + q];
+      pay[k] = ((const P*)p.payload_in)[b * kTile + q];
     } else {
       key[k] = skey[tile_slot(q)];
       int64_t i, j;
@@ -164,7 +168,21 @@ __global__ __launch_bounds__(kThreads) void sort_scatter_kernel(Pass p, const ui
       count[w][t] = in_tile;
       in_tile += c;
     }
-    const uint32_t total = t < (1 << p.bits) ? totals[t] : 0u;
+    uint32_t total = 0, ahead = 0;
+    if (t < (1 << p.bits)) {
+      const uint32_t* row = offsets + (int64_t)t * p.tiles.blocks;
+      if (p.few) {
+#pragma unroll 8
+        for (int q = 0; q < (int)p.tiles.blocks; ++q) {
+          const uint32_t c = row[q];
+          total += c;
+          if (q < (int)b) ahead += c;
+        }
+      } else {
+        total = totals[t];
+        ahead = row[b];
+      }
+    }
     uint32_t a = in_tile, g = total;
     for (int d = 1; d < 64; d <<= 1) {
       const uint32_t oa = __shfl_up(a, d), og = __shfl_up(g, d);
@@ -174,7 +192,7 @@ __global__ __launch_bounds__(kThreads) void sort_scatter_kernel(Pass p, const ui
     __syncthreads();
     for (int w = 0; w < wave; ++w) a += wave_sum[w][0], g += wave_sum[w][1];
     local[t] = a - in_tile;
-    global[t] = t < (1 << p.bits) ? g - total + offsets[(int64_t)t * p.tiles.blocks + b] : 0u;
+    global[t] = g - total + ahead;
   }
   __syncthreads();
 #pragma unroll
@@ -219,46 +237,66 @@ Layout layout(const TokenTiles& t, int payload) {
   return l;
 }
 
-template <typename P> void scatter(const Pass& p, const uint32_t* counts, const uint32_t* totals, uint32_t* keys, void* payload, hipStream_t s) {
-  hipLaunchKernelGGL(sort_scatter_kernel<P>, dim3((unsigned)p.tiles.blocks), dim3(kThreads), 0, s, p, counts, totals, keys, (P*)payload);
-  LGA_HIP_CHECK(hipGetLastError());
-}
-
 }  // namespace
 
-TokenTiles token_tiles(const TokenGrid& g) {
+TokenTiles token_tiles(const TokenGrid& g, int bits) {
   TokenTiles t;
   // sides: as many tokens along axis 0 as there are, up to 64 (256 bytes of int32 ids where they are neighbours)
   int shift0 = 0;
   while (shift0 < 6 && (1LL << shift0) < g.n0) ++shift0;
-  t.shift1 = 12 - shift0;
+  t.bits = bits;
+  t.shift1 = bits - shift0;
   t.across = (g.n1 + (1LL << t.shift1) - 1) >> t.shift1;
   t.blocks = ((g.n0 + (1LL << shift0) - 1) >> shift0) * t.across;
-  t.count = t.blocks * kSortTile;
-  if (t.count > 4294967295LL - kSortTile) throw std::runtime_error("embedding_grad: too many tokens");
+  t.count = t.blocks << bits;
+  if (t.count > 4294967295LL - kSortTile) throw std::runtime_error("embedding: too many tokens");
   return t;
 }
 
-int64_t token_sort_workspace(const TokenGrid& g, int payload) { return layout(token_tiles(g), payload).bytes; }
+// Small tiles where tiles of 4096 would leave most of the chip idle.
+TokenTiles sort_tiles(const TokenGrid& g) {
+  const TokenTiles small = token_tiles(g, 10);
+  if (small.blocks > kFewTiles) return token_tiles(g);
+  TokenTiles t = small;
+  t.blocks = (t.blocks + 3) / 4 * 4;      // whole multiples of kSortTile
+  t.count = t.blocks << 10;
+  return t;
+}
+
+int64_t token_sort_workspace(const TokenGrid& g, int payload) { return layout(sort_tiles(g), payload).bytes; }
 
 SortedTokens token_sort(const TokenGrid& g, const void* values, int64_t v0, int64_t v1, int payload, void* workspace, hipStream_t s) {
-  const TokenTiles tiles = token_tiles(g);
+  const TokenTiles tiles = sort_tiles(g);
   const Layout l = layout(tiles, payload);
   char* w = (char*)workspace;
   const int bits = bit_length(g.rows), passes = (bits + kMaxBits - 1) / kMaxBits, each = (bits + passes - 1) / passes;
+  const bool small = tiles.bits == 10;
+  const dim3 grid((unsigned)tiles.blocks), block(kThreads);
   uint32_t *counts = (uint32_t*)(w + l.counts), *totals = (uint32_t*)(w + l.totals);
-  Pass p{g, tiles, nullptr, values, v0, v1, 0, each};
+  Pass p{g, tiles, nullptr, values, v0, v1, 0, each, tiles.blocks <= kFewTiles};
   for (int k = 0; k < passes; ++k) {
     p.shift = k * each;
     p.bits = std::min(each, bits - p.shift);
     uint32_t* keys = (uint32_t*)(w + l.keys[k & 1]);
     void* pay = w + l.payload[k & 1];
-    hipLaunchKernelGGL(sort_count_kernel, dim3((unsigned)tiles.blocks), dim3(kThreads), 0, s, p, counts);
+    if (small) hipLaunchKernelGGL(sort_count_kernel<kSmallTile / kThreads>, grid, block, 0, s, p, counts);
+    else hipLaunchKernelGGL(sort_count_kernel<kSortTile / kThreads>, grid, block, 0, s, p, counts);
     LGA_HIP_CHECK(hipGetLastError());
-    hipLaunchKernelGGL(sort_offsets_kernel, dim3(1u << p.bits), dim3(kThreads), 0, s, counts, totals, tiles.blocks);
+    if (!p.few) {
+      hipLaunchKernelGGL(sort_offsets_kernel, dim3(1u << p.bits), block, 0, s, counts, totals, tiles.blocks);
+      LGA_HIP_CHECK(hipGetLastError());
+    }
+    auto scatter = [&](auto kernel, auto* to) {
+      hipLaunchKernelGGL(kernel, grid, block, 0, s, p, counts, totals, keys, to);
+    };
+    if (payload == 8) {
+      if (small) scatter(sort_scatter_kernel<uint64_t, kSmallTile / kThreads>, (uint64_t*)pay);
+      else scatter(sort_scatter_kernel<uint64_t, kSortTile / kThreads>, (uint64_t*)pay);
+    } else {
+      if (small) scatter(sort_scatter_kernel<uint32_t, kSmallTile / kThreads>, (uint32_t*)pay);
+      else scatter(sort_scatter_kernel<uint32_t, kSortTile / kThreads>, (uint32_t*)pay);
+    }
     LGA_HIP_CHECK(hipGetLastError());
-    if (payload == 8) scatter<uint64_t>(p, counts, totals, keys, pay, s);
-    else scatter<uint32_t>(p, counts, totals, keys, pay, s);
     p.keys_in = keys;
     p.payload_in = pay;
   }

@@ -13,14 +13,15 @@ struct TokenGrid {
   int64_t rows = 0;
 };
 
-// The grid is read in tiles of kSortTile tokens, side[0] x side[1]; a tile that reaches over the edge is filled up with
+// The grid is read in tiles of 1 << bits tokens, side[0] x side[1]; a tile that reaches over the edge is filled up with
 // absent tokens (id `rows`), so `count` of the sorted arrays is a multiple of kSortTile.
-constexpr int kSortTile = 4096;
+constexpr int kSortTile = 4096, kSmallTile = 1024;
 struct TokenTiles {
   int64_t across = 0, count = 0, blocks = 0;   // tiles along axis 1, tokens with the absent ones, tiles
-  int shift1 = 0;                              // side[1] = 1 << shift1
+  int bits = 12, shift1 = 0;                   // side[1] = 1 << shift1, side[0] = 1 << (bits - shift1)
 };
-TokenTiles token_tiles(const TokenGrid& g);
+// `bits`: 12, or 10 for small tiles.
+TokenTiles token_tiles(const TokenGrid& g, int bits = 12);
 
 // Where item q of a tile stands in LDS: tiles are written along one axis and read along the other, and this way neither
 // walk meets a bank twice.
@@ -31,6 +32,7 @@ int64_t token_sort_workspace(const TokenGrid& g, int payload);
 
 // Sorts ids with the payload of every token: its number i * n1 + j (values == nullptr, payload 4), or its value
 // values[i * v0 + j * v1] of `payload` bytes (4 or 8).  keys (uint32) and payloads are in the workspace.
+TokenTiles sort_tiles(const TokenGrid& g);      // what a sort of g uses
 struct SortedTokens {
   const uint32_t* keys = nullptr;
   const void* payload = nullptr;

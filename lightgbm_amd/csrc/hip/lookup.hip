@@ -160,87 +160,84 @@ constexpr int kPrivateItems = 16;     // tokens a lane holds
 // is loaded while the one before is added up.  kWhole: a lane's gradients of a step are neighbours and loaded as packs.
 template <typename T, typename I, bool kWhole>
 __global__ __launch_bounds__(64) void lookup_grad_private_kernel(const T* __restrict__ grad, TokenGrid grid, int64_t g0, int64_t g1, int width, int row_bits,
-                                                                 int items_along0, int64_t lines, int64_t steps, Wide<T>* __restrict__ parts) {
+                                                                 int items_along0, int lines, int steps, int each, Wide<T>* __restrict__ parts) {
   typedef Wide<T> W;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  W* sums = (W*)lds;
+  W* sums = (W*)lds;                  // one row more than the table has: tokens that take no part
   const int rows = (int)grid.rows, values = rows * width, lane = threadIdx.x;
-  volatile uint8_t* tag = (volatile uint8_t*)(sums + values);
-  for (int k = lane; k < values; k += 64) sums[k] = 0;
+  volatile uint8_t* tag = (volatile uint8_t*)(sums + values + width);
+  for (int k = lane; k < values + width; k += 64) sums[k] = 0;
   __syncthreads();
   const int64_t item_i = items_along0 ? 64 : 0, item_j = items_along0 ? 0 : 1;
-  auto place = [&](int64_t step, int64_t& i0, int64_t& j0) {
-    const int64_t si = step / lines, line = step - si * lines;
-    i0 = si * 64 * (items_along0 ? kPrivateItems : 1) + lane;
-    j0 = items_along0 ? line : line * kPrivateItems;
+  auto place = [&](int step, int64_t& i0, int64_t& j0) {
+    const int si = step / lines, line = step - si * lines;
+    i0 = (int64_t)si * 64 * (items_along0 ? kPrivateItems : 1) + lane;
+    j0 = (int64_t)line * (items_along0 ? 1 : kPrivateItems);
   };
-  auto load = [&](int64_t step, I (&id)[kPrivateItems], T (&g)[kPrivateItems]) {
+  // places behind the edge are read at the edge and take no part later
+  auto load = [&](int step, I (&id)[kPrivateItems], T (&g)[kPrivateItems]) {
     int64_t i0, j0;
     place(step, i0, j0);
+    const I* ids = (const I*)grid.ids;
 #pragma unroll
-    for (int u = 0; u < kPrivateItems; ++u) {
-      const int64_t i = i0 + u * item_i, j = j0 + u * item_j;
-      id[u] = -1;
-      if (i < grid.n0 && j < grid.n1) id[u] = ((const I*)grid.ids)[i * grid.s0 + j * grid.s1];
-    }
-    if (kWhole && i0 < grid.n0 && j0 + kPrivateItems <= grid.n1) {
+    for (int u = 0; u < kPrivateItems; ++u) id[u] = ids[min(i0 + u * item_i, grid.n0 - 1) * grid.s0 + min(j0 + u * item_j, grid.n1 - 1) * grid.s1];
+    if (kWhole && j0 + kPrivateItems <= grid.n1) {
       constexpr int kPack = 16 / sizeof(T);
+      const T* from = grad + min(i0, grid.n0 - 1) * g0 + j0;
 #pragma unroll
       for (int u = 0; u < kPrivateItems; u += kPack) {
-        const Pack<T, kPack> x = load_pack<T, kPack>(grad + i0 * g0 + j0 + u);
+        const Pack<T, kPack> x = load_pack<T, kPack>(from + u);
 #pragma unroll
         for (int v = 0; v < kPack; ++v) g[u + v] = x.v[v];
       }
     } else {
 #pragma unroll
-      for (int u = 0; u < kPrivateItems; ++u) {
-        const int64_t i = i0 + u * item_i, j = j0 + u * item_j;
-        g[u] = i < grid.n0 && j < grid.n1 ? grad[i * g0 + j * g1] : (T)0.f;
-      }
+      for (int u = 0; u < kPrivateItems; ++u) g[u] = grad[min(i0 + u * item_i, grid.n0 - 1) * g0 + min(j0 + u * item_j, grid.n1 - 1) * g1];
     }
   };
   int32_t row[kPrivateItems];
   I next_id[kPrivateItems];
   T g[kPrivateItems], next_g[kPrivateItems];
-  load(blockIdx.x, next_id, next_g);
-  for (int64_t step = blockIdx.x; step < steps; step += gridDim.x) {
+  const int end = min(steps, ((int)blockIdx.x + 1) * each);
+  if ((int)blockIdx.x * each < steps) load(blockIdx.x * each, next_id, next_g);
+  for (int step = blockIdx.x * each; step < end; ++step) {
+    int64_t i0, j0;
+    place(step, i0, j0);
 #pragma unroll
-    for (int u = 0; u < kPrivateItems; ++u) row[u] = next_id[u] >= 0 && next_id[u] < rows ? (int32_t)next_id[u] : -1, g[u] = next_g[u];
-    if (step + gridDim.x < steps) load(step + gridDim.x, next_id, next_g);
+    for (int u = 0; u < kPrivateItems; ++u) {
+      const bool there = i0 + u * item_i < grid.n0 && j0 + u * item_j < grid.n1;
+      row[u] = there && next_id[u] >= 0 && next_id[u] < rows ? (int32_t)next_id[u] : rows;
+      g[u] = next_g[u];
+    }
+    if (step + 1 < end) load(step + 1, next_id, next_g);
     uint8_t seen[kPrivateItems];
 #pragma unroll
     for (int u = 0; u < kPrivateItems; ++u) {
-      seen[u] = (uint8_t)lane;
-      if (row[u] >= 0) {
-        tag[row[u]] = (uint8_t)lane;
-        seen[u] = tag[row[u]];
-      }
+      tag[row[u]] = (uint8_t)lane;
+      seen[u] = tag[row[u]];
     }
 #pragma unroll
     for (int u = 0; u < kPrivateItems; ++u) {
-      int turn = 0, turns = 1;
-      if (__any(seen[u] != (uint8_t)lane)) {       // two lanes share a row
-        uint64_t same = __ballot(row[u] >= 0);
+      W* at = sums + row[u] * width;
+      const T* more = grad + (i0 + u * item_i) * g0 + (j0 + u * item_j) * g1;
+      auto add = [&] {
+        unsafeAtomicAdd(at, (W)g[u]);
+        if (width > 1 && row[u] < rows)
+          for (int c = 1; c < width; ++c) unsafeAtomicAdd(at + c, (W)more[c]);
+      };
+      if (!__any(row[u] < rows && seen[u] != (uint8_t)lane)) {
+        add();
+      } else {                        // two lanes share a row
+        uint64_t same = ~0ull;
         for (int bit = 0; bit < row_bits; ++bit) {
           const bool one = row[u] >> bit & 1;
           const uint64_t ones = __ballot(one);
           same &= one ? ones : ~ones;
         }
-        turn = __popcll(same & ((1ull << lane) - 1));
-        turns = row[u] >= 0 ? __popcll(same) : 1;
-        for (int d = 32; d; d >>= 1) turns = max(turns, __shfl_xor(turns, d));
+        const int turn = row[u] < rows ? __popcll(same & ((1ull << lane) - 1)) : -1;
+        for (int k = 0; __any(turn >= k); ++k)
+          if (turn == k) add();
       }
-      for (int k = 0; k < turns; ++k)
-        if (row[u] >= 0 && turn == k) {
-          W* at = sums + row[u] * width;
-          unsafeAtomicAdd(at, (W)g[u]);
-          if (width > 1) {
-            int64_t i0, j0;
-            place(step, i0, j0);
-            const T* more = grad + (i0 + u * item_i) * g0 + (j0 + u * item_j) * g1;
-            for (int c = 1; c < width; ++c) unsafeAtomicAdd(at + c, (W)more[c]);
-          }
-        }
     }
   }
   __syncthreads();
@@ -314,63 +311,99 @@ template <typename O> __device__ __forceinline__ void zero_rows(const Runs& r, O
   }
 }
 
-// Rows of more than kNarrow values: `group` lanes walk a piece, V columns a lane.
+// Rows of more than kNarrow values: `group` lanes walk a strip of kStrip tokens, V columns a lane; the strips of a workgroup
+// are a piece, and what crosses strips is joined in LDS.
+constexpr int kRunThreads = 512, kStrip = 32;
+enum { kHasHead = 1, kThrough = 2, kHasTail = 4 };      // of a strip: ends / passes on the run it begins in, begins the run it ends in
+
 template <typename T, typename O, int V>
-__global__ __launch_bounds__(kThreads) void lookup_grad_runs_kernel(Runs r, const T* __restrict__ grad, O* __restrict__ out, Wide<T>* __restrict__ head,
-                                                                    Wide<T>* __restrict__ tail, int zero_blocks, int group, int piece_tokens, Wide<T> scale) {
+__global__ __launch_bounds__(kRunThreads) void lookup_grad_runs_kernel(Runs r, const T* __restrict__ grad, O* __restrict__ out, Wide<T>* __restrict__ head,
+                                                                       Wide<T>* __restrict__ tail, int zero_blocks, int group, int strips_long, Wide<T> scale) {
   typedef Wide<T> W;
   if ((int)blockIdx.x < zero_blocks) {
-    if (blockIdx.y == 0) zero_rows(r, out, (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6), threadIdx.x & 63);
+    if (blockIdx.y == 0) zero_rows(r, out, (int64_t)blockIdx.x * (kRunThreads / 64) + (threadIdx.x >> 6), threadIdx.x & 63);
     return;
   }
   constexpr int kAhead = 8;
-  const int64_t piece = ((int64_t)blockIdx.x - zero_blocks) * (kThreads / group) + threadIdx.x / group;
-  const int64_t col = ((int64_t)blockIdx.y * group + threadIdx.x % group) * V;
-  const int64_t begin = piece * piece_tokens, end = begin + piece_tokens;
-  if (begin >= r.count || col >= r.width) return;
-  uint32_t cur = r.keys[begin];
-  if (cur >= (uint32_t)r.rows) return;
-  const uint32_t* token = (const uint32_t*)r.payload;
-  bool inside = begin == 0 || r.keys[begin - 1] != cur;
-  W acc[V];
-  for (int v = 0; v < V; ++v) acc[v] = 0;
-  auto close = [&] {
-    if (inside) {
-      Pack<O, V> o;
-      for (int v = 0; v < V; ++v) o.v[v] = (O)(acc[v] * scale);
-      store_pack<O, V>(out + (int64_t)cur * r.width + col, o);
-    } else {
-      for (int v = 0; v < V; ++v) head[piece * r.width + col + v] = acc[v];
-    }
+  __shared__ W shead[kRunThreads * V], stail[kRunThreads * V];
+  __shared__ int flags[kRunThreads / 8];
+  const int strips = kRunThreads / group, strip = threadIdx.x / group, lane = threadIdx.x % group;
+  const int64_t piece = (int64_t)blockIdx.x - zero_blocks, length = (int64_t)kStrip * strips_long;
+  const int64_t col = ((int64_t)blockIdx.y * group + lane) * V;
+  const int64_t begin = (piece * strips + strip) * length, end = begin + length;
+  const uint32_t rows = (uint32_t)r.rows, *token = (const uint32_t*)r.payload;
+  const bool live = col < r.width;
+  uint32_t cur = begin < r.count ? r.keys[begin] : rows;
+  int flag = 0;
+  auto write = [&](uint32_t row, const W (&sum)[V]) {
+    Pack<O, V> o;
+    for (int v = 0; v < V; ++v) o.v[v] = (O)(sum[v] * scale);
+    store_pack<O, V>(out + (int64_t)row * r.width + col, o);
   };
-  for (int64_t at = begin; at < end; at += kAhead) {
-    uint32_t key[kAhead];
-    Pack<T, V> g[kAhead];
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) key[u] = r.keys[at + u];
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      if (key[u] < (uint32_t)r.rows) {
-        const uint32_t tk = token[at + u], i = tk / (uint32_t)r.n1, j = tk - i * (uint32_t)r.n1;
-        g[u] = load_pack<T, V>(grad + i * r.g0 + j * r.g1 + col);
+  if (cur < rows) {
+    bool inside = begin == 0 || r.keys[begin - 1] != cur;
+    W acc[V];
+    for (int v = 0; v < V; ++v) acc[v] = 0;
+    auto close = [&] {
+      if (!inside) {
+        flag |= kHasHead;
+        for (int v = 0; v < V; ++v) shead[threadIdx.x * V + v] = acc[v];
+      } else if (live) {
+        write(cur, acc);
       }
+    };
+    for (int64_t at = begin; at < end && cur < rows; at += kAhead) {
+      uint32_t key[kAhead];
+      Pack<T, V> g[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (key[u] != cur) {
+      for (int u = 0; u < kAhead; ++u) key[u] = r.keys[at + u];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (key[u] < rows && live) {
+          const uint32_t tk = token[at + u], i = tk / (uint32_t)r.n1, j = tk - i * (uint32_t)r.n1;
+          g[u] = load_pack<T, V>(grad + i * r.g0 + j * r.g1 + col);
+        }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (key[u] != cur) {
+          if (cur < rows) close();
+          cur = key[u];
+          inside = true;
+          for (int v = 0; v < V; ++v) acc[v] = 0;
+        }
+        if (cur < rows)
+          for (int v = 0; v < V; ++v) acc[v] += (W)g[u].v[v];
+      }
+    }
+    if (cur < rows) {
+      if (end >= r.count || r.keys[end] != cur) {
         close();
-        if (key[u] >= (uint32_t)r.rows) return;
-        cur = key[u];
-        inside = true;
-        for (int v = 0; v < V; ++v) acc[v] = 0;
+      } else {
+        flag |= inside ? kHasTail : kHasHead | kThrough;
+        W* part = inside ? stail : shead;
+        for (int v = 0; v < V; ++v) part[threadIdx.x * V + v] = acc[v];
       }
-      for (int v = 0; v < V; ++v) acc[v] += (W)g[u].v[v];
     }
   }
-  if (end >= r.count || r.keys[end] != cur) {
-    close();
-  } else {
-    W* part = inside ? tail : head;
-    for (int v = 0; v < V; ++v) part[piece * r.width + col + v] = acc[v];
+  if (lane == 0) flags[strip] = flag;
+  __syncthreads();
+  if (!live) return;
+  // the run that begins in this strip and goes on, or (first strip) the one that the piece begins in
+  const bool first = strip == 0 && (flag & kHasHead);
+  for (int from_before = first ? 1 : 0; from_before >= 0; --from_before) {
+    if (!from_before && !(flag & kHasTail)) continue;
+    W sum[V];
+    for (int v = 0; v < V; ++v) sum[v] = (from_before ? shead : stail)[threadIdx.x * V + v];
+    bool open = from_before ? (flag & kThrough) != 0 : true;
+    int q = strip;
+    while (open && q + 1 < strips) {
+      ++q;
+      for (int v = 0; v < V; ++v) sum[v] += shead[(q * group + lane) * V + v];
+      open = (flags[q] & kThrough) != 0;
+    }
+    if (!open && !from_before) write(cur, sum);
+    else
+      for (int v = 0; v < V; ++v) (from_before ? head : tail)[piece * r.width + col + v] = sum[v];
   }
 }
 
@@ -464,7 +497,7 @@ __global__ __launch_bounds__(kThreads) void lookup_grad_narrow_kernel(Runs r, co
 template <typename W, typename O>
 __global__ __launch_bounds__(kThreads) void lookup_grad_join_kernel(Runs r, O* __restrict__ out, const W* __restrict__ head, const W* __restrict__ tail,
                                                                     int64_t piece_tokens, W scale) {
-  const int64_t piece = blockIdx.x, pieces = r.count / piece_tokens, begin = piece * piece_tokens;
+  const int64_t piece = blockIdx.x, pieces = (r.count + piece_tokens - 1) / piece_tokens, begin = piece * piece_tokens;
   if (piece + 1 >= pieces) return;
   const uint32_t row = r.keys[begin + piece_tokens];
   if (row >= (uint32_t)r.rows || r.keys[begin + piece_tokens - 1] != row || (begin && r.keys[begin - 1] == row)) return;
@@ -485,7 +518,7 @@ __global__ __launch_bounds__(kThreads) void lookup_grad_join_kernel(Runs r, O* _
     if (col < r.width) {
       if (part == 0) sum = tail[piece * r.width + col];
       const W* h = head + (piece + 1) * r.width + col;
-#pragma unroll 8
+#pragma unroll 16
       for (int64_t q = from; q < to; ++q) sum += h[q * r.width];
     }
     parts[part][lane] = sum;
@@ -537,7 +570,7 @@ constexpr int64_t kPrivateLds = 65536;
 struct GradPlan {
   TokenGrid grid;
   int64_t g0, g1;
-  int payload, vec, group;
+  int payload, vec, group, strips_long = 1;
   bool values;
   int64_t piece_tokens, pieces, sort_bytes, parts_bytes;
 };
@@ -569,10 +602,11 @@ GradPlan plan_grad(const LookupGradArgs& a) {
         break;
       }
     while (p.group > 8 && p.group / 2 * p.vec >= a.width) p.group /= 2;
-    p.piece_tokens = 32;
-    while (p.piece_tokens < 1024 && tiles.count / p.piece_tokens > 16384) p.piece_tokens *= 2;
+    p.strips_long = 1;
+    while (p.strips_long < 8 && tiles.count / (kStrip * p.strips_long) > 32768) p.strips_long *= 2;
+    p.piece_tokens = (int64_t)kStrip * p.strips_long * (kRunThreads / p.group);
   }
-  p.pieces = tiles.count / p.piece_tokens;
+  p.pieces = (tiles.count + p.piece_tokens - 1) / p.piece_tokens;
   p.sort_bytes = token_sort_workspace(p.grid, p.payload);
   p.parts_bytes = p.pieces * a.width * wide;
   return p;
@@ -590,7 +624,7 @@ struct PrivatePlan {
 
 PrivatePlan plan_private(const LookupGradArgs& a) {
   PrivatePlan p;
-  const int64_t wide = a.type == kF64 ? 8 : 4, tokens = a.n0 * a.n1, lds = a.rows * (a.width * wide + 1);
+  const int64_t wide = a.type == kF64 ? 8 : 4, tokens = a.n0 * a.n1, lds = (a.rows + 1) * (a.width * wide + 1);
   if (a.width > kNarrow || lds > kPrivateLds || tokens < 16 * a.rows) return p;
   p.grid.ids = (const void*)a.ids;
   p.grid.ids64 = (int)a.ids64;
@@ -615,11 +649,10 @@ PrivatePlan plan_private(const LookupGradArgs& a) {
 }
 
 template <typename T, typename O, int V> void launch_runs(const LookupGradArgs& a, const GradPlan& p, const Runs& r, Wide<T>* head, Wide<T>* tail) {
-  const int64_t zero_blocks = (a.rows + kZeroRows * (kThreads / 64) - 1) / (kZeroRows * (kThreads / 64));
-  const int64_t run_blocks = (p.pieces * p.group + kThreads - 1) / kThreads;
-  const dim3 grid((unsigned)(zero_blocks + run_blocks), (unsigned)((a.width + p.group * V - 1) / (p.group * V)));
-  hipLaunchKernelGGL((lookup_grad_runs_kernel<T, O, V>), grid, dim3(kThreads), 0, (hipStream_t)a.stream, r, (const T*)a.grad, (O*)a.out, head, tail,
-                     (int)zero_blocks, p.group, (int)p.piece_tokens, (Wide<T>)a.scale);
+  const int64_t zero_blocks = (a.rows + kZeroRows * (kRunThreads / 64) - 1) / (kZeroRows * (kRunThreads / 64));
+  const dim3 grid((unsigned)(zero_blocks + p.pieces), (unsigned)((a.width + p.group * V - 1) / (p.group * V)));
+  hipLaunchKernelGGL((lookup_grad_runs_kernel<T, O, V>), grid, dim3(kRunThreads), 0, (hipStream_t)a.stream, r, (const T*)a.grad, (O*)a.out, head, tail,
+                     (int)zero_blocks, p.group, p.strips_long, (Wide<T>)a.scale);
 }
 
 template <typename T, typename O> void run_lookup_grad(const LookupGradArgs& a) {
@@ -640,7 +673,7 @@ template <typename T, typename O> void run_lookup_grad(const LookupGradArgs& a) 
     while (a.rows >> bits) ++bits;
     auto run = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3(few.waves), dim3(64), few.lds, s, (const T*)a.grad, few.grid, few.g0, few.g1, (int)a.width, bits, few.items_along0,
-                         few.lines, few.steps, parts);
+                         (int)few.lines, (int)few.steps, (int)((few.steps + few.waves - 1) / few.waves), parts);
     };
     if (a.ids64) few.whole ? run(lookup_grad_private_kernel<T, int64_t, true>) : run(lookup_grad_private_kernel<T, int64_t, false>);
     else few.whole ? run(lookup_grad_private_kernel<T, int32_t, true>) : run(lookup_grad_private_kernel<T, int32_t, false>);

@@ -173,10 +173,10 @@ __global__ __launch_bounds__(kThreads) void sort_scatter_kernel(Pass p, const ui
       const uint32_t* row = offsets + (int64_t)t * p.tiles.blocks;
       if (p.few) {
 #pragma unroll 8
-        for (int q = 0; q < (int)p.tiles.blocks; ++q) {
-          const uint32_t c = row[q];
-          total += c;
-          if (q < (int)b) ahead += c;
+        for (int q = 0; q < (int)p.tiles.blocks; q += 4) {       // a multiple of 4
+          const uint4 c = *(const uint4*)(row + q);
+          total += c.x + c.y + c.z + c.w;
+          ahead += (q < (int)b ? c.x : 0) + (q + 1 < (int)b ? c.y : 0) + (q + 2 < (int)b ? c.z : 0) + (q + 3 < (int)b ? c.w : 0);
         }
       } else {
         total = totals[t];
@@ -273,7 +273,7 @@ SortedTokens token_sort(const TokenGrid& g, const void* values, int64_t v0, int6
   const bool small = tiles.bits == 10;
   const dim3 grid((unsigned)tiles.blocks), block(kThreads);
   uint32_t *counts = (uint32_t*)(w + l.counts), *totals = (uint32_t*)(w + l.totals);
-  Pass p{g, tiles, nullptr, values, v0, v1, 0, each, tiles.blocks <= kFewTiles};
+  Pass p{g, tiles, nullptr, values, v0, v1, 0, each, small};
   for (int k = 0; k < passes; ++k) {
     p.shift = k * each;
     p.bits = std::min(each, bits - p.shift);

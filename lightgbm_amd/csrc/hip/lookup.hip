@@ -158,21 +158,21 @@ constexpr int kPrivateItems = 16;     // tokens a lane holds
 
 // A step: 64 x kPrivateItems tokens; lanes along axis 0, items along axis 1 or (few tokens there) along axis 0 too.  A step
 // is loaded while the one before is added up.  kWhole: a lane's gradients of a step are neighbours and loaded as packs.
-template <typename T, typename I, bool kWhole>
+template <typename T, typename I, bool kAlong0, bool kWhole>
 __global__ __launch_bounds__(64) void lookup_grad_private_kernel(const T* __restrict__ grad, TokenGrid grid, int64_t g0, int64_t g1, int width, int row_bits,
-                                                                 int items_along0, int lines, int steps, int each, Wide<T>* __restrict__ parts) {
+                                                                 int lines, int steps, int each, Wide<T>* __restrict__ parts) {
   typedef Wide<T> W;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   W* sums = (W*)lds;                  // one row more than the table has: tokens that take no part
   const int rows = (int)grid.rows, values = rows * width, lane = threadIdx.x;
-  volatile uint8_t* tag = (volatile uint8_t*)(sums + values + width);
+  uint8_t* tag = (uint8_t*)(sums + values + width);
   for (int k = lane; k < values + width; k += 64) sums[k] = 0;
   __syncthreads();
-  const int64_t item_i = items_along0 ? 64 : 0, item_j = items_along0 ? 0 : 1;
+  constexpr int item_i = kAlong0 ? 64 : 0, item_j = kAlong0 ? 0 : 1;
   auto place = [&](int step, int64_t& i0, int64_t& j0) {
     const int si = step / lines, line = step - si * lines;
-    i0 = (int64_t)si * 64 * (items_along0 ? kPrivateItems : 1) + lane;
-    j0 = (int64_t)line * (items_along0 ? 1 : kPrivateItems);
+    i0 = (int64_t)si * 64 * (kAlong0 ? kPrivateItems : 1) + lane;
+    j0 = (int64_t)line * (kAlong0 ? 1 : kPrivateItems);
   };
   // places behind the edge are read at the edge and take no part later
   auto load = [&](int step, I (&id)[kPrivateItems], T (&g)[kPrivateItems]) {
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(64) void lookup_grad_private_kernel(const T* __rest
     const I* ids = (const I*)grid.ids;
 #pragma unroll
     for (int u = 0; u < kPrivateItems; ++u) id[u] = ids[min(i0 + u * item_i, grid.n0 - 1) * grid.s0 + min(j0 + u * item_j, grid.n1 - 1) * grid.s1];
-    if (kWhole && j0 + kPrivateItems <= grid.n1) {
+    if (kWhole && !kAlong0 && j0 + kPrivateItems <= grid.n1) {
       constexpr int kPack = 16 / sizeof(T);
       const T* from = grad + min(i0, grid.n0 - 1) * g0 + j0;
 #pragma unroll
@@ -214,7 +214,9 @@ __global__ __launch_bounds__(64) void lookup_grad_private_kernel(const T* __rest
 #pragma unroll
     for (int u = 0; u < kPrivateItems; ++u) {
       tag[row[u]] = (uint8_t)lane;
+      in_order();
       seen[u] = tag[row[u]];
+      in_order();
     }
 #pragma unroll
     for (int u = 0; u < kPrivateItems; ++u) {
@@ -672,11 +674,16 @@ template <typename T, typename O> void run_lookup_grad(const LookupGradArgs& a) 
     int bits = 1;
     while (a.rows >> bits) ++bits;
     auto run = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(few.waves), dim3(64), few.lds, s, (const T*)a.grad, few.grid, few.g0, few.g1, (int)a.width, bits, few.items_along0,
+      hipLaunchKernelGGL(kernel, dim3(few.waves), dim3(64), few.lds, s, (const T*)a.grad, few.grid, few.g0, few.g1, (int)a.width, bits,
                          (int)few.lines, (int)few.steps, (int)((few.steps + few.waves - 1) / few.waves), parts);
     };
-    if (a.ids64) few.whole ? run(lookup_grad_private_kernel<T, int64_t, true>) : run(lookup_grad_private_kernel<T, int64_t, false>);
-    else few.whole ? run(lookup_grad_private_kernel<T, int32_t, true>) : run(lookup_grad_private_kernel<T, int32_t, false>);
+    auto by_ids = [&](auto id) {
+      typedef decltype(id) I;
+      if (few.items_along0) run(lookup_grad_private_kernel<T, I, true, false>);
+      else if (few.whole) run(lookup_grad_private_kernel<T, I, false, true>);
+      else run(lookup_grad_private_kernel<T, I, false, false>);
+    };
+    a.ids64 ? by_ids((int64_t)0) : by_ids((int32_t)0);
     LGA_HIP_CHECK(hipGetLastError());
     hipLaunchKernelGGL((lookup_grad_total_kernel<W, O>), dim3((unsigned)((values + 63) / 64)), dim3(kThreads), 0, s, parts, (O*)a.out, values, few.waves,
                        (W)a.scale);

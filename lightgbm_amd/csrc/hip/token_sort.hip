@@ -153,11 +153,12 @@ __global__ __launch_bounds__(kThreads) void sort_scatter_kernel(Pass p, const ui
       const uint64_t ones = __ballot(one);
       same &= one ? ones : ~ones;
     }
-    volatile uint32_t* const mine = &count[wave][digit];     // other lanes of the wave write it between two keys
-    const uint32_t before = *mine;
+    in_order();                        // other lanes of the wave write the counters between two keys
+    const uint32_t before = count[wave][digit];
+    in_order();
     const int lower = __popcll(same & ((1ull << lane) - 1));
     rank[k] = before + (uint32_t)lower;
-    if (lower == 0) *mine = before + (uint32_t)__popcll(same);
+    if (lower == 0) count[wave][digit] = before + (uint32_t)__popcll(same);
   }
   __syncthreads();
   // one lane a digit: keys of the digit in the waves before, in the tile, in the digits below (of the tile and of all)

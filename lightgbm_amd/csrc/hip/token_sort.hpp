@@ -23,6 +23,10 @@ struct TokenTiles {
 // `bits`: 12, or 10 for small tiles.
 TokenTiles token_tiles(const TokenGrid& g, int bits = 12);
 
+// LDS accesses of a wave run in program order; this keeps the compiler from moving or merging them across this point, as
+// it could for accesses of one lane.
+__device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
+
 // Where item q of a tile stands in LDS: tiles are written along one axis and read along the other, and this way neither
 // walk meets a bank twice.
 __device__ __forceinline__ int tile_slot(int q) { return (q & ~63) | ((q ^ (q >> 6)) & 63); }

@@ -149,15 +149,18 @@ __global__ __launch_bounds__(kThreads) void lookup_grad_owned_kernel(const T* __
       if (first + r < rows) out[(first + r) * width + col] = (O)(acc[r][t] * scale);
 }
 
-// Few rows, many tokens: every wave keeps sums of the whole table in LDS and adds its tokens to them one wave of 64 at a
-// time; the waves' sums are added up in order afterwards.  LDS instructions of one wave run in their order, and no two lanes
-// of one add share an address, so the order of additions is fixed:  tag[row] = lane, read back, tells whether all rows of
-// the 64 differ (whichever of two lanes is read back, one of them sees the other); if not, lanes of one row find each other
-// with ballots and take turns.
-constexpr int kPrivateItems = 16;     // tokens a lane holds
+// Few rows, many tokens: every wave keeps sums of the whole table in LDS and adds its tokens to them, kGroup x 64 at a
+// time; the waves' sums are added up in order afterwards.  LDS accesses of one wave run in their order, so the additions
+// have a fixed order as long as no two lanes touch one row at a time:  tag[row] = lane, read back, tells whether lanes share
+// a row (whichever of two lanes is read back, the other one sees it); if so, they find each other with ballots and
+// take turns.  LDS float atomics would need no reading back, but take about 200 cycles for 64 lanes: 130 us for the 13.7 M
+// tokens of 300 trees x 45800 rows, where this takes 63 us (a third of it waits for loads: LDS holds three waves a CU).
+constexpr int kPrivateItems = 32;     // tokens a lane holds
+constexpr int kGroup = 4;             // of which so many are added at a time
 
 // A step: 64 x kPrivateItems tokens; lanes along axis 0, items along axis 1 or (few tokens there) along axis 0 too.  A step
-// is loaded while the one before is added up.  kWhole: a lane's gradients of a step are neighbours and loaded as packs.
+// is loaded while the one before is added up.  kWhole: gradients of one
+// value that are neighbours along axis 1 and start at multiples of 16 bytes.
 template <typename T, typename I, bool kAlong0, bool kWhole>
 __global__ __launch_bounds__(64) void lookup_grad_private_kernel(const T* __restrict__ grad, TokenGrid grid, int64_t g0, int64_t g1, int width, int row_bits,
                                                                  int lines, int steps, int each, Wide<T>* __restrict__ parts) {
@@ -174,25 +177,42 @@ __global__ __launch_bounds__(64) void lookup_grad_private_kernel(const T* __rest
     i0 = (int64_t)si * 64 * (kAlong0 ? kPrivateItems : 1) + lane;
     j0 = (int64_t)line * (kAlong0 ? 1 : kPrivateItems);
   };
-  // places behind the edge are read at the edge and take no part later
+  const I* ids = (const I*)grid.ids;
+  // All of a lane's items are there; a lane behind the edge of axis 0 reads the last ones and takes no part.
+  auto inner = [&](int64_t i0, int64_t j0) {
+    return kAlong0 ? i0 - lane + 64 * kPrivateItems <= grid.n0 : j0 + kPrivateItems <= grid.n1;
+  };
   auto load = [&](int step, I (&id)[kPrivateItems], T (&g)[kPrivateItems]) {
     int64_t i0, j0;
     place(step, i0, j0);
-    const I* ids = (const I*)grid.ids;
+    if (inner(i0, j0)) {
+      i0 = min(i0, grid.n0 - 1);
+      const I* at = ids + i0 * grid.s0 + j0 * grid.s1;
+      const int64_t next = kAlong0 ? 64 * grid.s0 : grid.s1;
 #pragma unroll
-    for (int u = 0; u < kPrivateItems; ++u) id[u] = ids[min(i0 + u * item_i, grid.n0 - 1) * grid.s0 + min(j0 + u * item_j, grid.n1 - 1) * grid.s1];
-    if (kWhole && !kAlong0 && j0 + kPrivateItems <= grid.n1) {
-      constexpr int kPack = 16 / sizeof(T);
-      const T* from = grad + min(i0, grid.n0 - 1) * g0 + j0;
+      for (int u = 0; u < kPrivateItems; ++u) id[u] = at[u * next];
+      const T* from = grad + i0 * g0 + j0 * g1;
+      if constexpr (kWhole) {
+        constexpr int kPack = 16 / sizeof(T);
 #pragma unroll
-      for (int u = 0; u < kPrivateItems; u += kPack) {
-        const Pack<T, kPack> x = load_pack<T, kPack>(from + u);
+        for (int u = 0; u < kPrivateItems; u += kPack) {
+          const Pack<T, kPack> x = load_pack<T, kPack>(from + u);
 #pragma unroll
-        for (int v = 0; v < kPack; ++v) g[u + v] = x.v[v];
+          for (int v = 0; v < kPack; ++v) g[u + v] = x.v[v];
+        }
+      } else {
+        const int64_t on = kAlong0 ? 64 * g0 : g1;
+#pragma unroll
+        for (int u = 0; u < kPrivateItems; ++u) g[u] = from[u * on];
       }
     } else {
 #pragma unroll
-      for (int u = 0; u < kPrivateItems; ++u) g[u] = grad[min(i0 + u * item_i, grid.n0 - 1) * g0 + min(j0 + u * item_j, grid.n1 - 1) * g1];
+      for (int u = 0; u < kPrivateItems; ++u) {
+        const int64_t i = i0 + u * item_i, j = j0 + u * item_j;
+        id[u] = -1;
+        g[u] = (T)0.f;
+        if (i < grid.n0 && j < grid.n1) id[u] = ids[i * grid.s0 + j * grid.s1], g[u] = grad[i * g0 + j * g1];
+      }
     }
   };
   int32_t row[kPrivateItems];
@@ -203,44 +223,78 @@ __global__ __launch_bounds__(64) void lookup_grad_private_kernel(const T* __rest
   for (int step = blockIdx.x * each; step < end; ++step) {
     int64_t i0, j0;
     place(step, i0, j0);
+    const int limit = i0 < grid.n0 ? rows : 0;
 #pragma unroll
     for (int u = 0; u < kPrivateItems; ++u) {
-      const bool there = i0 + u * item_i < grid.n0 && j0 + u * item_j < grid.n1;
-      row[u] = there && next_id[u] >= 0 && next_id[u] < rows ? (int32_t)next_id[u] : rows;
+      row[u] = next_id[u] >= 0 && next_id[u] < limit ? (int32_t)next_id[u] : rows;
       g[u] = next_g[u];
     }
     if (step + 1 < end) load(step + 1, next_id, next_g);
-    uint8_t seen[kPrivateItems];
+    const T* from = grad + i0 * g0 + j0 * g1;
+    uint32_t meets = 0;               // groups of items in which lanes share a row: later, read once more
 #pragma unroll
-    for (int u = 0; u < kPrivateItems; ++u) {
-      tag[row[u]] = (uint8_t)lane;
+    for (int u0 = 0; u0 < kPrivateItems; u0 += kGroup) {
+      uint8_t seen[kGroup];
+      W sum[kGroup];
+#pragma unroll
+      for (int k = 0; k < kGroup; ++k) tag[row[u0 + k]] = (uint8_t)lane;
       in_order();
-      seen[u] = tag[row[u]];
+#pragma unroll
+      for (int k = 0; k < kGroup; ++k) seen[k] = tag[row[u0 + k]];
+#pragma unroll
+      for (int k = 0; k < kGroup; ++k) sum[k] = sums[row[u0 + k] * width];
+      bool other = false;
+#pragma unroll
+      for (int k = 0; k < kGroup; ++k) other |= row[u0 + k] < rows && seen[k] != (uint8_t)lane;
+      if (__any(other)) {
+        meets |= 1u << u0;
+      } else {
+        // a lane's own items of one row follow each other in registers; the last one is stored last
+#pragma unroll
+        for (int k = 0; k < kGroup; ++k) {
+#pragma unroll
+          for (int e = 0; e < k; ++e) sum[k] = row[u0 + e] == row[u0 + k] ? sum[e] : sum[k];
+          sum[k] += (W)g[u0 + k];
+        }
+#pragma unroll
+        for (int k = 0; k < kGroup; ++k) {
+          sums[row[u0 + k] * width] = sum[k];
+          in_order();
+        }
+        for (int c = 1; c < width; ++c)
+#pragma unroll
+          for (int k = 0; k < kGroup; ++k) {
+            if (row[u0 + k] < rows) sums[row[u0 + k] * width + c] += (W)from[(u0 + k) * item_i * g0 + (u0 + k) * item_j * g1 + c];
+            in_order();
+          }
+      }
       in_order();
     }
-#pragma unroll
-    for (int u = 0; u < kPrivateItems; ++u) {
-      W* at = sums + row[u] * width;
-      const T* more = grad + (i0 + u * item_i) * g0 + (j0 + u * item_j) * g1;
-      auto add = [&] {
-        unsafeAtomicAdd(at, (W)g[u]);
-        if (width > 1 && row[u] < rows)
-          for (int c = 1; c < width; ++c) unsafeAtomicAdd(at + c, (W)more[c]);
-      };
-      if (!__any(row[u] < rows && seen[u] != (uint8_t)lane)) {
-        add();
-      } else {                        // two lanes share a row
+    for (; meets; meets &= meets - 1) {
+      const int u0 = __ffs(meets) - 1;
+      for (int u = u0; u < u0 + kGroup; ++u) {
+        const int64_t i = i0 + u * item_i, j = j0 + u * item_j;
+        const bool there = i < grid.n0 && j < grid.n1;
+        const I id = there ? ids[i * grid.s0 + j * grid.s1] : (I)-1;
+        const W value = there ? (W)grad[i * g0 + j * g1] : (W)0;
+        const int at = id >= 0 && id < rows ? (int)id : rows;
         uint64_t same = ~0ull;
         for (int bit = 0; bit < row_bits; ++bit) {
-          const bool one = row[u] >> bit & 1;
+          const bool one = at >> bit & 1;
           const uint64_t ones = __ballot(one);
           same &= one ? ones : ~ones;
         }
-        const int turn = row[u] < rows ? __popcll(same & ((1ull << lane) - 1)) : -1;
-        for (int k = 0; __any(turn >= k); ++k)
-          if (turn == k) add();
+        const int turn = at < rows ? __popcll(same & ((1ull << lane) - 1)) : -1;
+        for (int k = 0; __any(turn >= k); ++k) {
+          if (turn == k) {
+            sums[at * width] += value;
+            for (int c = 1; c < width; ++c) sums[at * width + c] += (W)from[u * item_i * g0 + u * item_j * g1 + c];
+          }
+          in_order();
+        }
       }
     }
+    in_order();
   }
   __syncthreads();
   for (int k = lane; k < values; k += 64) parts[(int64_t)blockIdx.x * values + k] = sums[k];
@@ -566,8 +620,7 @@ template <typename T> void run_lookup(const LookupArgs& a) {
 
 // Up to this many tokens every workgroup looks through all ids for its own rows; above, they are sorted.
 constexpr int64_t kOwnedTokens = 2048;
-// LDS a wave may take for sums of the whole table.
-constexpr int64_t kPrivateLds = 65536;
+constexpr int64_t kPrivateLds = 65536;      // of a wave, for sums of the whole table
 
 struct GradPlan {
   TokenGrid grid;

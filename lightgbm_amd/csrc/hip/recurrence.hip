@@ -5,7 +5,7 @@
 // Behind a sequence's length the state is kept and nothing is read: whatever stands there cannot reach a result.
 //
 // A run of steps is an affine map h -> A h + H, and maps compose associatively: (A, H) after (A', H') is
-// (A A', A H' + H).  The steps are cut into chunks of kSteps that one lane holds in registers, kSlots chunks make a tile
+// (A A', A H' + H).  The steps are cut into chunks that one lane holds in registers, up to kMaxSlots chunks make a tile
 // (one workgroup, 64 channel packs wide).  A tile folds its chunks through LDS, hands its map to the tiles behind it
 // through memory, folds the maps before it, and then walks its chunks again from the exact state before each: every
 // value is read once and written once.  All folds run in the order of the steps, so results do not depend on timing.
@@ -20,8 +20,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kLanes = 64;          // channel packs of a tile
-constexpr int kSteps = 16;          // steps a lane holds
-constexpr int kMaxSlots = 8;        // chunks of a tile
+constexpr int kScanSteps = 16, kGradSteps = 8;      // steps a lane holds
+constexpr int kMaxSlots = 16;       // chunks of a tile
 constexpr int kCheckpoint = 32;     // every 32nd tile hands on the state itself, so that no tile folds more than 31 maps
 constexpr uint64_t kEmpty = ~0ull;  // a word nobody has written yet: a NaN that publish() never stores
 
@@ -380,28 +380,36 @@ __global__ __launch_bounds__(kLanes* kMaxSlots) void scan_grad_kernel(ScanGradAr
     for (int v = 0; v < V; ++v) ((W*)a.grad_state)[c + v] = e[v];
 }
 
-// grad_gate[q][t][g] = sum of the slopes of the sequences and channels that share the gate, in a fixed order:
-// lanes over them, then a tree.
-template <typename W, typename G>
+// grad_gate[q][t][g] = sum of the slopes of the sequences and channels that share the gate, in a fixed order: `team` lanes
+// (a wave, or the workgroup where more than kWaveTerms share a gate) side by side, then a tree.
+constexpr int64_t kWaveTerms = 2048;
+
+template <typename W, typename G, int kTeam>
 __global__ __launch_bounds__(kThreads) void gate_sum_kernel(const W* __restrict__ slope, G* __restrict__ out, int64_t batch, int64_t steps,
                                                             int64_t width, int64_t groups, int64_t gate_batch) {
-  __shared__ W part[kThreads];
-  const int64_t per = width / groups, shared = gate_batch == batch ? 1 : batch;
-  for (int64_t o = blockIdx.x; o < gate_batch * steps * groups; o += gridDim.x) {
-    const int64_t q = o / (steps * groups), t = o / groups % steps, g = o % groups;
+  __shared__ W part[kThreads / 64];
+  const int64_t per = width / groups, shared = gate_batch == batch ? 1 : batch, sums = gate_batch * steps * groups;
+  const int lane = threadIdx.x % kTeam;
+  for (int64_t base = (int64_t)blockIdx.x * (kThreads / kTeam); base < sums; base += (int64_t)gridDim.x * (kThreads / kTeam)) {
+    const int64_t o = base + threadIdx.x / kTeam;
     W sum = 0;
-    for (int64_t k = threadIdx.x; k < shared * per; k += kThreads) {
-      const int64_t b = q + k / per, d = g * per + k % per;
-      sum += slope[(b * steps + t) * width + d];
+    if (o < sums) {
+      const int64_t qt = o / groups, g = o - qt * groups, q = qt / steps, t = qt - q * steps;
+      for (int64_t b = q; b < q + shared; ++b) {
+        const W* row = slope + (b * steps + t) * width + g * per;
+#pragma unroll 4
+        for (int64_t d = lane; d < per; d += kTeam) sum += row[d];
+      }
     }
-    part[threadIdx.x] = sum;
-    __syncthreads();
-    for (int s = kThreads / 2; s; s >>= 1) {
-      if ((int)threadIdx.x < s) part[threadIdx.x] += part[threadIdx.x + s];
+    for (int s = 32; s; s >>= 1) sum += __shfl_xor(sum, s);
+    if constexpr (kTeam > 64) {
+      if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = sum;
+      __syncthreads();
+      sum = 0;
+      for (int w = 0; w < kThreads / 64; ++w) sum += part[w];
       __syncthreads();
     }
-    if (threadIdx.x == 0) out[o] = (G)part[0];
-    __syncthreads();
+    if (lane == 0 && o < sums) out[o] = (G)sum;
   }
 }
 
@@ -419,20 +427,24 @@ bool two_wide(const ScanGradArgs& a) {
   return even_rows(a) && a.g_b % 2 == 0 && a.g_t % 2 == 0 && a.h_b % 2 == 0 && a.h_t % 2 == 0 && aligned(a.grad_states, size) && aligned(a.states, size);
 }
 
-Cut cut_steps(int64_t batch, int64_t steps, int64_t width, int v, int per_lane) {
+Cut cut_steps(int64_t batch, int64_t steps, int64_t width, int v, int per_lane, int max_slots) {
   Cut k;
   k.packs = batch * width / v;
   k.lanes = kLanes;
   while (k.lanes > 1 && k.lanes / 2 >= k.packs) k.lanes /= 2;
   const int64_t chunks = std::max<int64_t>(1, (steps + per_lane - 1) / per_lane);
   k.slots = 1;
-  while (k.slots < kMaxSlots && k.slots < chunks) k.slots *= 2;
+  while (k.slots < max_slots && k.slots < chunks) k.slots *= 2;
   k.tiles = (chunks + k.slots - 1) / k.slots;
   if (k.tiles == 1 && k.slots == 1) k.lanes = k.packs >= kThreads ? kThreads : k.lanes;
   k.pack_rows = (k.packs + k.lanes - 1) / k.lanes;
   if (k.tiles * k.pack_rows > 2147483647LL) throw std::runtime_error("gated_scan: the tensor is too large");
   return k;
 }
+
+// Two workgroups of 8 chunks a CU overlap loads with sums better than one of 16 (8 x 4096 x 2560 bf16: 156 against 161 us),
+// but a long sequence has fewer maps to fold in larger tiles (1 x 65537 x 1024 bf16: 116 against 128 us).
+int scan_slots(const ScanArgs& a) { return a.steps > 64 * 8 * kScanSteps ? kMaxSlots : 8; }
 
 template <typename A> void check_args(const A& a) {
   if (a.batch < 0 || a.steps < 0 || a.width < 0) throw std::runtime_error("gated_scan: a negative size");
@@ -455,12 +467,12 @@ template <typename F> auto by_types(int64_t type, int64_t gate_type, bool gate, 
 template <int N> struct Const { static constexpr int value = N; };
 
 // f(gate kind, channels a lane, steps a lane)
-template <bool Two, typename A, typename F> void by_shape(const A& a, F f) {
+template <bool Two, int Steps, typename A, typename F> void by_shape(const A& a, F f) {
   auto with_kind = [&](auto kind) {
     if constexpr (Two) {
-      if (two_wide(a)) return a.steps <= 1 ? f(kind, Const<2>(), Const<1>()) : f(kind, Const<2>(), Const<kSteps>());
+      if (two_wide(a)) return a.steps <= 1 ? f(kind, Const<2>(), Const<1>()) : f(kind, Const<2>(), Const<Steps>());
     }
-    return a.steps <= 1 ? f(kind, Const<1>(), Const<1>()) : f(kind, Const<1>(), Const<kSteps>());
+    return a.steps <= 1 ? f(kind, Const<1>(), Const<1>()) : f(kind, Const<1>(), Const<Steps>());
   };
   if (!a.gate) with_kind(Const<kNoGate>());
   else if (a.groups == a.width) with_kind(Const<kOwnGate>());
@@ -483,7 +495,7 @@ bool sums_gates(const ScanGradArgs& a) { return a.gate && (a.groups != a.width |
 int64_t scan_workspace(const ScanArgs& a) {
   check_args(a);
   const int v = two_wide(a) ? 2 : 1;
-  const Cut k = cut_steps(a.batch, a.steps, a.width, v, a.steps <= 1 ? 1 : kSteps);
+  const Cut k = cut_steps(a.batch, a.steps, a.width, v, a.steps <= 1 ? 1 : kScanSteps, scan_slots(a));
   return 8 * (a.type == kF64 ? work_words<double>(k, v) : work_words<float>(k, v));
 }
 
@@ -494,9 +506,9 @@ void gated_scan(const ScanArgs& a) {
   by_types(a.type, a.gate_type, a.gate != 0, [&](auto tt, auto gg) {
     typedef decltype(tt) T;
     typedef decltype(gg) G;
-    by_shape<sizeof(T) < 8>(a, [&](auto kind, auto v, auto l) {
+    by_shape<sizeof(T) < 8, kScanSteps>(a, [&](auto kind, auto v, auto l) {
       constexpr int V = decltype(v)::value, L = decltype(l)::value;
-      const Cut k = cut_steps(a.batch, a.steps, a.width, V, L);
+      const Cut k = cut_steps(a.batch, a.steps, a.width, V, L, scan_slots(a));
       clear_work<Wide<T>>(k, V, (uint64_t*)a.work, (hipStream_t)a.stream);
       hipLaunchKernelGGL((scan_kernel<T, G, (GateKind)decltype(kind)::value, V, L>), dim3((unsigned)(k.tiles * k.pack_rows)), dim3(k.lanes * k.slots),
                          fold_bytes<Wide<T>>(k, V), (hipStream_t)a.stream, a, k);
@@ -508,7 +520,7 @@ void gated_scan(const ScanArgs& a) {
 int64_t scan_grad_workspace(const ScanGradArgs& a) {
   check_args(a);
   const int v = two_wide(a) ? 2 : 1;
-  const Cut k = cut_steps(a.batch, a.steps, a.width, v, a.steps <= 1 ? 1 : kSteps);
+  const Cut k = cut_steps(a.batch, a.steps, a.width, v, a.steps <= 1 ? 1 : kGradSteps, kMaxSlots);
   const int64_t slopes = sums_gates(a) ? a.batch * a.steps * a.width * (a.type == kF64 ? 8 : 4) : 0;
   return 8 * (a.type == kF64 ? work_words<double>(k, v) : work_words<float>(k, v)) + slopes;
 }
@@ -522,9 +534,9 @@ void gated_scan_grad(const ScanGradArgs& a) {
     typedef decltype(gg) G;
     typedef Wide<T> W;
     const hipStream_t s = (hipStream_t)a.stream;
-    by_shape<sizeof(T) < 8>(a, [&](auto kind, auto v, auto l) {
+    by_shape<sizeof(T) < 8, kGradSteps>(a, [&](auto kind, auto v, auto l) {
       constexpr int V = decltype(v)::value, L = decltype(l)::value;
-      const Cut k = cut_steps(a.batch, a.steps, a.width, V, L);
+      const Cut k = cut_steps(a.batch, a.steps, a.width, V, L, kMaxSlots);
       uint64_t* work = (uint64_t*)a.work;
       clear_work<W>(k, V, work, s);
       const int64_t slopes = sums_gates(a) ? (int64_t)(work + work_words<W>(k, V)) : 0;
@@ -532,9 +544,13 @@ void gated_scan_grad(const ScanGradArgs& a) {
                          fold_bytes<W>(k, V), s, a, k, work, slopes);
       LGA_HIP_CHECK(hipGetLastError());
       if (slopes) {
-        const int64_t sums = a.gate_batch * a.steps * a.groups;
-        hipLaunchKernelGGL((gate_sum_kernel<W, G>), dim3((unsigned)std::min<int64_t>(sums, 1 << 20)), dim3(kThreads), 0, s, (const W*)slopes, (G*)a.grad_gate,
-                           a.batch, a.steps, a.width, a.groups, a.gate_batch);
+        const int64_t sums = a.gate_batch * a.steps * a.groups, terms = a.width / a.groups * (a.batch / a.gate_batch);
+        auto run = [&](auto kernel, int64_t team) {
+          hipLaunchKernelGGL(kernel, dim3((unsigned)std::min<int64_t>((sums * team + kThreads - 1) / kThreads, 1 << 20)), dim3(kThreads), 0, s,
+                             (const W*)slopes, (G*)a.grad_gate, a.batch, a.steps, a.width, a.groups, a.gate_batch);
+        };
+        if (terms <= kWaveTerms) run(gate_sum_kernel<W, G, 64>, 64);
+        else run(gate_sum_kernel<W, G, kThreads>, kThreads);
         LGA_HIP_CHECK(hipGetLastError());
       }
     });

@@ -109,7 +109,7 @@ def _declare(lib, hip: bool):
             "lga_hip_comm_create_rccl": (c_int, [c_int, c_int, c_void_p, c_int, P(c_void_p)]),
             "lga_hip_comm_create_loopback_group": (c_int, [c_int, P(c_void_p)]),
             "lga_hip_op": (c_int, [c_char_p, P(c_void_p), c_int, P(c_int64), c_int]),
-            "lga_hip_embedding": (c_int, [c_char_p]),
+            "lga_hip_embedding": (c_int, [c_char_p, P(c_int64)]),
             "lga_hip_embedding_grad": (c_int, [c_char_p, P(c_int64)]),
             "lga_hip_gated_scan": (c_int, [c_char_p, P(c_int64)]),
             "lga_hip_gated_scan_grad": (c_int, [c_char_p, P(c_int64)]),

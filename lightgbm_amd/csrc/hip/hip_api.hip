@@ -174,31 +174,37 @@ int lga_hip_op(const char* name, void** ptrs, int nptr, const int64_t* ints, int
 // Row lookup and gated recurrence (ops/lookup.py, ops/recurrence.py): `args` holds the words of the structure of that
 // name in lookup.hpp / recurrence.hpp, copied because the caller's bytes need not be aligned.  Nothing is synchronised;
 // the work goes to the stream named in `args`.
-int lga_hip_embedding(const void* args) {
-  return hguard([&] { LookupArgs a; std::memcpy(&a, args, sizeof a); lookup(a); });
+// `workspace` is set to the bytes that have to be at `work`; where those are missing (work == 0) nothing is launched.
+int lga_hip_embedding(const void* args, int64_t* workspace) {
+  return hguard([&] {
+    LookupArgs a;
+    std::memcpy(&a, args, sizeof a);
+    *workspace = 0;
+    lookup(a);
+  });
 }
 int lga_hip_embedding_grad(const void* args, int64_t* workspace) {
   return hguard([&] {
     LookupGradArgs a;
     std::memcpy(&a, args, sizeof a);
-    if (workspace) *workspace = lookup_grad_workspace(a);
-    else lookup_grad(a);
+    *workspace = lookup_grad_workspace(a);
+    if (a.work || !*workspace) lookup_grad(a);
   });
 }
 int lga_hip_gated_scan(const void* args, int64_t* workspace) {
   return hguard([&] {
     ScanArgs a;
     std::memcpy(&a, args, sizeof a);
-    if (workspace) *workspace = scan_workspace(a);
-    else gated_scan(a);
+    *workspace = scan_workspace(a);
+    if (a.work || !*workspace) gated_scan(a);
   });
 }
 int lga_hip_gated_scan_grad(const void* args, int64_t* workspace) {
   return hguard([&] {
     ScanGradArgs a;
     std::memcpy(&a, args, sizeof a);
-    if (workspace) *workspace = scan_grad_workspace(a);
-    else gated_scan_grad(a);
+    *workspace = scan_grad_workspace(a);
+    if (a.work || !*workspace) gated_scan_grad(a);
   });
 }
 

@@ -3,12 +3,13 @@ from __future__ import annotations
 
 import ctypes
 
+import torch
+
 from .. import _lib
 from .._lib import LightGBMError
 
 _core = None
-_TYPE_CODES = {}
-_FLOATS = ("bfloat16", "float16", "float32", "float64")
+_TYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2, torch.float64: 3}
 
 
 def core():
@@ -24,9 +25,6 @@ def core():
 
 def type_code(dtype) -> int:
     """0..3 for bf16, fp16, fp32, fp64; -1 for every other type."""
-    if not _TYPE_CODES:
-        import torch
-        _TYPE_CODES.update({getattr(torch, name): i for i, name in enumerate(_FLOATS)})
     return _TYPE_CODES.get(dtype, -1)
 
 
@@ -35,22 +33,20 @@ def fail(what: str):
 
 
 def need_tensor(op: str, name: str, t):
-    import torch
     if not isinstance(t, torch.Tensor):
         fail(f"{op}: {name} has to be a torch tensor, got {type(t).__name__}")
     if t.requires_grad and torch.is_grad_enabled():
         fail(f"{op}: {name} requires grad, and nothing is recorded here: call it under torch.no_grad() and take the gradient from {op}_grad")
-    return t
 
 
 def need_type(op: str, name: str, t) -> int:
-    code = type_code(t.dtype)
+    code = _TYPE_CODES.get(t.dtype, -1)
     if code < 0:
         fail(f"{op}: {name} has to be bfloat16, float16, float32 or float64, got {t.dtype}")
     return code
 
 
-def need_device(op: str, first, *others):
+def need_device(op: str, first, *others) -> int:
     """All tensors on one GPU; returns its index."""
     device = first.device
     for t in others:
@@ -62,25 +58,26 @@ def need_device(op: str, first, *others):
 
 
 def stream_of(device: int) -> int:
-    import torch
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def launch(fn, args: bytes) -> None:
-    if fn(args, None) != 0:
+def run(fn, pack, device) -> None:
+    """Calls the core with the words that ``pack(address of the workspace)`` gives.  Without a workspace the core launches
+    only what needs none and says how much is missing."""
+    need = ctypes.c_int64()
+    if fn(pack(0), need) != 0:
         _lib.check(-1)
-
-
-def workspace_bytes(fn, args: bytes) -> int:
-    n = ctypes.c_int64()
-    if fn(args, ctypes.byref(n)) != 0:
-        _lib.check(-1)
-    return n.value
+    if need.value:
+        work = torch.empty(need.value, dtype=torch.uint8, device=device)
+        if fn(pack(work.data_ptr()), need) != 0:
+            _lib.check(-1)
 
 
 def two_dims(shape, *strides):
     """Merges neighbouring dimensions that every stride tuple walks evenly.  Returns (sizes, [strides, ...]) of two
     dimensions, or None if more are left."""
+    if len(shape) == 1:
+        return (1, shape[0]), [(0, s[0]) for s in strides]
     sizes, kept = [], [[] for _ in strides]
     for d, n in enumerate(shape):
         if n == 1:

@@ -9,7 +9,9 @@ from __future__ import annotations
 
 import struct
 
-from ._args import core, fail, launch, need_device, need_tensor, need_type, stream_of, two_dims, type_code, workspace_bytes
+import torch
+
+from ._args import core, fail, need_device, need_tensor, need_type, run, stream_of, two_dims, type_code
 
 _LOOKUP = struct.Struct("14qd")
 _LOOKUP_GRAD = struct.Struct("17qd")
@@ -17,7 +19,6 @@ _MAX_TOKENS = 2**31 - 1
 
 
 def _check_ids(op: str, ids) -> int:
-    import torch
     need_tensor(op, "ids", ids)
     if ids.dtype not in (torch.int32, torch.int64):
         fail(f"{op}: ids have to be int32 or int64, got {ids.dtype}")
@@ -34,7 +35,6 @@ def embedding(table, ids, scale: float = 1.0):
     fp64) and rounded once.  Strided tables and ids are read in place as long as a row's values are neighbours and the
     ids' dimensions merge to two; otherwise they are copied first.
     """
-    import torch
     need_tensor("embedding", "table", table)
     code = need_type("embedding", "table", table)
     if table.dim() != 2:
@@ -52,10 +52,9 @@ def embedding(table, ids, scale: float = 1.0):
     (n0, n1), ((s0, s1),) = view
     out = torch.empty((*ids.shape, width), dtype=table.dtype, device=table.device)
     if out.numel():
-        args = _LOOKUP.pack(table.data_ptr(), ids.data_ptr(), out.data_ptr(), stream_of(device), device, rows, width, table.stride(0),
-                            n0, n1, s0, s1, code, wide_ids, float(scale))
-        if lib.lga_hip_embedding(args) != 0:
-            launch(lib.lga_hip_embedding, args)
+        run(lib.lga_hip_embedding,
+            lambda work: _LOOKUP.pack(table.data_ptr(), ids.data_ptr(), out.data_ptr(), stream_of(device), device, rows, width, table.stride(0),
+                                      n0, n1, s0, s1, code, wide_ids, float(scale)), table.device)
     return out
 
 
@@ -67,7 +66,6 @@ def embedding_grad(grad, ids, num_rows: int, scale: float = 1.0, dtype=None):
     or float32; the sums are held in 32 bits (64 for fp64).  The tokens are sorted, so every row is added up in the order
     of its tokens and the result does not depend on timing.
     """
-    import torch
     need_tensor("embedding_grad", "grad", grad)
     code = need_type("embedding_grad", "grad", grad)
     wide_ids = _check_ids("embedding_grad", ids)
@@ -92,12 +90,7 @@ def embedding_grad(grad, ids, num_rows: int, scale: float = 1.0, dtype=None):
     (n0, n1), ((s0, s1), (g0, g1)) = view
     out = torch.empty((num_rows, width), dtype=out_type, device=grad.device)
     if out.numel():
-        fn = lib.lga_hip_embedding_grad
-
-        def pack(work: int) -> bytes:
-            return _LOOKUP_GRAD.pack(grad.data_ptr(), ids.data_ptr(), out.data_ptr(), work, stream_of(device), device, num_rows, width,
-                                     n0, n1, s0, s1, g0, g1, code, out_code, wide_ids, float(scale))
-        need = workspace_bytes(fn, pack(0))
-        work = torch.empty(need, dtype=torch.uint8, device=grad.device) if need else None
-        launch(fn, pack(work.data_ptr() if need else 0))
+        run(lib.lga_hip_embedding_grad,
+            lambda work: _LOOKUP_GRAD.pack(grad.data_ptr(), ids.data_ptr(), out.data_ptr(), work, stream_of(device), device, num_rows, width,
+                                           n0, n1, s0, s1, g0, g1, code, out_code, wide_ids, float(scale)), grad.device)
     return out

@@ -11,14 +11,15 @@ from __future__ import annotations
 
 import struct
 
-from ._args import core, fail, launch, need_device, need_tensor, need_type, stream_of, workspace_bytes
+import torch
+
+from ._args import core, fail, need_device, need_tensor, need_type, run, stream_of
 
 _SCAN = struct.Struct("20q")
 _SCAN_GRAD = struct.Struct("29q")
 
 
 def _wide(t):
-    import torch
     return torch.float64 if t.dtype == torch.float64 else torch.float32
 
 
@@ -29,7 +30,6 @@ def _rows(t):
 
 def _check(op: str, x, code: int, gate, lengths, ends):
     """Checks what forward and backward share; returns (gate, gate type code, groups)."""
-    import torch
     b, t, d = x.shape
     gate_code = groups = 0
     if gate is not None:
@@ -80,7 +80,6 @@ def gated_scan(x, gate=None, state=None, *, mix: bool = False, lengths=None):
     is not used.  States are carried in float32 (float64 for fp64), which is also the type of ``state`` and ``last``: feeding
     ``last`` back in continues a sequence, step by step or in pieces.
     """
-    import torch
     need_tensor("gated_scan", "x", x)
     code = need_type("gated_scan", "x", x)
     if x.dim() != 3:
@@ -95,15 +94,11 @@ def gated_scan(x, gate=None, state=None, *, mix: bool = False, lengths=None):
     states = torch.empty((b, t, d), dtype=x.dtype, device=x.device)
     last = torch.empty((b, d), dtype=_wide(x), device=x.device)
     if last.numel():
-        fn = lib.lga_hip_gated_scan
         gate_b, gate_t = _gate_steps(gate, b)
-
-        def pack(work: int) -> bytes:
-            return _SCAN.pack(x.data_ptr(), _address(gate) if t else 0, _address(state), _address(lengths), states.data_ptr(), last.data_ptr(), work,
-                              stream_of(device), device, b, t, d, x.stride(0), x.stride(1), gate_b, gate_t, groups, code, gate_code, bool(mix))
-        need = workspace_bytes(fn, pack(0))
-        work = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-        launch(fn, pack(_address(work)))
+        run(lib.lga_hip_gated_scan,
+            lambda work: _SCAN.pack(x.data_ptr(), _address(gate) if t else 0, _address(state), _address(lengths), states.data_ptr(), last.data_ptr(),
+                                    work, stream_of(device), device, b, t, d, x.stride(0), x.stride(1), gate_b, gate_t, groups, code, gate_code,
+                                    bool(mix)), x.device)
     return states, last
 
 
@@ -116,7 +111,6 @@ def gated_scan_grad(grad_states, states, gate=None, state=None, *, x=None, grad_
     type and shape - summed over the channels and sequences that shared a gate - and is ``None`` without one.  Behind a
     sequence's length all of them are zero.
     """
-    import torch
     need_tensor("gated_scan_grad", "grad_states", grad_states)
     need_tensor("gated_scan_grad", "states", states)
     code = need_type("gated_scan_grad", "states", states)
@@ -139,18 +133,14 @@ def gated_scan_grad(grad_states, states, gate=None, state=None, *, x=None, grad_
     grad_state = torch.empty((b, d), dtype=_wide(states), device=states.device)
     grad_gate = None if gate is None else torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
     if grad_state.numel():
-        fn = lib.lga_hip_gated_scan_grad
         gate_b, gate_t = _gate_steps(gate, b)
         x_b, x_t = (x.stride(0), x.stride(1)) if mix else (0, 0)
-
-        def pack(work: int) -> bytes:
-            return _SCAN_GRAD.pack(grad_states.data_ptr(), states.data_ptr(), _address(gate) if t else 0, _address(state), _address(x),
-                                   _address(grad_last), _address(lengths), grad_x.data_ptr(), grad_state.data_ptr(), _address(grad_gate), work,
-                                   stream_of(device), device, b, t, d, grad_states.stride(0), grad_states.stride(1), states.stride(0),
-                                   states.stride(1), x_b, x_t, gate_b, gate_t, groups, 0 if gate is None else gate.shape[0], code, gate_code, bool(mix))
-        need = workspace_bytes(fn, pack(0))
-        work = torch.empty(need, dtype=torch.uint8, device=states.device) if need else None
-        launch(fn, pack(_address(work)))
+        gates = 0 if gate is None else gate.shape[0]
+        run(lib.lga_hip_gated_scan_grad,
+            lambda work: _SCAN_GRAD.pack(grad_states.data_ptr(), states.data_ptr(), _address(gate) if t else 0, _address(state), _address(x),
+                                         _address(grad_last), _address(lengths), grad_x.data_ptr(), grad_state.data_ptr(), _address(grad_gate), work,
+                                         stream_of(device), device, b, t, d, grad_states.stride(0), grad_states.stride(1), states.stride(0),
+                                         states.stride(1), x_b, x_t, gate_b, gate_t, groups, gates, code, gate_code, bool(mix)), states.device)
     elif grad_gate is not None:
         grad_gate.zero_()
     return grad_x, grad_state, grad_gate

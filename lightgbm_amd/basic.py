@@ -932,6 +932,18 @@ class Booster:
                                     c_str(params_to_string(kwargs))))
         return out
 
+    def refit_stages(self, data, label, weight=None, num_steps: int = 20, learning_rate: float = 1.0, lambda_l2: float = 0.0,
+                     stages: str = "all", device: Optional[str] = None) -> "Booster":
+        """A new booster with this model's tree structures and ALL leaf values refitted to ``data`` together, where
+        :meth:`refit` goes tree after tree: ``num_steps`` steps of descent on the weighted mean loss, averaged over the
+        predictions after 1, 2, ..., all iterations (``stages="all"``: models cut off at any ``num_iteration`` stay good)
+        or of the whole model alone (``stages="last"``).  A step is scaled leaf by leaf with a bound of the curvature, so
+        the loss never rises for learning rates up to 2; ``lambda_l2`` holds the values near the old ones.  Objectives
+        ``regression``, ``binary`` and ``multiclass``.  Runs in fp64, on the GPU (``device="gpu"``, or by size) with the
+        lookup and recurrence of ``lightgbm_amd.ops`` and their gradients."""
+        from .stages import refit_stages
+        return refit_stages(self, data, label, weight, num_steps, learning_rate, lambda_l2, stages, device)
+
     def reset_parameter(self, params: Dict[str, Any]) -> "Booster":
         lib, _ = _lib.load()
         check(lib.lga_booster_reset_parameter(self._handle, c_str(params_to_string(params))))
@@ -1077,6 +1089,16 @@ class Booster:
         if pred_contrib or K > 1:
             return out.reshape(nrow, width)
         return out
+
+    def staged_predict(self, data, start_iteration: int = 0, num_iteration: Optional[int] = None, raw_score: bool = False,
+                       device: Optional[str] = None) -> np.ndarray:
+        """Predictions after every iteration: ``out[k]`` is what ``predict(start_iteration=start_iteration,
+        num_iteration=k + 1)`` gives, up to the rounding of fp64 sums in another order; ``[iterations, rows]``, or
+        ``[iterations, rows, num_class]`` for multiclass models.  All trees are walked once and their leaf values run
+        through one scan, on the GPU (``device="gpu"``, or by size) or in NumPy.  Early stopping of predictions
+        (``pred_early_stop``) is left out of account."""
+        from .stages import staged_predict
+        return staged_predict(self, data, start_iteration, num_iteration, raw_score, device)
 
     def _predict_early_stop(self, mat, start_iteration, num_iteration, raw_score, device, kind, sigmoid, freq, margin):
         """Classification with ``pred_early_stop``: the raw score is built up ``freq`` iterations at a time, and a row

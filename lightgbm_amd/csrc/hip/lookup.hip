@@ -59,11 +59,11 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void lookup_tile_kernel(const T* __restrict__ table, const void* __restrict__ ids, T* __restrict__ out, int64_t rows,
                                                                int width, int64_t table_stride, TokenGrid grid, TokenTiles tiles, Wide<T> scale) {
   __shared__ int32_t id_of[kSortTile];
-  const int shift1 = tiles.shift1, side1 = 1 << shift1, shift0 = 12 - shift1;
+  const int shift1 = tiles.shift1, side1 = 1 << shift1, shift0 = tiles.bits - shift1, size = 1 << tiles.bits;
   const int64_t ti = blockIdx.x / tiles.across, i0 = ti << shift0, j0 = (blockIdx.x - ti * tiles.across) << shift1;
   const bool along0 = grid.s0 < grid.s1;
 #pragma unroll 8
-  for (int n = threadIdx.x; n < kSortTile; n += kThreads) {
+  for (int n = threadIdx.x; n < size; n += kThreads) {
     const int i = along0 ? n & ((1 << shift0) - 1) : n >> shift1, j = along0 ? n >> shift0 : n & (side1 - 1);
     int32_t id = -1;
     if (i0 + i < grid.n0 && j0 + j < grid.n1) {
@@ -76,7 +76,7 @@ __global__ __launch_bounds__(kThreads) void lookup_tile_kernel(const T* __restri
   const int live1 = (int)min((int64_t)side1, grid.n1 - j0), live0 = (int)min((int64_t)1 << shift0, grid.n0 - i0);
   if (width == 1) {
 #pragma unroll 8
-    for (int n = threadIdx.x; n < kSortTile; n += kThreads) {
+    for (int n = threadIdx.x; n < size; n += kThreads) {
       const int i = n >> shift1, j = n & (side1 - 1);
       if (i >= live0 || j >= live1) continue;
       const int32_t id = id_of[tile_slot(n)];
@@ -84,10 +84,11 @@ __global__ __launch_bounds__(kThreads) void lookup_tile_kernel(const T* __restri
     }
     return;
   }
-  const int line = live1 * width, total = live0 * line;
+  // divisions by multiplication: exact, as no n times its divisor reaches 2^32
+  const uint32_t line = live1 * width, total = live0 * line, by_line = (uint32_t)((1ull << 32) / line + 1), by_width = (uint32_t)((1ull << 32) / width + 1);
 #pragma unroll 4
-  for (int n = threadIdx.x; n < total; n += kThreads) {
-    const int i = n / line, e = n - i * line, j = e / width;
+  for (uint32_t n = threadIdx.x; n < total; n += kThreads) {
+    const uint32_t i = line > 1 ? __umulhi(n, by_line) : n, e = n - i * line, j = __umulhi(e, by_width);
     const int32_t id = id_of[tile_slot(i << shift1 | j)];
     out[((i0 + i) * grid.n1 + j0) * width + e] = id >= 0 ? (T)((Wide<T>)table[id * table_stride + e - j * width] * scale) : (T)(Wide<T>)0;
   }
@@ -95,6 +96,7 @@ __global__ __launch_bounds__(kThreads) void lookup_tile_kernel(const T* __restri
 
 constexpr int kOwnRows = 8;       // table rows a workgroup owns
 constexpr int kListSize = 1024;   // tokens it collects before it adds them up
+constexpr int kAhead = 16;        // gradients loaded before they are added
 
 // A workgroup owns kOwnRows rows of the table and 256 columns: it reads all ids, collects the tokens of its rows in their
 // order (ballot compaction) and adds their gradients up in that order, so sums do not depend on timing.
@@ -136,9 +138,16 @@ __global__ __launch_bounds__(kThreads) void lookup_grad_owned_kernel(const T* __
     __syncthreads();
     if (filled >= kListSize || base + kThreads >= tokens) {
       if (col < width)
-        for (int k = 0; k < filled; ++k) {
-          const int64_t tk = list_token[k], i = tk / n1, j = tk - i * n1;
-          acc[list_row[k]][t] += (Wide<T>)grad[i * g0 + j * g1 + col];
+        for (int k = 0; k < filled; k += kAhead) {
+          T g[kAhead];
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {
+            const uint32_t tk = list_token[min(k + u, filled - 1)], i = tk / (uint32_t)n1, j = tk - i * (uint32_t)n1;
+            g[u] = grad[i * g0 + j * g1 + col];
+          }
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u)
+            if (k + u < filled) acc[list_row[k + u]][t] += (Wide<T>)g[u];
         }
       filled = 0;
       __syncthreads();
@@ -149,7 +158,7 @@ __global__ __launch_bounds__(kThreads) void lookup_grad_owned_kernel(const T* __
       if (first + r < rows) out[(first + r) * width + col] = (O)(acc[r][t] * scale);
 }
 
-// Few rows, many tokens: every wave keeps sums of the whole table in LDS and adds its tokens to them, kGroup x 64 at a
+// Few rows, many tokens: every wave keeps sums of one column of the table in LDS and adds its tokens to them, kGroup x 64 at a
 // time; the waves' sums are added up in order afterwards.  LDS accesses of one wave run in their order, so the additions
 // have a fixed order as long as no two lanes touch one row at a time:  tag[row] = lane, read back, tells whether lanes share
 // a row (whichever of two lanes is read back, the other one sees it); if so, they find each other with ballots and
@@ -164,12 +173,13 @@ constexpr int kGroup = 4;             // of which so many are added at a time
 template <typename T, typename I, bool kAlong0, bool kWhole>
 __global__ __launch_bounds__(64) void lookup_grad_private_kernel(const T* __restrict__ grad, TokenGrid grid, int64_t g0, int64_t g1, int width, int row_bits,
                                                                  int lines, int steps, int each, Wide<T>* __restrict__ parts) {
+  grad += blockIdx.y;                 // the wave's column
   typedef Wide<T> W;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   W* sums = (W*)lds;                  // one row more than the table has: tokens that take no part
-  const int rows = (int)grid.rows, values = rows * width, lane = threadIdx.x;
-  uint8_t* tag = (uint8_t*)(sums + values + width);
-  for (int k = lane; k < values + width; k += 64) sums[k] = 0;
+  const int rows = (int)grid.rows, lane = threadIdx.x;
+  uint8_t* tag = (uint8_t*)(sums + rows + 1);
+  for (int k = lane; k <= rows; k += 64) sums[k] = 0;
   __syncthreads();
   constexpr int item_i = kAlong0 ? 64 : 0, item_j = kAlong0 ? 0 : 1;
   auto place = [&](int step, int64_t& i0, int64_t& j0) {
@@ -230,7 +240,6 @@ __global__ __launch_bounds__(64) void lookup_grad_private_kernel(const T* __rest
       g[u] = next_g[u];
     }
     if (step + 1 < end) load(step + 1, next_id, next_g);
-    const T* from = grad + i0 * g0 + j0 * g1;
     uint32_t meets = 0;               // groups of items in which lanes share a row: later, read once more
 #pragma unroll
     for (int u0 = 0; u0 < kPrivateItems; u0 += kGroup) {
@@ -242,7 +251,7 @@ __global__ __launch_bounds__(64) void lookup_grad_private_kernel(const T* __rest
 #pragma unroll
       for (int k = 0; k < kGroup; ++k) seen[k] = tag[row[u0 + k]];
 #pragma unroll
-      for (int k = 0; k < kGroup; ++k) sum[k] = sums[row[u0 + k] * width];
+      for (int k = 0; k < kGroup; ++k) sum[k] = sums[row[u0 + k]];
       bool other = false;
 #pragma unroll
       for (int k = 0; k < kGroup; ++k) other |= row[u0 + k] < rows && seen[k] != (uint8_t)lane;
@@ -258,15 +267,9 @@ __global__ __launch_bounds__(64) void lookup_grad_private_kernel(const T* __rest
         }
 #pragma unroll
         for (int k = 0; k < kGroup; ++k) {
-          sums[row[u0 + k] * width] = sum[k];
+          sums[row[u0 + k]] = sum[k];
           in_order();
         }
-        for (int c = 1; c < width; ++c)
-#pragma unroll
-          for (int k = 0; k < kGroup; ++k) {
-            if (row[u0 + k] < rows) sums[row[u0 + k] * width + c] += (W)from[(u0 + k) * item_i * g0 + (u0 + k) * item_j * g1 + c];
-            in_order();
-          }
       }
       in_order();
     }
@@ -286,10 +289,7 @@ __global__ __launch_bounds__(64) void lookup_grad_private_kernel(const T* __rest
         }
         const int turn = at < rows ? __popcll(same & ((1ull << lane) - 1)) : -1;
         for (int k = 0; __any(turn >= k); ++k) {
-          if (turn == k) {
-            sums[at * width] += value;
-            for (int c = 1; c < width; ++c) sums[at * width + c] += (W)from[u * item_i * g0 + u * item_j * g1 + c];
-          }
+          if (turn == k) sums[at] += value;
           in_order();
         }
       }
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(64) void lookup_grad_private_kernel(const T* __rest
     in_order();
   }
   __syncthreads();
-  for (int k = lane; k < values; k += 64) parts[(int64_t)blockIdx.x * values + k] = sums[k];
+  for (int k = lane; k < rows; k += 64) parts[((int64_t)blockIdx.x * rows + k) * width + blockIdx.y] = sums[k];
 }
 
 // out = scale * the waves' sums, 64 values side by side, the waves in kThreads / 64 parts.
@@ -380,7 +380,7 @@ __global__ __launch_bounds__(kRunThreads) void lookup_grad_runs_kernel(Runs r, c
     if (blockIdx.y == 0) zero_rows(r, out, (int64_t)blockIdx.x * (kRunThreads / 64) + (threadIdx.x >> 6), threadIdx.x & 63);
     return;
   }
-  constexpr int kAhead = 8;
+  constexpr int kAhead = 8;     // (of its own)
   __shared__ W shead[kRunThreads * V], stail[kRunThreads * V];
   __shared__ int flags[kRunThreads / 8];
   const int strips = kRunThreads / group, strip = threadIdx.x / group, lane = threadIdx.x % group;
@@ -602,7 +602,8 @@ template <typename T> void run_lookup(const LookupArgs& a) {
     grid.ids64 = (int)a.ids64;
     grid.n0 = a.n0, grid.n1 = a.n1, grid.s0 = a.s0, grid.s1 = a.s1;
     grid.rows = a.rows;
-    const TokenTiles tiles = token_tiles(grid);
+    TokenTiles tiles = token_tiles(grid, 10);      // small tiles until there are enough for every CU
+    if (tiles.blocks > 4096) tiles = token_tiles(grid);
     hipLaunchKernelGGL(lookup_tile_kernel<T>, dim3((unsigned)tiles.blocks), dim3(kThreads), 0, (hipStream_t)a.stream, (const T*)a.table, (const void*)a.ids,
                        (T*)a.out, a.rows, (int)a.width, a.table_stride, grid, tiles, (Wide<T>)a.scale);
   } else {
@@ -620,7 +621,7 @@ template <typename T> void run_lookup(const LookupArgs& a) {
 
 // Up to this many tokens every workgroup looks through all ids for its own rows; above, they are sorted.
 constexpr int64_t kOwnedTokens = 2048;
-constexpr int64_t kPrivateLds = 65536;      // of a wave, for sums of the whole table
+constexpr int64_t kPrivateLds = 65536;      // of a wave, for the sums of a column
 
 struct GradPlan {
   TokenGrid grid;
@@ -669,7 +670,7 @@ GradPlan plan_grad(const LookupGradArgs& a) {
 
 bool owned(const LookupGradArgs& a) { return a.n0 * a.n1 <= kOwnedTokens; }
 
-// Few rows and many tokens: sums of the whole table in a wave's share of LDS.
+// Few rows and many tokens: sums of a column of the table in a wave's share of LDS.
 struct PrivatePlan {
   TokenGrid grid;
   int64_t g0, g1, lines, steps;
@@ -679,7 +680,7 @@ struct PrivatePlan {
 
 PrivatePlan plan_private(const LookupGradArgs& a) {
   PrivatePlan p;
-  const int64_t wide = a.type == kF64 ? 8 : 4, tokens = a.n0 * a.n1, lds = (a.rows + 1) * (a.width * wide + 1);
+  const int64_t wide = a.type == kF64 ? 8 : 4, tokens = a.n0 * a.n1, lds = (a.rows + 1) * (wide + 1);
   if (a.width > kNarrow || lds > kPrivateLds || tokens < 16 * a.rows) return p;
   p.grid.ids = (const void*)a.ids;
   p.grid.ids64 = (int)a.ids64;
@@ -699,7 +700,7 @@ PrivatePlan plan_private(const LookupGradArgs& a) {
   p.whole = !p.items_along0 && a.width == 1 && p.g1 == 1 && p.g0 % pack == 0 && a.grad % 16 == 0;
   p.lds = (int)((lds + 15) / 16 * 16);
   const int64_t fit = 256 * std::min<int64_t>(8, std::max<int64_t>(1, 163840 / p.lds));
-  p.waves = (int)std::max<int64_t>(1, std::min({fit, p.steps, tokens / std::max<int64_t>(1024, 2 * a.rows)}));
+  p.waves = (int)std::max<int64_t>(1, std::min({fit / a.width, p.steps, tokens / std::max<int64_t>(1024, 2 * a.rows)}));
   return p;
 }
 
@@ -727,7 +728,7 @@ template <typename T, typename O> void run_lookup_grad(const LookupGradArgs& a) 
     int bits = 1;
     while (a.rows >> bits) ++bits;
     auto run = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(few.waves), dim3(64), few.lds, s, (const T*)a.grad, few.grid, few.g0, few.g1, (int)a.width, bits,
+      hipLaunchKernelGGL(kernel, dim3(few.waves, (unsigned)a.width), dim3(64), few.lds, s, (const T*)a.grad, few.grid, few.g0, few.g1, (int)a.width, bits,
                          (int)few.lines, (int)few.steps, (int)((few.steps + few.waves - 1) / few.waves), parts);
     };
     auto by_ids = [&](auto id) {

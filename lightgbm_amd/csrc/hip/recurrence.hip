@@ -27,6 +27,13 @@ constexpr uint64_t kEmpty = ~0ull;  // a word nobody has written yet: a NaN that
 
 enum GateKind { kNoGate, kOwnGate, kSharedGate };
 
+// How the slopes of shared gates are summed: by teams of lanes (0: not), whose sums stand as [rows][steps][teams]; `done`: a
+// team is a whole gate group, and its sum is the gate's gradient.
+struct GateSums {
+  int team = 0, done = 0;
+  int64_t rows = 1, teams = 1;
+};
+
 __device__ __forceinline__ float smallest(float) { return 1.40129846e-45f; }
 __device__ __forceinline__ double smallest(double) { return 4.9406564584124654e-324; }
 __device__ __forceinline__ float abs_of(float x) { return __builtin_fabsf(x); }
@@ -275,9 +282,36 @@ __global__ __launch_bounds__(kLanes* kMaxSlots) void scan_kernel(ScanArgs a, Cut
     for (int v = 0; v < V; ++v) ((W*)a.last)[c + v] = h[v];
 }
 
+// Sums v[j] over the `team` lanes (a power of two) that this lane belongs to, for all N of them (a power of two): lanes
+// exchange halves of what they still hold, so that N sums over 64 lanes take N - 1 + log2(64 / N) exchanges.  Afterwards the
+// lane holds in v[0] the sum of item `mine`; `holds`: it is the one of its team that holds it.
+template <typename W, int N> __device__ __forceinline__ void team_sums(W (&v)[N], int team, int& mine, bool& holds) {
+  const int lane = threadIdx.x & (team - 1);
+  int bit = 1;
+  mine = 0;
+#pragma unroll
+  for (int n = N; n > 1; n /= 2) {
+    if (bit < team) {
+      const bool upper = (lane & bit) != 0;
+#pragma unroll
+      for (int j = 0; j < N / 2; ++j)
+        if (j < n / 2) {
+          const W give = upper ? v[j] : v[j + n / 2], keep = upper ? v[j + n / 2] : v[j];
+          v[j] = keep + __shfl_xor(give, bit);
+        }
+      mine += upper ? n / 2 : 0;
+      bit *= 2;
+    }
+  }
+  holds = lane < bit;
+  for (; bit < team; bit *= 2) v[0] += __shfl_xor(v[0], bit);
+}
+
 // Backwards: step r of a chunk is step steps - 1 - r of the sequence.
+// Where neighbouring channels share a gate, teams of `team` lanes (at least as many as steps) add their slopes up: `slopes`
+// then has one value per team and step, [slope_rows][steps][teams a row].
 template <typename T, typename G, GateKind K, int V, int L>
-__global__ __launch_bounds__(kLanes* kMaxSlots) void scan_grad_kernel(ScanGradArgs a, Cut k, uint64_t* work, int64_t slopes) {
+__global__ __launch_bounds__(kLanes* kMaxSlots) void scan_grad_kernel(ScanGradArgs a, Cut k, uint64_t* work, int64_t slopes, GateSums sums) {
   typedef Wide<T> W;
   int64_t tile, row;
   take_tile(k, work, tile, row);
@@ -340,10 +374,11 @@ __global__ __launch_bounds__(kLanes* kMaxSlots) void scan_grad_kernel(ScanGradAr
   } else {
     for (int v = 0; v < V; ++v) e[v] = first[v];
   }
-  if (!live) return;
+  if (!live && !sums.team) return;
   T* dx = (T*)a.grad_x + b * a.steps * a.width + d;
   G* da = (G*)a.grad_gate + b * a.steps * a.width + d;
   W* slope = (W*)slopes + b * a.steps * a.width + d;
+  W total[L];
 #pragma unroll
   for (int j = 0; j < L; ++j) {
     const int64_t t = t0 - j;
@@ -368,13 +403,33 @@ __global__ __launch_bounds__(kLanes* kMaxSlots) void scan_grad_kernel(ScanGradAr
       }
       o.v[v] = t < len ? (T)value : (T)(W)0;
     }
-    if (t >= 0) {
+    if (t >= 0 && live) {
       store_pack<T, V>(dx + t * a.width, o);
       if constexpr (K != kNoGate) {
-        if (slopes) store_pack<W, V>(slope + t * a.width, os);
-        else store_pack<G, V>(da + t * a.width, og);
+        if (!sums.team) {
+          if (slopes) store_pack<W, V>(slope + t * a.width, os);
+          else store_pack<G, V>(da + t * a.width, og);
+        }
       }
     }
+    if constexpr (K != kNoGate) {
+      total[j] = 0;
+      for (int v = 0; v < V; ++v) total[j] += live ? os.v[v] : (W)0;
+    }
+  }
+  if constexpr (K != kNoGate) {
+    if (sums.team) {
+      int mine;
+      bool holds;
+      team_sums<W, L>(total, sums.team, mine, holds);
+      const int64_t t = t0 - mine, at = pack / sums.team, r = at / sums.teams;
+      if (holds && t >= 0 && r < sums.rows) {
+        const int64_t to = (r * a.steps + t) * sums.teams + at - r * sums.teams;
+        if (sums.done) ((G*)a.grad_gate)[to] = (G)total[0];
+        else ((W*)slopes)[to] = total[0];
+      }
+    }
+    if (!live) return;
   }
   if (tile == k.tiles - 1 && slot == k.slots - 1)
     for (int v = 0; v < V; ++v) ((W*)a.grad_state)[c + v] = e[v];
@@ -444,7 +499,8 @@ Cut cut_steps(int64_t batch, int64_t steps, int64_t width, int v, int per_lane, 
 
 // Two workgroups of 8 chunks a CU overlap loads with sums better than one of 16 (8 x 4096 x 2560 bf16: 156 against 161 us),
 // but a long sequence has fewer maps to fold in larger tiles (1 x 65537 x 1024 bf16: 116 against 128 us).
-int scan_slots(const ScanArgs& a) { return a.steps > 64 * 8 * kScanSteps ? kMaxSlots : 8; }
+// Up to kMaxSlots chunks are one tile, which needs neither a workspace nor tickets.
+int scan_slots(const ScanArgs& a) { return a.steps > 64 * 8 * kScanSteps || a.steps <= kMaxSlots * kScanSteps ? kMaxSlots : 8; }
 
 template <typename A> void check_args(const A& a) {
   if (a.batch < 0 || a.steps < 0 || a.width < 0) throw std::runtime_error("gated_scan: a negative size");
@@ -490,6 +546,35 @@ template <typename W> void clear_work(const Cut& k, int v, uint64_t* work, hipSt
 
 bool sums_gates(const ScanGradArgs& a) { return a.gate && (a.groups != a.width || a.gate_batch != a.batch); }
 
+// Teams of at least 8 lanes within a gate group (or, with one gate a step for everything, over all lanes) sum up in the
+// backward kernel; a group like 103 channels has none, and its slopes go through memory value by value.
+GateSums gate_sums(const ScanGradArgs& a, const Cut& k, int v) {
+  GateSums g;
+  if (!sums_gates(a)) return g;
+  const int64_t per = a.width / a.groups;
+  const int most = std::min(k.lanes, 64);
+  int team = 0;
+  if (a.groups == 1 && a.gate_batch == 1) {
+    team = most;
+    g.teams = (k.packs + team - 1) / team;
+  } else if (per % v == 0) {
+    team = 1;
+    while (team < most && per / v % (team * 2) == 0) team *= 2;
+    g.rows = a.batch;
+    g.teams = a.width / v / team;
+    g.done = per / v == team && a.gate_batch == a.batch;
+  }
+  g.team = team >= 8 ? team : 0;
+  if (!g.team) return GateSums{};
+  if (a.groups == 1 && a.gate_batch == 1 && g.teams == 1) g.done = 1;
+  return g;
+}
+
+int64_t slope_values(const ScanGradArgs& a, const GateSums& g) {
+  if (!sums_gates(a) || g.done) return 0;
+  return g.team ? g.rows * a.steps * g.teams : a.batch * a.steps * a.width;
+}
+
 }  // namespace
 
 int64_t scan_workspace(const ScanArgs& a) {
@@ -521,8 +606,7 @@ int64_t scan_grad_workspace(const ScanGradArgs& a) {
   check_args(a);
   const int v = two_wide(a) ? 2 : 1;
   const Cut k = cut_steps(a.batch, a.steps, a.width, v, a.steps <= 1 ? 1 : kGradSteps, kMaxSlots);
-  const int64_t slopes = sums_gates(a) ? a.batch * a.steps * a.width * (a.type == kF64 ? 8 : 4) : 0;
-  return 8 * (a.type == kF64 ? work_words<double>(k, v) : work_words<float>(k, v)) + slopes;
+  return 8 * (a.type == kF64 ? work_words<double>(k, v) : work_words<float>(k, v)) + slope_values(a, gate_sums(a, k, v)) * (a.type == kF64 ? 8 : 4);
 }
 
 void gated_scan_grad(const ScanGradArgs& a) {
@@ -539,15 +623,18 @@ void gated_scan_grad(const ScanGradArgs& a) {
       const Cut k = cut_steps(a.batch, a.steps, a.width, V, L, kMaxSlots);
       uint64_t* work = (uint64_t*)a.work;
       clear_work<W>(k, V, work, s);
-      const int64_t slopes = sums_gates(a) ? (int64_t)(work + work_words<W>(k, V)) : 0;
+      const GateSums g = gate_sums(a, k, V);
+      const int64_t slopes = slope_values(a, g) ? (int64_t)(work + work_words<W>(k, V)) : 0;
       hipLaunchKernelGGL((scan_grad_kernel<T, G, (GateKind)decltype(kind)::value, V, L>), dim3((unsigned)(k.tiles * k.pack_rows)), dim3(k.lanes * k.slots),
-                         fold_bytes<W>(k, V), s, a, k, work, slopes);
+                         fold_bytes<W>(k, V), s, a, k, work, slopes, g);
       LGA_HIP_CHECK(hipGetLastError());
       if (slopes) {
-        const int64_t sums = a.gate_batch * a.steps * a.groups, terms = a.width / a.groups * (a.batch / a.gate_batch);
+        // the slopes, or the teams' sums of them: [rows][steps][across]
+        const int64_t rows = g.team ? g.rows : a.batch, across = g.team ? g.teams : a.width;
+        const int64_t sums = a.gate_batch * a.steps * a.groups, terms = across / a.groups * (rows / std::min(rows, a.gate_batch));
         auto run = [&](auto kernel, int64_t team) {
           hipLaunchKernelGGL(kernel, dim3((unsigned)std::min<int64_t>((sums * team + kThreads - 1) / kThreads, 1 << 20)), dim3(kThreads), 0, s,
-                             (const W*)slopes, (G*)a.grad_gate, a.batch, a.steps, a.width, a.groups, a.gate_batch);
+                             (const W*)slopes, (G*)a.grad_gate, rows, a.steps, across, a.groups, a.gate_batch);
         };
         if (terms <= kWaveTerms) run(gate_sum_kernel<W, G, 64>, 64);
         else run(gate_sum_kernel<W, G, kThreads>, kThreads);

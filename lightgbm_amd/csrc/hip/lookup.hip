@@ -620,8 +620,8 @@ template <typename T> void run_lookup(const LookupArgs& a) {
 }
 
 // Up to this many tokens every workgroup looks through all ids for its own rows; above, they are sorted.
-constexpr int64_t kOwnedTokens = 2048;
-constexpr int64_t kPrivateLds = 65536;      // of a wave, for the sums of a column
+constexpr int64_t kOwnedTokens = 512;
+constexpr int64_t kPrivateLds = 81920;      // of a wave, for the sums of a column
 
 struct GradPlan {
   TokenGrid grid;
@@ -700,7 +700,7 @@ PrivatePlan plan_private(const LookupGradArgs& a) {
   p.whole = !p.items_along0 && a.width == 1 && p.g1 == 1 && p.g0 % pack == 0 && a.grad % 16 == 0;
   p.lds = (int)((lds + 15) / 16 * 16);
   const int64_t fit = 256 * std::min<int64_t>(8, std::max<int64_t>(1, 163840 / p.lds));
-  p.waves = (int)std::max<int64_t>(1, std::min({fit / a.width, p.steps, tokens / std::max<int64_t>(1024, 2 * a.rows)}));
+  p.waves = (int)std::max<int64_t>(1, std::min({fit / a.width, p.steps, tokens / std::max<int64_t>(1024, a.rows)}));
   return p;
 }
 
@@ -728,6 +728,7 @@ template <typename T, typename O> void run_lookup_grad(const LookupGradArgs& a) 
     int bits = 1;
     while (a.rows >> bits) ++bits;
     auto run = [&](auto kernel) {
+      if (few.lds > 65536) LGA_HIP_CHECK(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, few.lds));
       hipLaunchKernelGGL(kernel, dim3(few.waves, (unsigned)a.width), dim3(64), few.lds, s, (const T*)a.grad, few.grid, few.g0, few.g1, (int)a.width, bits,
                          (int)few.lines, (int)few.steps, (int)((few.steps + few.waves - 1) / few.waves), parts);
     };

@@ -215,6 +215,97 @@ __global__ __launch_bounds__(kThreads) void sort_scatter_kernel(Pass p, const ui
 
 static_assert(kBins == kThreads, "one lane a digit");
 
+// Up to kSortTile tokens: one workgroup takes all passes in LDS, in place of two launches a pass.
+constexpr int kOneThreads = 1024, kOneWaves = kOneThreads / 64, kOneItems = kSortTile / kOneThreads;
+
+template <typename P>
+__global__ __launch_bounds__(kOneThreads) void sort_one_kernel(Pass p, int passes, int total_bits, uint32_t* __restrict__ keys_out, P* __restrict__ payload_out) {
+  __shared__ uint32_t skey[kSortTile];
+  __shared__ P spay[kSortTile];
+  __shared__ uint16_t count[kOneWaves][kBins];
+  __shared__ uint32_t local[kBins], wave_sum[kBins / 64];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const uint32_t tokens = (uint32_t)(p.grid.n0 * p.grid.n1);
+  uint32_t key[kOneItems], rank[kOneItems];
+  P pay[kOneItems];
+#pragma unroll
+  for (int k = 0; k < kOneItems; ++k) {
+    const uint32_t q = wave * (kSortTile / kOneWaves) + k * 64 + lane;
+    key[k] = (uint32_t)p.grid.rows;
+    pay[k] = 0;
+    if (q < tokens) {
+      const uint32_t i = q / (uint32_t)p.grid.n1, j = q - i * (uint32_t)p.grid.n1;
+      key[k] = grid_key(p.grid, i, j);
+      pay[k] = p.payload_in ? ((const P*)p.payload_in)[i * p.v0 + j * p.v1] : (P)q;
+    }
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * p.bits, bits = min(p.bits, total_bits - shift);
+    const uint32_t mask = (1u << bits) - 1;
+    for (int d = t; d < kOneWaves * kBins; d += kOneThreads) (&count[0][0])[d] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kOneItems; ++k) {
+      const uint32_t digit = (key[k] >> shift) & mask;
+      uint64_t same = ~0ull;
+      for (int bit = 0; bit < bits; ++bit) {
+        const bool one = (digit >> bit) & 1;
+        const uint64_t ones = __ballot(one);
+        same &= one ? ones : ~ones;
+      }
+      in_order();
+      const uint32_t before = count[wave][digit];
+      in_order();
+      const int lower = __popcll(same & ((1ull << lane) - 1));
+      rank[k] = before + (uint32_t)lower;
+      if (lower == 0) count[wave][digit] = (uint16_t)(before + (uint32_t)__popcll(same));
+    }
+    __syncthreads();
+    uint32_t in_tile = 0, a = 0;
+    if (t < kBins) {
+      for (int w = 0; w < kOneWaves; ++w) {
+        const uint32_t c = count[w][t];
+        count[w][t] = (uint16_t)in_tile;
+        in_tile += c;
+      }
+      a = in_tile;
+      for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t o = __shfl_up(a, d);
+        if (lane >= d) a += o;
+      }
+      if (lane == 63) wave_sum[wave] = a;
+    }
+    __syncthreads();
+    if (t < kBins) {
+      for (int w = 0; w < wave; ++w) a += wave_sum[w];
+      local[t] = a - in_tile;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kOneItems; ++k) {
+      const uint32_t digit = (key[k] >> shift) & mask, at = local[digit] + count[wave][digit] + rank[k];
+      skey[at] = key[k];
+      spay[at] = pay[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kOneItems; ++k) {
+      const int q = wave * (kSortTile / kOneWaves) + k * 64 + lane;
+      key[k] = skey[q];
+      pay[k] = spay[q];
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int k = 0; k < kOneItems; ++k) {
+    const int q = wave * (kSortTile / kOneWaves) + k * 64 + lane;
+    keys_out[q] = key[k];
+    payload_out[q] = pay[k];
+  }
+}
+
+bool one_tile(const TokenGrid& g) { return g.n0 * g.n1 <= kSortTile; }
+
 int bit_length(int64_t v) {
   int n = 0;
   while (v > 0) ++n, v >>= 1;
@@ -256,6 +347,13 @@ TokenTiles token_tiles(const TokenGrid& g, int bits) {
 
 // Small tiles where tiles of 4096 would leave most of the chip idle.
 TokenTiles sort_tiles(const TokenGrid& g) {
+  if (one_tile(g)) {
+    TokenTiles t;
+    t.shift1 = t.bits;
+    t.across = t.blocks = 1;
+    t.count = kSortTile;
+    return t;
+  }
   const TokenTiles small = token_tiles(g, 10);
   if (small.blocks > kFewTiles) return token_tiles(g);
   TokenTiles t = small;
@@ -275,6 +373,15 @@ SortedTokens token_sort(const TokenGrid& g, const void* values, int64_t v0, int6
   const dim3 grid((unsigned)tiles.blocks), block(kThreads);
   uint32_t *counts = (uint32_t*)(w + l.counts), *totals = (uint32_t*)(w + l.totals);
   Pass p{g, tiles, nullptr, values, v0, v1, 0, each, small};
+  if (one_tile(g)) {
+    uint32_t* keys = (uint32_t*)(w + l.keys[0]);
+    void* pay = w + l.payload[0];
+    p.bits = each;
+    if (payload == 8) hipLaunchKernelGGL(sort_one_kernel<uint64_t>, dim3(1), dim3(kOneThreads), 0, s, p, passes, bits, keys, (uint64_t*)pay);
+    else hipLaunchKernelGGL(sort_one_kernel<uint32_t>, dim3(1), dim3(kOneThreads), 0, s, p, passes, bits, keys, (uint32_t*)pay);
+    LGA_HIP_CHECK(hipGetLastError());
+    return {keys, pay, tiles.count};
+  }
   for (int k = 0; k < passes; ++k) {
     p.shift = k * each;
     p.bits = std::min(each, bits - p.shift);

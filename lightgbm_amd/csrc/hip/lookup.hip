@@ -31,25 +31,25 @@ __global__ __launch_bounds__(kThreads) void lookup_rows_kernel(const T* __restri
   const bool named = id >= 0 && id < rows;
   const T* from = table + (named ? id * table_stride : 0);
   T* to = out + token * width;
-  const int step = group * V;
-  int64_t c = (int64_t)(threadIdx.x % group) * V;
+  const int packs = (int)((width + V - 1) / V), end = (int)(width - V);
+  int c = threadIdx.x % group;
   constexpr int kAhead = 4;
-  for (; c + (kAhead - 1) * step < width; c += kAhead * step) {
+  for (; c + (kAhead - 1) * group < packs; c += kAhead * group) {
     Pack<T, V> x[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
-      if (named) x[u] = load_pack<T, V>(from + c + u * step);
+      if (named) x[u] = load_pack<T, V>(from + min((c + u * group) * V, end));
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       for (int v = 0; v < V; ++v) x[u].v[v] = named ? (T)((W)x[u].v[v] * scale) : (T)(W)0;
-      store_pack<T, V>(to + c + u * step, x[u]);
+      store_pack<T, V>(to + min((c + u * group) * V, end), x[u]);
     }
   }
-  for (; c < width; c += step) {
+  for (; c < packs; c += group) {
     Pack<T, V> x;
-    if (named) x = load_pack<T, V>(from + c);
+    if (named) x = load_pack<T, V>(from + min(c * V, end));
     for (int v = 0; v < V; ++v) x.v[v] = named ? (T)((W)x.v[v] * scale) : (T)(W)0;
-    store_pack<T, V>(to + c, x);
+    store_pack<T, V>(to + min(c * V, end), x);
   }
 }
 
@@ -169,7 +169,7 @@ constexpr int kGroup = 4;             // of which so many are added at a time
 
 // A step: 64 x kPrivateItems tokens; lanes along axis 0, items along axis 1 or (few tokens there) along axis 0 too.  A step
 // is loaded while the one before is added up.  kWhole: gradients of one
-// value that are neighbours along axis 1 and start at multiples of 16 bytes.
+// value that are neighbours along axis 1.
 template <typename T, typename I, bool kAlong0, bool kWhole>
 __global__ __launch_bounds__(64) void lookup_grad_private_kernel(const T* __restrict__ grad, TokenGrid grid, int64_t g0, int64_t g1, int width, int row_bits,
                                                                  int lines, int steps, int each, Wide<T>* __restrict__ parts) {
@@ -203,12 +203,12 @@ __global__ __launch_bounds__(64) void lookup_grad_private_kernel(const T* __rest
       for (int u = 0; u < kPrivateItems; ++u) id[u] = at[u * next];
       const T* from = grad + i0 * g0 + j0 * g1;
       if constexpr (kWhole) {
-        constexpr int kPack = 16 / sizeof(T);
+        constexpr int V = 16 / sizeof(T);
 #pragma unroll
-        for (int u = 0; u < kPrivateItems; u += kPack) {
-          const Pack<T, kPack> x = load_pack<T, kPack>(from + u);
+        for (int u = 0; u < kPrivateItems; u += V) {
+          const Pack<T, V> x = load_pack<T, V>(from + u);
 #pragma unroll
-          for (int v = 0; v < kPack; ++v) g[u + v] = x.v[v];
+          for (int v = 0; v < V; ++v) g[u + v] = x.v[v];
         }
       } else {
         const int64_t on = kAlong0 ? 64 * g0 : g1;
@@ -351,18 +351,13 @@ template <typename O> __device__ __forceinline__ void zero_rows(const Runs& r, O
   const bool absent = lane < kZeroRows && first + lane < r.rows && !has_tokens(r, (uint32_t)(first + lane));
   uint64_t todo = __ballot(absent);
   constexpr int kWords = 16 / sizeof(O);
-  const bool whole = r.width % kWords == 0;
   while (todo) {
     O* row = out + (first + __ffsll((unsigned long long)todo) - 1) * r.width;
     todo &= todo - 1;
-    if (whole) {
-      for (int64_t c = (int64_t)lane * kWords; c < r.width; c += 64 * kWords) {
-        Pack<O, kWords> z;
-        for (int v = 0; v < kWords; ++v) z.v[v] = (O)0.f;
-        store_pack<O, kWords>(row + c, z);
-      }
-    } else {
-      for (int64_t c = lane; c < r.width; c += 64) row[c] = (O)0.f;
+    for (int64_t c = (int64_t)lane * kWords; c < r.width; c += 64 * kWords) {
+      Pack<O, kWords> z;
+      for (int v = 0; v < kWords; ++v) z.v[v] = (O)0.f;
+      store_pack<O, kWords>(row + min(c, r.width - kWords), z);
     }
   }
 }
@@ -385,10 +380,10 @@ __global__ __launch_bounds__(kRunThreads) void lookup_grad_runs_kernel(Runs r, c
   __shared__ int flags[kRunThreads / 8];
   const int strips = kRunThreads / group, strip = threadIdx.x / group, lane = threadIdx.x % group;
   const int64_t piece = (int64_t)blockIdx.x - zero_blocks, length = (int64_t)kStrip * strips_long;
-  const int64_t col = ((int64_t)blockIdx.y * group + lane) * V;
+  const int64_t pack = ((int64_t)blockIdx.y * group + lane) * V, col = min(pack, r.width - V);
   const int64_t begin = (piece * strips + strip) * length, end = begin + length;
   const uint32_t rows = (uint32_t)r.rows, *token = (const uint32_t*)r.payload;
-  const bool live = col < r.width;
+  const bool live = pack < r.width;
   uint32_t cur = begin < r.count ? r.keys[begin] : rows;
   int flag = 0;
   auto write = [&](uint32_t row, const W (&sum)[V]) {
@@ -587,16 +582,11 @@ __global__ __launch_bounds__(kThreads) void lookup_grad_join_kernel(Runs r, O* _
   }
 }
 
-template <typename T, int V> void launch_rows(const LookupArgs& a, int64_t tokens) {
-  int group = 64;
-  while (group > 1 && group / 2 * V >= a.width) group /= 2;
-  hipLaunchKernelGGL((lookup_rows_kernel<T, V>), dim3((unsigned)((tokens * group + kThreads - 1) / kThreads)), dim3(kThreads), 0, (hipStream_t)a.stream,
-                     (const T*)a.table, (const void*)a.ids, (T*)a.out, a.rows, a.width, a.table_stride, a.n1, a.s0, a.s1, (int)a.ids64, tokens, group,
-                     (Wide<T>)a.scale);
-}
+// Elements of a row a lane loads at a time.
+template <typename T> constexpr int kPack = 16 / sizeof(T);
 
 template <typename T> void run_lookup(const LookupArgs& a) {
-  const int64_t tokens = a.n0 * a.n1, size = sizeof(T);
+  const int64_t tokens = a.n0 * a.n1;
   if (a.width <= kNarrow) {
     TokenGrid grid;
     grid.ids64 = (int)a.ids64;
@@ -607,14 +597,12 @@ template <typename T> void run_lookup(const LookupArgs& a) {
     hipLaunchKernelGGL(lookup_tile_kernel<T>, dim3((unsigned)tiles.blocks), dim3(kThreads), 0, (hipStream_t)a.stream, (const T*)a.table, (const void*)a.ids,
                        (T*)a.out, a.rows, (int)a.width, a.table_stride, grid, tiles, (Wide<T>)a.scale);
   } else {
-    int64_t v = 16 / size;
-    while (v > 1 && (a.width % v || a.table_stride % v || a.table % (v * size))) v /= 2;
-    if (v == 1) launch_rows<T, 1>(a, tokens);
-    else if (v == 2) launch_rows<T, 2>(a, tokens);
-    else if constexpr (sizeof(T) <= 4) {
-      if (v == 4) launch_rows<T, 4>(a, tokens);
-      else if constexpr (sizeof(T) == 2) launch_rows<T, 8>(a, tokens);
-    }
+    constexpr int V = kPack<T>;
+    int group = 64;
+    while (group > 1 && group / 2 * V >= a.width) group /= 2;
+    hipLaunchKernelGGL((lookup_rows_kernel<T, V>), dim3((unsigned)((tokens * group + kThreads - 1) / kThreads)), dim3(kThreads), 0, (hipStream_t)a.stream,
+                       (const T*)a.table, (const void*)a.ids, (T*)a.out, a.rows, a.width, a.table_stride, a.n1, a.s0, a.s1, (int)a.ids64, tokens, group,
+                       (Wide<T>)a.scale);
   }
   LGA_HIP_CHECK(hipGetLastError());
 }
@@ -652,11 +640,7 @@ GradPlan plan_grad(const LookupGradArgs& a) {
   if (a.width <= kNarrow) {
     p.piece_tokens = kNarrowPiece;
   } else {
-    for (int v = (int)(16 / size); v > 1; v /= 2)
-      if (a.width % v == 0 && a.g0 % v == 0 && a.g1 % v == 0 && a.grad % (v * size) == 0) {
-        p.vec = v;
-        break;
-      }
+    p.vec = (int)(16 / size);
     while (p.group > 8 && p.group / 2 * p.vec >= a.width) p.group /= 2;
     p.strips_long = 1;
     while (p.strips_long < 8 && tiles.count / (kStrip * p.strips_long) > 32768) p.strips_long *= 2;
@@ -696,8 +680,7 @@ PrivatePlan plan_private(const LookupGradArgs& a) {
   p.lines = p.items_along0 ? p.grid.n1 : (p.grid.n1 + kPrivateItems - 1) / kPrivateItems;
   const int64_t side0 = p.items_along0 ? 64 * kPrivateItems : 64;
   p.steps = (p.grid.n0 + side0 - 1) / side0 * p.lines;
-  const int64_t pack = a.type == kF64 ? 2 : a.type == kF32 ? 4 : 8;
-  p.whole = !p.items_along0 && a.width == 1 && p.g1 == 1 && p.g0 % pack == 0 && a.grad % 16 == 0;
+  p.whole = !p.items_along0 && a.width == 1 && p.g1 == 1;
   p.lds = (int)((lds + 15) / 16 * 16);
   const int64_t fit = 256 * std::min<int64_t>(8, std::max<int64_t>(1, 163840 / p.lds));
   p.waves = (int)std::max<int64_t>(1, std::min({fit / a.width, p.steps, tokens / std::max<int64_t>(1024, a.rows)}));
@@ -759,16 +742,8 @@ template <typename T, typename O> void run_lookup_grad(const LookupGradArgs& a) 
     }
     if (!p.values)
       hipLaunchKernelGGL((lookup_grad_narrow_kernel<T, O, false>), grid, dim3(kThreads), 0, s, r, (const T*)a.grad, (O*)a.out, head, tail, zero_blocks, (W)a.scale);
-  } else if (p.vec == 1) {
-    launch_runs<T, O, 1>(a, p, r, head, tail);
-  } else if (p.vec == 2) {
-    launch_runs<T, O, 2>(a, p, r, head, tail);
-  } else if constexpr (sizeof(T) <= 4) {
-    if (p.vec == 4) {
-      launch_runs<T, O, 4>(a, p, r, head, tail);
-    } else if constexpr (sizeof(T) == 2) {
-      launch_runs<T, O, 8>(a, p, r, head, tail);
-    }
+  } else {
+    launch_runs<T, O, kPack<T>>(a, p, r, head, tail);
   }
   LGA_HIP_CHECK(hipGetLastError());
   hipLaunchKernelGGL((lookup_grad_join_kernel<W, O>), dim3((unsigned)p.pieces, (unsigned)std::min<int64_t>((a.width + 63) / 64, 8)), dim3(kThreads), 0, s, r, (O*)a.out, head, tail, p.piece_tokens, (W)a.scale);

@@ -172,6 +172,20 @@ __device__ __forceinline__ void carry_in(const Cut& k, uint64_t* work, int64_t t
   for (int v = 0; v < V; ++v) carry[v] = fma_wide(mine[v].a, carry[v], mine[v].h);
 }
 
+// The channels of a pack: d .. d + V - 1 of sequence b.  The last pack of a width that V does not divide starts earlier; its
+// first `again` channels are those of the pack before too.
+template <int V> struct Channels {
+  int64_t b, d;
+  int again;
+  __device__ __forceinline__ Channels(int64_t pack, int64_t width) {
+    const int64_t row = (width + V - 1) / V;
+    b = pack / row;
+    const int64_t first = (pack - b * row) * V;
+    d = min(first, width - V);
+    again = (int)(first - d);
+  }
+};
+
 template <typename G, GateKind K, int V> struct GateRow {
   const G* base = nullptr;
   int64_t step = 0;
@@ -211,7 +225,8 @@ __global__ __launch_bounds__(kLanes* kMaxSlots) void scan_kernel(ScanArgs a, Cut
   const int lane = threadIdx.x % k.lanes, slot = threadIdx.x / k.lanes;
   const int64_t pack = row * k.lanes + lane;
   const bool live = pack < k.packs;
-  const int64_t c = live ? pack * V : 0, b = c / a.width, d = c - b * a.width;
+  const Channels<V> at(live ? pack : 0, a.width);
+  const int64_t b = at.b, d = at.d, c = b * a.width + d;
   const int64_t t0 = (tile * k.slots + slot) * L, len = live ? length_of(a.lengths, b, a.steps) : 0;
   const T* x = (const T*)a.x + b * a.x_b + d;
   const GateRow<G, K, V> gate(a.gate, b, a.gate_b, a.gate_t, d, K == kSharedGate ? a.width / a.groups : 1);
@@ -318,7 +333,8 @@ __global__ __launch_bounds__(kLanes* kMaxSlots) void scan_grad_kernel(ScanGradAr
   const int lane = threadIdx.x % k.lanes, slot = threadIdx.x / k.lanes;
   const int64_t pack = row * k.lanes + lane;
   const bool live = pack < k.packs;
-  const int64_t c = live ? pack * V : 0, b = c / a.width, d = c - b * a.width;
+  const Channels<V> at(live ? pack : 0, a.width);
+  const int64_t b = at.b, d = at.d, c = b * a.width + d;
   const int64_t t0 = a.steps - 1 - (tile * k.slots + slot) * L, len = live ? length_of(a.lengths, b, a.steps) : 0;
   const T* dh = (const T*)a.grad_states + b * a.g_b + d;
   const T* hs = (const T*)a.states + b * a.h_b + d;
@@ -374,7 +390,7 @@ __global__ __launch_bounds__(kLanes* kMaxSlots) void scan_grad_kernel(ScanGradAr
   } else {
     for (int v = 0; v < V; ++v) e[v] = first[v];
   }
-  if (!live && !sums.team) return;
+  if (!live && (K != kSharedGate || !sums.team)) return;
   T* dx = (T*)a.grad_x + b * a.steps * a.width + d;
   G* da = (G*)a.grad_gate + b * a.steps * a.width + d;
   W* slope = (W*)slopes + b * a.steps * a.width + d;
@@ -406,25 +422,25 @@ __global__ __launch_bounds__(kLanes* kMaxSlots) void scan_grad_kernel(ScanGradAr
     if (t >= 0 && live) {
       store_pack<T, V>(dx + t * a.width, o);
       if constexpr (K != kNoGate) {
-        if (!sums.team) {
+        if (K != kSharedGate || !sums.team) {
           if (slopes) store_pack<W, V>(slope + t * a.width, os);
           else store_pack<G, V>(da + t * a.width, og);
         }
       }
     }
-    if constexpr (K != kNoGate) {
+    if constexpr (K == kSharedGate) {
       total[j] = 0;
-      for (int v = 0; v < V; ++v) total[j] += live ? os.v[v] : (W)0;
+      for (int v = 0; v < V; ++v) total[j] += live && v >= at.again ? os.v[v] : (W)0;
     }
   }
-  if constexpr (K != kNoGate) {
+  if constexpr (K == kSharedGate) {
     if (sums.team) {
       int mine;
       bool holds;
       team_sums<W, L>(total, sums.team, mine, holds);
-      const int64_t t = t0 - mine, at = pack / sums.team, r = at / sums.teams;
+      const int64_t t = t0 - mine, part = pack / sums.team, r = part / sums.teams;
       if (holds && t >= 0 && r < sums.rows) {
-        const int64_t to = (r * a.steps + t) * sums.teams + at - r * sums.teams;
+        const int64_t to = (r * a.steps + t) * sums.teams + part - r * sums.teams;
         if (sums.done) ((G*)a.grad_gate)[to] = (G)total[0];
         else ((W*)slopes)[to] = total[0];
       }
@@ -468,23 +484,12 @@ __global__ __launch_bounds__(kThreads) void gate_sum_kernel(const W* __restrict_
   }
 }
 
-bool aligned(int64_t address, int64_t bytes) { return address % bytes == 0; }
-
-// Two channels a lane where every row of every tensor starts at a multiple of both.
-template <typename A> bool even_rows(const A& a) {
-  const int64_t size = a.type == kF64 ? 8 : a.type == kF32 ? 4 : 2, gate = a.gate_type == kF64 ? 8 : a.gate_type == kF32 ? 4 : 2;
-  if (a.type == kF64 || a.width % 2 || a.x_b % 2 || a.x_t % 2 || !aligned(a.x, 2 * size)) return false;
-  return !a.gate || a.groups != a.width || (a.gate_b % 2 == 0 && a.gate_t % 2 == 0 && aligned(a.gate, 2 * gate));
-}
-bool two_wide(const ScanArgs& a) { return even_rows(a); }
-bool two_wide(const ScanGradArgs& a) {
-  const int64_t size = a.type == kF32 ? 8 : 4;
-  return even_rows(a) && a.g_b % 2 == 0 && a.g_t % 2 == 0 && a.h_b % 2 == 0 && a.h_t % 2 == 0 && aligned(a.grad_states, size) && aligned(a.states, size);
-}
+// Two channels a lane for the types of up to 32 bits.
+template <typename A> bool two_wide(const A& a) { return a.type != kF64 && a.width >= 2; }
 
 Cut cut_steps(int64_t batch, int64_t steps, int64_t width, int v, int per_lane, int max_slots) {
   Cut k;
-  k.packs = batch * width / v;
+  k.packs = batch * ((width + v - 1) / v);
   k.lanes = kLanes;
   while (k.lanes > 1 && k.lanes / 2 >= k.packs) k.lanes /= 2;
   const int64_t chunks = std::max<int64_t>(1, (steps + per_lane - 1) / per_lane);
@@ -550,7 +555,7 @@ bool sums_gates(const ScanGradArgs& a) { return a.gate && (a.groups != a.width |
 // backward kernel; a group like 103 channels has none, and its slopes go through memory value by value.
 GateSums gate_sums(const ScanGradArgs& a, const Cut& k, int v) {
   GateSums g;
-  if (!sums_gates(a)) return g;
+  if (!sums_gates(a) || a.groups == a.width) return g;
   const int64_t per = a.width / a.groups;
   const int most = std::min(k.lanes, 64);
   int team = 0;

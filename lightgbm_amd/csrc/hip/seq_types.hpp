@@ -16,8 +16,10 @@ template <typename T> using Wide = typename WideOf<T>::type;
 __device__ __forceinline__ float fma_wide(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
 __device__ __forceinline__ double fma_wide(double a, double b, double c) { return __builtin_fma(a, b, c); }
 
-// V neighbouring elements, loaded and stored as one word of V * sizeof(T) bytes.
-template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
+// V neighbouring elements, loaded and stored as words of up to 16 bytes wherever they start: global memory takes them at
+// any multiple of the element's size.  Where V does not divide a row, the row's last pack starts V before its end and
+// shares elements with the one before; both hold the same values of them.
+template <typename T, int V> struct __attribute__((packed, aligned(sizeof(T)))) Pack { T v[V]; };
 
 template <typename T, int V> __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
   return *reinterpret_cast<const Pack<T, V>*>(p);

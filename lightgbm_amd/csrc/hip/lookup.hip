@@ -327,20 +327,11 @@ __global__ __launch_bounds__(kThreads) void lookup_grad_total_kernel(const W* __
 struct Runs {
   const uint32_t* keys;     // sorted ids, `rows` for tokens that take no part
   const void* payload;      // token numbers, or (narrow kernel) the gradients themselves
+  const uint8_t* named;     // [rows]
   int64_t count;            // a multiple of the piece length
   int64_t rows, width, n1, g0, g1;
 };
 constexpr uint32_t kNobody = ~0u;
-
-__device__ __forceinline__ bool has_tokens(const Runs& r, uint32_t row) {
-  int64_t lo = 0, hi = r.count;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (r.keys[mid] < row) lo = mid + 1;
-    else hi = mid;
-  }
-  return lo < r.count && r.keys[lo] == row;
-}
 
 constexpr int kZeroRows = 16;      // rows a wave looks after
 
@@ -348,7 +339,7 @@ constexpr int kZeroRows = 16;      // rows a wave looks after
 template <typename O> __device__ __forceinline__ void zero_rows(const Runs& r, O* __restrict__ out, int64_t wave, int lane) {
   const int64_t first = wave * kZeroRows;
   if (first >= r.rows) return;
-  const bool absent = lane < kZeroRows && first + lane < r.rows && !has_tokens(r, (uint32_t)(first + lane));
+  const bool absent = lane < kZeroRows && first + lane < r.rows && !r.named[first + lane];
   uint64_t todo = __ballot(absent);
   constexpr int kWords = 16 / sizeof(O);
   while (todo) {
@@ -362,26 +353,27 @@ template <typename O> __device__ __forceinline__ void zero_rows(const Runs& r, O
   }
 }
 
-// Rows of more than kNarrow values: `group` lanes walk a strip of kStrip tokens, V columns a lane; the strips of a workgroup
+// Rows of more than kNarrow values: `group` lanes walk a strip of `length` tokens, V columns a lane; the strips of a workgroup
 // are a piece, and what crosses strips is joined in LDS.
-constexpr int kRunThreads = 512, kStrip = 32;
+constexpr int kRunThreads = 512, kStage = 32;     // ids and tokens of a strip wait in LDS, kStage at a time
 enum { kHasHead = 1, kThrough = 2, kHasTail = 4 };      // of a strip: ends / passes on the run it begins in, begins the run it ends in
 
 template <typename T, typename O, int V>
 __global__ __launch_bounds__(kRunThreads) void lookup_grad_runs_kernel(Runs r, const T* __restrict__ grad, O* __restrict__ out, Wide<T>* __restrict__ head,
-                                                                       Wide<T>* __restrict__ tail, int zero_blocks, int group, int strips_long, Wide<T> scale) {
+                                                                       Wide<T>* __restrict__ tail, int zero_blocks, int group, int length, Wide<T> scale) {
   typedef Wide<T> W;
   if ((int)blockIdx.x < zero_blocks) {
     if (blockIdx.y == 0) zero_rows(r, out, (int64_t)blockIdx.x * (kRunThreads / 64) + (threadIdx.x >> 6), threadIdx.x & 63);
     return;
   }
-  constexpr int kAhead = 8;     // (of its own)
+  constexpr int kAhead = 4;
   __shared__ W shead[kRunThreads * V], stail[kRunThreads * V];
+  __shared__ uint32_t skey[kRunThreads / 8 * kStage], stoken[kRunThreads / 8 * kStage];
   __shared__ int flags[kRunThreads / 8];
   const int strips = kRunThreads / group, strip = threadIdx.x / group, lane = threadIdx.x % group;
-  const int64_t piece = (int64_t)blockIdx.x - zero_blocks, length = (int64_t)kStrip * strips_long;
+  const int64_t piece = (int64_t)blockIdx.x - zero_blocks;
   const int64_t pack = ((int64_t)blockIdx.y * group + lane) * V, col = min(pack, r.width - V);
-  const int64_t begin = (piece * strips + strip) * length, end = begin + length;
+  const int64_t begin = (piece * strips + strip) * length, end = begin + length;      // lengths divide kSortTile
   const uint32_t rows = (uint32_t)r.rows, *token = (const uint32_t*)r.payload;
   const bool live = pack < r.width;
   uint32_t cur = begin < r.count ? r.keys[begin] : rows;
@@ -392,7 +384,8 @@ __global__ __launch_bounds__(kRunThreads) void lookup_grad_runs_kernel(Runs r, c
     store_pack<O, V>(out + (int64_t)row * r.width + col, o);
   };
   if (cur < rows) {
-    bool inside = begin == 0 || r.keys[begin - 1] != cur;
+    const uint32_t ahead = begin ? r.keys[begin - 1] : kNobody, behind = end < r.count ? r.keys[end] : kNobody;
+    bool inside = ahead != cur;
     W acc[V];
     for (int v = 0; v < V; ++v) acc[v] = 0;
     auto close = [&] {
@@ -403,31 +396,42 @@ __global__ __launch_bounds__(kRunThreads) void lookup_grad_runs_kernel(Runs r, c
         write(cur, acc);
       }
     };
-    for (int64_t at = begin; at < end && cur < rows; at += kAhead) {
-      uint32_t key[kAhead];
-      Pack<T, V> g[kAhead];
+    uint32_t *keys = skey + strip * kStage, *tokens = stoken + strip * kStage;
+    const int stage = min(kStage, length);
+    for (int64_t at = begin; at < end && cur < rows; at += stage) {
+      in_order();                     // the strip's lanes are of one wave
+      for (int n = lane; n < stage; n += group) {
+        keys[n] = r.keys[at + n];
+        tokens[n] = token[at + n];
+      }
+      in_order();
+#pragma unroll 1
+      for (int from = 0; from < stage && cur < rows; from += kAhead) {
+        uint32_t key[kAhead];
+        Pack<T, V> g[kAhead];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) key[u] = r.keys[at + u];
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (key[u] < rows && live) {
-          const uint32_t tk = token[at + u], i = tk / (uint32_t)r.n1, j = tk - i * (uint32_t)r.n1;
-          g[u] = load_pack<T, V>(grad + i * r.g0 + j * r.g1 + col);
+        for (int u = 0; u < kAhead; ++u) {
+          key[u] = keys[from + u];
+          if (key[u] < rows && live) {
+            const uint32_t tk = tokens[from + u], i = tk / (uint32_t)r.n1, j = tk - i * (uint32_t)r.n1;
+            g[u] = load_pack<T, V>(grad + i * r.g0 + j * r.g1 + col);
+          }
         }
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        if (key[u] != cur) {
-          if (cur < rows) close();
-          cur = key[u];
-          inside = true;
-          for (int v = 0; v < V; ++v) acc[v] = 0;
+        for (int u = 0; u < kAhead; ++u) {
+          if (key[u] != cur) {
+            if (cur < rows) close();
+            cur = key[u];
+            inside = true;
+            for (int v = 0; v < V; ++v) acc[v] = 0;
+          }
+          if (cur < rows)
+            for (int v = 0; v < V; ++v) acc[v] += (W)g[u].v[v];
         }
-        if (cur < rows)
-          for (int v = 0; v < V; ++v) acc[v] += (W)g[u].v[v];
       }
     }
     if (cur < rows) {
-      if (end >= r.count || r.keys[end] != cur) {
+      if (behind != cur) {
         close();
       } else {
         flag |= inside ? kHasTail : kHasHead | kThrough;
@@ -468,7 +472,7 @@ __global__ __launch_bounds__(kThreads) void lookup_grad_narrow_kernel(Runs r, co
   typedef Wide<T> W;
   if ((int)blockIdx.x < zero_blocks) {
     const int64_t row = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (row < r.rows && !has_tokens(r, (uint32_t)row))
+    if (row < r.rows && !r.named[row])
       for (int64_t c = 0; c < r.width; ++c) out[row * r.width + c] = (O)0.f;
     return;
   }
@@ -614,7 +618,7 @@ constexpr int64_t kPrivateLds = 81920;      // of a wave, for the sums of a colu
 struct GradPlan {
   TokenGrid grid;
   int64_t g0, g1;
-  int payload, vec, group, strips_long = 1;
+  int payload, vec, group, strip = 32;
   bool values;
   int64_t piece_tokens, pieces, sort_bytes, parts_bytes;
 };
@@ -642,9 +646,11 @@ GradPlan plan_grad(const LookupGradArgs& a) {
   } else {
     p.vec = (int)(16 / size);
     while (p.group > 8 && p.group / 2 * p.vec >= a.width) p.group /= 2;
-    p.strips_long = 1;
-    while (p.strips_long < 8 && tiles.count / (kStrip * p.strips_long) > 32768) p.strips_long *= 2;
-    p.piece_tokens = (int64_t)kStrip * p.strips_long * (kRunThreads / p.group);
+    // shorter strips where there are few: 901 tokens of 3154 fp16 values 17 us with 16, 25 us with 32; 65537 of 1024 bf16
+    // values 51 us with 16, 49 us with 32
+    p.strip = tiles.count <= 16384 ? 16 : 32;
+    while (p.strip < 256 && tiles.count / p.strip > 32768) p.strip *= 2;
+    p.piece_tokens = (int64_t)p.strip * (kRunThreads / p.group);
   }
   p.pieces = (tiles.count + p.piece_tokens - 1) / p.piece_tokens;
   p.sort_bytes = token_sort_workspace(p.grid, p.payload);
@@ -691,7 +697,7 @@ template <typename T, typename O, int V> void launch_runs(const LookupGradArgs& 
   const int64_t zero_blocks = (a.rows + kZeroRows * (kRunThreads / 64) - 1) / (kZeroRows * (kRunThreads / 64));
   const dim3 grid((unsigned)(zero_blocks + p.pieces), (unsigned)((a.width + p.group * V - 1) / (p.group * V)));
   hipLaunchKernelGGL((lookup_grad_runs_kernel<T, O, V>), grid, dim3(kRunThreads), 0, (hipStream_t)a.stream, r, (const T*)a.grad, (O*)a.out, head, tail,
-                     (int)zero_blocks, p.group, p.strips_long, (Wide<T>)a.scale);
+                     (int)zero_blocks, p.group, p.strip, (Wide<T>)a.scale);
 }
 
 template <typename T, typename O> void run_lookup_grad(const LookupGradArgs& a) {
@@ -730,7 +736,7 @@ template <typename T, typename O> void run_lookup_grad(const LookupGradArgs& a) 
   }
   const GradPlan p = plan_grad(a);
   const SortedTokens t = token_sort(p.grid, p.values ? (const void*)a.grad : nullptr, p.g0, p.g1, p.payload, (void*)a.work, s);
-  const Runs r{t.keys, t.payload, t.count, a.rows, a.width, p.grid.n1, p.g0, p.g1};
+  const Runs r{t.keys, t.payload, t.named, t.count, a.rows, a.width, p.grid.n1, p.g0, p.g1};
   W* head = (W*)((char*)a.work + p.sort_bytes);
   W* tail = (W*)((char*)head + p.parts_bytes);
   if (a.width <= kNarrow) {

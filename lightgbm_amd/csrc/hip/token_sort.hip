@@ -19,6 +19,7 @@ struct Pass {
   const uint32_t* keys_in;      // null: first pass, keys come from the grid
   const void* payload_in;
   int64_t v0, v1;               // first pass: payload (i, j) is at i * v0 + j * v1; payload_in null: the token's number
+  uint8_t* named;               // cleared by the first count, set by the last scatter (null in the other passes)
   int shift, bits;
   bool few;                     // few tiles: no kernel of its own for the offsets
 };
@@ -51,6 +52,8 @@ __global__ __launch_bounds__(kThreads) void sort_count_kernel(Pass p, uint32_t* 
   const int64_t b = blockIdx.x;
   for (int d = threadIdx.x; d < kBins; d += kThreads) bin[d] = 0;
   __syncthreads();
+  if (!p.keys_in)
+    for (int64_t r = b * kThreads + threadIdx.x; r < p.grid.rows; r += (int64_t)gridDim.x * kThreads) p.named[r] = 0;
   const uint32_t mask = (1u << p.bits) - 1;
 #pragma unroll 4
   for (int k = 0; k < kItems; ++k) {
@@ -210,6 +213,7 @@ __global__ __launch_bounds__(kThreads) void sort_scatter_kernel(Pass p, const ui
     const uint32_t to = global[digit] + n - local[digit];
     keys_out[to] = ky;
     payload_out[to] = spay[n];
+    if (p.named && ky < (uint32_t)p.grid.rows) p.named[ky] = 1;
   }
 }
 
@@ -228,6 +232,7 @@ __global__ __launch_bounds__(kOneThreads) void sort_one_kernel(Pass p, int passe
   const uint32_t tokens = (uint32_t)(p.grid.n0 * p.grid.n1);
   uint32_t key[kOneItems], rank[kOneItems];
   P pay[kOneItems];
+  for (int64_t r = t; r < p.grid.rows; r += kOneThreads) p.named[r] = 0;
 #pragma unroll
   for (int k = 0; k < kOneItems; ++k) {
     const uint32_t q = wave * (kSortTile / kOneWaves) + k * 64 + lane;
@@ -301,6 +306,7 @@ __global__ __launch_bounds__(kOneThreads) void sort_one_kernel(Pass p, int passe
     const int q = wave * (kSortTile / kOneWaves) + k * 64 + lane;
     keys_out[q] = key[k];
     payload_out[q] = pay[k];
+    if (key[k] < (uint32_t)p.grid.rows) p.named[key[k]] = 1;      // behind the barriers of the passes
   }
 }
 
@@ -313,9 +319,9 @@ int bit_length(int64_t v) {
 }
 
 struct Layout {
-  int64_t keys[2], payload[2], counts, totals, bytes;
+  int64_t keys[2], payload[2], counts, totals, named, bytes;
 };
-Layout layout(const TokenTiles& t, int payload) {
+Layout layout(const TokenTiles& t, int payload, int64_t rows) {
   Layout l;
   int64_t at = 0;
   auto take = [&](int64_t n) { const int64_t here = at; at += (n + 255) / 256 * 256; return here; };
@@ -325,6 +331,7 @@ Layout layout(const TokenTiles& t, int payload) {
   }
   l.counts = take(t.blocks * kBins * 4);
   l.totals = take(kBins * 4);
+  l.named = take(rows);
   l.bytes = at;
   return l;
 }
@@ -362,17 +369,18 @@ TokenTiles sort_tiles(const TokenGrid& g) {
   return t;
 }
 
-int64_t token_sort_workspace(const TokenGrid& g, int payload) { return layout(sort_tiles(g), payload).bytes; }
+int64_t token_sort_workspace(const TokenGrid& g, int payload) { return layout(sort_tiles(g), payload, g.rows).bytes; }
 
 SortedTokens token_sort(const TokenGrid& g, const void* values, int64_t v0, int64_t v1, int payload, void* workspace, hipStream_t s) {
   const TokenTiles tiles = sort_tiles(g);
-  const Layout l = layout(tiles, payload);
+  const Layout l = layout(tiles, payload, g.rows);
   char* w = (char*)workspace;
   const int bits = bit_length(g.rows), passes = (bits + kMaxBits - 1) / kMaxBits, each = (bits + passes - 1) / passes;
   const bool small = tiles.bits == 10;
   const dim3 grid((unsigned)tiles.blocks), block(kThreads);
   uint32_t *counts = (uint32_t*)(w + l.counts), *totals = (uint32_t*)(w + l.totals);
-  Pass p{g, tiles, nullptr, values, v0, v1, 0, each, small};
+  uint8_t* named = (uint8_t*)(w + l.named);
+  Pass p{g, tiles, nullptr, values, v0, v1, named, 0, each, small};
   if (one_tile(g)) {
     uint32_t* keys = (uint32_t*)(w + l.keys[0]);
     void* pay = w + l.payload[0];
@@ -380,7 +388,7 @@ SortedTokens token_sort(const TokenGrid& g, const void* values, int64_t v0, int6
     if (payload == 8) hipLaunchKernelGGL(sort_one_kernel<uint64_t>, dim3(1), dim3(kOneThreads), 0, s, p, passes, bits, keys, (uint64_t*)pay);
     else hipLaunchKernelGGL(sort_one_kernel<uint32_t>, dim3(1), dim3(kOneThreads), 0, s, p, passes, bits, keys, (uint32_t*)pay);
     LGA_HIP_CHECK(hipGetLastError());
-    return {keys, pay, tiles.count};
+    return {keys, pay, named, tiles.count};
   }
   for (int k = 0; k < passes; ++k) {
     p.shift = k * each;
@@ -394,6 +402,7 @@ SortedTokens token_sort(const TokenGrid& g, const void* values, int64_t v0, int6
       hipLaunchKernelGGL(sort_offsets_kernel, dim3(1u << p.bits), block, 0, s, counts, totals, tiles.blocks);
       LGA_HIP_CHECK(hipGetLastError());
     }
+    p.named = k + 1 == passes ? named : nullptr;
     auto scatter = [&](auto kernel, auto* to) {
       hipLaunchKernelGGL(kernel, grid, block, 0, s, p, counts, totals, keys, to);
     };
@@ -408,7 +417,7 @@ SortedTokens token_sort(const TokenGrid& g, const void* values, int64_t v0, int6
     p.keys_in = keys;
     p.payload_in = pay;
   }
-  return {p.keys_in, p.payload_in, tiles.count};
+  return {p.keys_in, p.payload_in, named, tiles.count};
 }
 
 }  // namespace lga

@@ -35,11 +35,12 @@ __device__ __forceinline__ int tile_slot(int q) { return (q & ~63) | ((q ^ (q >>
 int64_t token_sort_workspace(const TokenGrid& g, int payload);
 
 // Sorts ids with the payload of every token: its number i * n1 + j (values == nullptr, payload 4), or its value
-// values[i * v0 + j * v1] of `payload` bytes (4 or 8).  keys (uint32) and payloads are in the workspace.
+// values[i * v0 + j * v1] of `payload` bytes (4 or 8).  keys (uint32), payloads and the named rows are in the workspace.
 TokenTiles sort_tiles(const TokenGrid& g);      // what a sort of g uses
 struct SortedTokens {
   const uint32_t* keys = nullptr;
   const void* payload = nullptr;
+  const uint8_t* named = nullptr;      // [rows]: 1 where an id names the row
   int64_t count = 0;
 };
 SortedTokens token_sort(const TokenGrid& g, const void* values, int64_t v0, int64_t v1, int payload, void* workspace, hipStream_t s);

@@ -168,8 +168,9 @@ constexpr int kPrivateItems = 32;     // tokens a lane holds
 constexpr int kGroup = 4;             // of which so many are added at a time
 
 // A step: 64 x kPrivateItems tokens; lanes along axis 0, items along axis 1 or (few tokens there) along axis 0 too.  A step
-// is loaded while the one before is added up.  kWhole: gradients of one
-// value that are neighbours along axis 1.
+// is loaded while the one before is added up.  Every step runs the same straight code, which a wave of few steps mostly waits
+// for: places behind an edge are read at the edge and take no part.  kWhole: gradients of one value that are neighbours along
+// axis 1.
 template <typename T, typename I, bool kAlong0, bool kWhole>
 __global__ __launch_bounds__(64) void lookup_grad_private_kernel(const T* __restrict__ grad, TokenGrid grid, int64_t g0, int64_t g1, int width, int row_bits,
                                                                  int lines, int steps, int each, Wide<T>* __restrict__ parts) {
@@ -182,64 +183,67 @@ __global__ __launch_bounds__(64) void lookup_grad_private_kernel(const T* __rest
   for (int k = lane; k <= rows; k += 64) sums[k] = 0;
   __syncthreads();
   constexpr int item_i = kAlong0 ? 64 : 0, item_j = kAlong0 ? 0 : 1;
-  auto place = [&](int step, int64_t& i0, int64_t& j0) {
+  const I* ids = (const I*)grid.ids;
+  // Where a step's items begin; its first `again` items belong to the step before (the last step of a line is moved back).
+  auto place = [&](int step, int64_t& i0, int64_t& j0, int& again) {
     const int si = step / lines, line = step - si * lines;
     i0 = (int64_t)si * 64 * (kAlong0 ? kPrivateItems : 1) + lane;
     j0 = (int64_t)line * (kAlong0 ? 1 : kPrivateItems);
-  };
-  const I* ids = (const I*)grid.ids;
-  // All of a lane's items are there; a lane behind the edge of axis 0 reads the last ones and takes no part.
-  auto inner = [&](int64_t i0, int64_t j0) {
-    return kAlong0 ? i0 - lane + 64 * kPrivateItems <= grid.n0 : j0 + kPrivateItems <= grid.n1;
-  };
-  auto load = [&](int step, I (&id)[kPrivateItems], T (&g)[kPrivateItems]) {
-    int64_t i0, j0;
-    place(step, i0, j0);
-    if (inner(i0, j0)) {
-      i0 = min(i0, grid.n0 - 1);
-      const I* at = ids + i0 * grid.s0 + j0 * grid.s1;
-      const int64_t next = kAlong0 ? 64 * grid.s0 : grid.s1;
-#pragma unroll
-      for (int u = 0; u < kPrivateItems; ++u) id[u] = at[u * next];
-      const T* from = grad + i0 * g0 + j0 * g1;
-      if constexpr (kWhole) {
-        constexpr int V = 16 / sizeof(T);
-#pragma unroll
-        for (int u = 0; u < kPrivateItems; u += V) {
-          const Pack<T, V> x = load_pack<T, V>(from + u);
-#pragma unroll
-          for (int v = 0; v < V; ++v) g[u + v] = x.v[v];
-        }
-      } else {
-        const int64_t on = kAlong0 ? 64 * g0 : g1;
-#pragma unroll
-        for (int u = 0; u < kPrivateItems; ++u) g[u] = from[u * on];
-      }
-    } else {
-#pragma unroll
-      for (int u = 0; u < kPrivateItems; ++u) {
-        const int64_t i = i0 + u * item_i, j = j0 + u * item_j;
-        id[u] = -1;
-        g[u] = (T)0.f;
-        if (i < grid.n0 && j < grid.n1) id[u] = ids[i * grid.s0 + j * grid.s1], g[u] = grad[i * g0 + j * g1];
-      }
+    again = 0;
+    if constexpr (!kAlong0) {
+      again = (int)max((int64_t)0, j0 + kPrivateItems - grid.n1);
+      j0 -= again;
     }
   };
   int32_t row[kPrivateItems];
   I next_id[kPrivateItems];
   T g[kPrivateItems], next_g[kPrivateItems];
-  const int end = min(steps, ((int)blockIdx.x + 1) * each);
-  if ((int)blockIdx.x * each < steps) load(blockIdx.x * each, next_id, next_g);
-  for (int step = blockIdx.x * each; step < end; ++step) {
-    int64_t i0, j0;
-    place(step, i0, j0);
-    const int limit = i0 < grid.n0 ? rows : 0;
+  const int first = blockIdx.x * each, end = min(steps, first + each);
+  for (int ahead = first; ahead <= end; ++ahead) {      // the step that is loaded; the one before is added up
+    const int step = ahead - 1;
+    int64_t i0 = 0, j0 = 0;
+    int again = 0;
+    if (step >= first) {
+      place(step, i0, j0, again);
 #pragma unroll
-    for (int u = 0; u < kPrivateItems; ++u) {
-      row[u] = next_id[u] >= 0 && next_id[u] < limit ? (int32_t)next_id[u] : rows;
-      g[u] = next_g[u];
+      for (int u = 0; u < kPrivateItems; ++u) {
+        const int limit = i0 + u * item_i < grid.n0 && u >= again ? rows : 0;
+        row[u] = next_id[u] >= 0 && next_id[u] < limit ? (int32_t)next_id[u] : rows;
+        g[u] = next_g[u];
+      }
     }
-    if (step + 1 < end) load(step + 1, next_id, next_g);
+    if (ahead < end) {
+      int64_t i, j;
+      int skip;
+      place(ahead, i, j, skip);
+      if constexpr (kAlong0) {
+#pragma unroll
+        for (int u = 0; u < kPrivateItems; ++u) {
+          const int64_t at = min(i + u * 64, grid.n0 - 1);
+          next_id[u] = ids[at * grid.s0 + j * grid.s1];
+          next_g[u] = grad[at * g0 + j * g1];
+        }
+      } else {
+        i = min(i, grid.n0 - 1);
+        const I* at = ids + i * grid.s0 + j * grid.s1;
+        const T* from = grad + i * g0 + j * g1;
+#pragma unroll
+        for (int u = 0; u < kPrivateItems; ++u) next_id[u] = at[u * grid.s1];
+        if constexpr (kWhole) {
+          constexpr int V = 16 / sizeof(T);
+#pragma unroll
+          for (int u = 0; u < kPrivateItems; u += V) {
+            const Pack<T, V> x = load_pack<T, V>(from + u);
+#pragma unroll
+            for (int v = 0; v < V; ++v) next_g[u + v] = x.v[v];
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < kPrivateItems; ++u) next_g[u] = from[u * g1];
+        }
+      }
+    }
+    if (step < first) continue;
     uint32_t meets = 0;               // groups of items in which lanes share a row: later, read once more
 #pragma unroll
     for (int u0 = 0; u0 < kPrivateItems; u0 += kGroup) {
@@ -277,7 +281,7 @@ __global__ __launch_bounds__(64) void lookup_grad_private_kernel(const T* __rest
       const int u0 = __ffs(meets) - 1;
       for (int u = u0; u < u0 + kGroup; ++u) {
         const int64_t i = i0 + u * item_i, j = j0 + u * item_j;
-        const bool there = i < grid.n0 && j < grid.n1;
+        const bool there = i < grid.n0 && u >= again;
         const I id = there ? ids[i * grid.s0 + j * grid.s1] : (I)-1;
         const W value = there ? (W)grad[i * g0 + j * g1] : (W)0;
         const int at = id >= 0 && id < rows ? (int)id : rows;
@@ -300,17 +304,19 @@ __global__ __launch_bounds__(64) void lookup_grad_private_kernel(const T* __rest
   for (int k = lane; k < rows; k += 64) parts[((int64_t)blockIdx.x * rows + k) * width + blockIdx.y] = sums[k];
 }
 
-// out = scale * the waves' sums, 64 values side by side, the waves in kThreads / 64 parts.
+// out = scale * the waves' sums, 64 values side by side, the waves in kTotalThreads / 64 parts.
+constexpr int kTotalThreads = 1024;
+
 template <typename W, typename O>
-__global__ __launch_bounds__(kThreads) void lookup_grad_total_kernel(const W* __restrict__ parts, O* __restrict__ out, int64_t values, int waves, W scale) {
-  constexpr int kParts = kThreads / 64;
+__global__ __launch_bounds__(kTotalThreads) void lookup_grad_total_kernel(const W* __restrict__ parts, O* __restrict__ out, int64_t values, int waves, W scale) {
+  constexpr int kParts = kTotalThreads / 64;
   __shared__ W of_part[kParts][64];
   const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
   const int64_t at = (int64_t)blockIdx.x * 64 + lane;
   const int each = (waves + kParts - 1) / kParts, from = part * each, to = min(waves, from + each);
   W sum = 0;
   if (at < values) {
-#pragma unroll 8
+#pragma unroll 16
     for (int w = from; w < to; ++w) sum += parts[(int64_t)w * values + at];
   }
   of_part[part][lane] = sum;
@@ -613,7 +619,7 @@ template <typename T> void run_lookup(const LookupArgs& a) {
 
 // Up to this many tokens every workgroup looks through all ids for its own rows; above, they are sorted.
 constexpr int64_t kOwnedTokens = 512;
-constexpr int64_t kPrivateLds = 81920;      // of a wave, for the sums of a column
+constexpr int64_t kPrivateLds = 160 * 1024;      // of a wave, for the sums of a column
 
 struct GradPlan {
   TokenGrid grid;
@@ -682,7 +688,7 @@ PrivatePlan plan_private(const LookupGradArgs& a) {
     std::swap(p.grid.s0, p.grid.s1);
     std::swap(p.g0, p.g1);
   }
-  p.items_along0 = p.grid.n1 < kPrivateItems / 2;
+  p.items_along0 = p.grid.n1 < kPrivateItems;
   p.lines = p.items_along0 ? p.grid.n1 : (p.grid.n1 + kPrivateItems - 1) / kPrivateItems;
   const int64_t side0 = p.items_along0 ? 64 * kPrivateItems : 64;
   p.steps = (p.grid.n0 + side0 - 1) / side0 * p.lines;
@@ -729,7 +735,7 @@ template <typename T, typename O> void run_lookup_grad(const LookupGradArgs& a) 
     };
     a.ids64 ? by_ids((int64_t)0) : by_ids((int32_t)0);
     LGA_HIP_CHECK(hipGetLastError());
-    hipLaunchKernelGGL((lookup_grad_total_kernel<W, O>), dim3((unsigned)((values + 63) / 64)), dim3(kThreads), 0, s, parts, (O*)a.out, values, few.waves,
+    hipLaunchKernelGGL((lookup_grad_total_kernel<W, O>), dim3((unsigned)((values + 63) / 64)), dim3(kTotalThreads), 0, s, parts, (O*)a.out, values, few.waves,
                        (W)a.scale);
     LGA_HIP_CHECK(hipGetLastError());
     return;

@@ -55,42 +55,67 @@ __global__ __launch_bounds__(kThreads) void lookup_rows_kernel(const T* __restri
 
 // Narrow rows: a workgroup takes a tile of tokens, reads its ids along the axis on which they are neighbours, and writes
 // along the axis on which the results are.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void lookup_tile_kernel(const T* __restrict__ table, const void* __restrict__ ids, T* __restrict__ out, int64_t rows,
+template <typename T, typename I, int kBits>
+__global__ __launch_bounds__(kThreads) void lookup_tile_kernel(const T* __restrict__ table, const I* __restrict__ ids, T* __restrict__ out, int64_t rows,
                                                                int width, int64_t table_stride, TokenGrid grid, TokenTiles tiles, Wide<T> scale) {
-  __shared__ int32_t id_of[kSortTile];
-  const int shift1 = tiles.shift1, side1 = 1 << shift1, shift0 = tiles.bits - shift1, size = 1 << tiles.bits;
+  constexpr int kSize = 1 << kBits, kItems = kSize / kThreads;
+  __shared__ int32_t id_of[kSize];
+  const int shift1 = tiles.shift1, side1 = 1 << shift1, shift0 = kBits - shift1;
   const int64_t ti = blockIdx.x / tiles.across, i0 = ti << shift0, j0 = (blockIdx.x - ti * tiles.across) << shift1;
   const bool along0 = grid.s0 < grid.s1;
-#pragma unroll 8
-  for (int n = threadIdx.x; n < size; n += kThreads) {
-    const int i = along0 ? n & ((1 << shift0) - 1) : n >> shift1, j = along0 ? n >> shift0 : n & (side1 - 1);
-    int32_t id = -1;
-    if (i0 + i < grid.n0 && j0 + j < grid.n1) {
-      const int64_t v = load_id(ids, (i0 + i) * grid.s0 + (j0 + j) * grid.s1, grid.ids64);
-      if (v >= 0 && v < rows) id = (int32_t)v;
+  const int live1 = (int)min((int64_t)side1, grid.n1 - j0), live0 = (int)min((int64_t)1 << shift0, grid.n0 - i0);
+  // A lane's items are kThreads apart, which is a fixed way in both walks unless an axis is longer than that and not all.
+  const bool whole = live0 == 1 << shift0 && live1 == side1 && (shift1 <= 8 || shift1 == kBits);
+  const int t = threadIdx.x;
+  if (whole) {
+    const int i = along0 ? t & ((1 << shift0) - 1) : t >> shift1, j = along0 ? t >> shift0 : t & (side1 - 1);
+    const int64_t next = along0 ? (int64_t)(kThreads >> shift0) * grid.s1 : shift1 <= 8 ? (int64_t)(kThreads >> shift1) * grid.s0 : kThreads * grid.s1;
+    const I* from = ids + (i0 + i) * grid.s0 + (j0 + j) * grid.s1;
+    I id[kItems];
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) id[k] = from[k * next];
+    int at = i << shift1 | j;
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      id_of[tile_slot(at)] = id[k] >= 0 && id[k] < rows ? (int32_t)id[k] : -1;
+      at += along0 ? kThreads >> shift0 : kThreads;
     }
-    id_of[tile_slot(i << shift1 | j)] = id;
+  } else {
+    for (int n = t; n < kSize; n += kThreads) {
+      const int i = along0 ? n & ((1 << shift0) - 1) : n >> shift1, j = along0 ? n >> shift0 : n & (side1 - 1);
+      int32_t id = -1;
+      if (i < live0 && j < live1) {
+        const I v = ids[(i0 + i) * grid.s0 + (j0 + j) * grid.s1];
+        if (v >= 0 && v < rows) id = (int32_t)v;
+      }
+      id_of[tile_slot(i << shift1 | j)] = id;
+    }
   }
   __syncthreads();
-  const int live1 = (int)min((int64_t)side1, grid.n1 - j0), live0 = (int)min((int64_t)1 << shift0, grid.n0 - i0);
+  auto value = [&](int32_t id, int col) { return id >= 0 ? (T)((Wide<T>)table[id * table_stride + col] * scale) : (T)(Wide<T>)0; };
   if (width == 1) {
-#pragma unroll 8
-    for (int n = threadIdx.x; n < size; n += kThreads) {
+    if (whole) {
+      T* to = out + (i0 + (t >> shift1)) * grid.n1 + j0 + (t & (side1 - 1));
+      const int64_t next = shift1 <= 8 ? (int64_t)(kThreads >> shift1) * grid.n1 : kThreads;
+      T v[kItems];
+#pragma unroll
+      for (int k = 0; k < kItems; ++k) v[k] = value(id_of[tile_slot(t + k * kThreads)], 0);
+#pragma unroll
+      for (int k = 0; k < kItems; ++k) to[k * next] = v[k];
+      return;
+    }
+    for (int n = t; n < kSize; n += kThreads) {
       const int i = n >> shift1, j = n & (side1 - 1);
-      if (i >= live0 || j >= live1) continue;
-      const int32_t id = id_of[tile_slot(n)];
-      out[(i0 + i) * grid.n1 + j0 + j] = id >= 0 ? (T)((Wide<T>)table[id * table_stride] * scale) : (T)(Wide<T>)0;
+      if (i < live0 && j < live1) out[(i0 + i) * grid.n1 + j0 + j] = value(id_of[tile_slot(n)], 0);
     }
     return;
   }
   // divisions by multiplication: exact, as no n times its divisor reaches 2^32
   const uint32_t line = live1 * width, total = live0 * line, by_line = (uint32_t)((1ull << 32) / line + 1), by_width = (uint32_t)((1ull << 32) / width + 1);
 #pragma unroll 4
-  for (uint32_t n = threadIdx.x; n < total; n += kThreads) {
-    const uint32_t i = line > 1 ? __umulhi(n, by_line) : n, e = n - i * line, j = __umulhi(e, by_width);
-    const int32_t id = id_of[tile_slot(i << shift1 | j)];
-    out[((i0 + i) * grid.n1 + j0) * width + e] = id >= 0 ? (T)((Wide<T>)table[id * table_stride + e - j * width] * scale) : (T)(Wide<T>)0;
+  for (uint32_t n = t; n < total; n += kThreads) {
+    const uint32_t i = __umulhi(n, by_line), e = n - i * line, j = __umulhi(e, by_width);
+    out[((i0 + i) * grid.n1 + j0) * width + e] = value(id_of[tile_slot(i << shift1 | j)], e - j * width);
   }
 }
 
@@ -604,8 +629,15 @@ template <typename T> void run_lookup(const LookupArgs& a) {
     grid.rows = a.rows;
     TokenTiles tiles = token_tiles(grid, 10);      // small tiles until there are enough for every CU
     if (tiles.blocks > 4096) tiles = token_tiles(grid);
-    hipLaunchKernelGGL(lookup_tile_kernel<T>, dim3((unsigned)tiles.blocks), dim3(kThreads), 0, (hipStream_t)a.stream, (const T*)a.table, (const void*)a.ids,
-                       (T*)a.out, a.rows, (int)a.width, a.table_stride, grid, tiles, (Wide<T>)a.scale);
+    auto run = [&](auto kernel, auto* ids) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)tiles.blocks), dim3(kThreads), 0, (hipStream_t)a.stream, (const T*)a.table, ids, (T*)a.out, a.rows,
+                         (int)a.width, a.table_stride, grid, tiles, (Wide<T>)a.scale);
+    };
+    auto by_ids = [&](auto* ids) {
+      typedef std::remove_const_t<std::remove_pointer_t<decltype(ids)>> I;
+      tiles.bits == 10 ? run(lookup_tile_kernel<T, I, 10>, ids) : run(lookup_tile_kernel<T, I, 12>, ids);
+    };
+    a.ids64 ? by_ids((const int64_t*)a.ids) : by_ids((const int32_t*)a.ids);
   } else {
     constexpr int V = kPack<T>;
     int group = 64;

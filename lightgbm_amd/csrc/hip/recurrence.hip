@@ -22,7 +22,6 @@ constexpr int kThreads = 256;
 constexpr int kLanes = 64;          // channel packs of a tile
 constexpr int kScanSteps = 16, kGradSteps = 8;      // steps a lane holds
 constexpr int kMaxSlots = 16;       // chunks of a tile
-constexpr int kCheckpoint = 32;     // every 32nd tile hands on the state itself, so that no tile folds more than 31 maps
 constexpr uint64_t kEmpty = ~0ull;  // a word nobody has written yet: a NaN that publish() never stores
 
 enum GateKind { kNoGate, kOwnGate, kSharedGate };
@@ -95,12 +94,13 @@ struct Cut {
   int64_t pack_rows;  // workgroups side by side: packs / lanes, rounded up
   int64_t tiles;      // workgroups one behind the other
   int lanes, slots;   // of a workgroup
+  int checkpoint;     // every so many tiles one hands on the state itself: no tile folds more maps than come behind it
 };
 
 // Workspace of a cut into several tiles, in words: [0] tickets, then the tiles' maps, then the checkpoints' states.
 template <typename W> __host__ __device__ inline int64_t map_words(const Cut& k, int v) { return k.tiles * k.pack_rows * k.lanes * v * kMapWords<W>; }
 template <typename W> inline int64_t work_words(const Cut& k, int v) {
-  return k.tiles < 2 ? 0 : 8 + map_words<W>(k, v) + (k.tiles / kCheckpoint + 1) * k.pack_rows * k.lanes * v * kMapWords<W>;
+  return k.tiles < 2 ? 0 : 8 + map_words<W>(k, v) + (k.tiles / k.checkpoint + 1) * k.pack_rows * k.lanes * v * kMapWords<W>;
 }
 
 // Which tile a workgroup is.  Several tiles: by ticket, in the order in which workgroups really start, so that whatever a
@@ -139,7 +139,7 @@ __device__ __forceinline__ void carry_in(const Cut& k, uint64_t* work, int64_t t
     uint64_t* checkpoints = tile_maps + k.tiles * stride;
     if (slot == k.slots - 1 && tile + 1 < k.tiles)
       for (int v = 0; v < V; ++v) publish(tile_maps + tile * stride + v * kMapWords<W>, after(own[v], mine[v]));
-    const int64_t from = tile / kCheckpoint * kCheckpoint;    // first tile behind the last checkpoint
+    const int64_t from = tile / k.checkpoint * k.checkpoint;    // first tile behind the last checkpoint
     const int before = (int)(tile - from), share = (before + k.slots - 1) / k.slots;
     Map<W> part[V];
     for (int v = 0; v < V; ++v) part[v] = {1, 0};
@@ -153,7 +153,7 @@ __device__ __forceinline__ void carry_in(const Cut& k, uint64_t* work, int64_t t
     if (from > 0)
       for (int v = 0; v < V; ++v) {
         Map<W> m;
-        fetch(checkpoints + (from / kCheckpoint - 1) * stride + v * kMapWords<W>, m);
+        fetch(checkpoints + (from / k.checkpoint - 1) * stride + v * kMapWords<W>, m);
         carry[v] = m.h;
       }
     __syncthreads();
@@ -163,10 +163,10 @@ __device__ __forceinline__ void carry_in(const Cut& k, uint64_t* work, int64_t t
           const Map<W> m = parts[s * k.lanes + lane][v];
           carry[v] = fma_wide(m.a, carry[v], m.h);
         }
-    if (slot == k.slots - 1 && (tile + 1) % kCheckpoint == 0 && tile + 1 < k.tiles)
+    if (slot == k.slots - 1 && (tile + 1) % k.checkpoint == 0 && tile + 1 < k.tiles)
       for (int v = 0; v < V; ++v) {
         const Map<W> m = after(own[v], mine[v]);
-        publish(checkpoints + tile / kCheckpoint * stride + v * kMapWords<W>, Map<W>{0, fma_wide(m.a, carry[v], m.h)});
+        publish(checkpoints + tile / k.checkpoint * stride + v * kMapWords<W>, Map<W>{0, fma_wide(m.a, carry[v], m.h)});
       }
   }
   for (int v = 0; v < V; ++v) carry[v] = fma_wide(mine[v].a, carry[v], mine[v].h);
@@ -186,23 +186,51 @@ template <int V> struct Channels {
   }
 };
 
+// The gates of a lane's channels.  Of a shared gate one load serves the pack, unless a group ends within a pack of the wave;
+// where a step has one gate and steps are neighbours, a chunk's gates are loaded as one pack.
 template <typename G, GateKind K, int V> struct GateRow {
   const G* base = nullptr;
   int64_t step = 0;
   int64_t group[V];
+  bool split = false;
   __device__ __forceinline__ GateRow(int64_t gate, int64_t b, int64_t gate_b, int64_t gate_t, int64_t d, int64_t per) {
     if constexpr (K != kNoGate) {
       base = (const G*)gate + b * gate_b + (K == kOwnGate ? d : 0);
       step = gate_t;
       for (int v = 0; v < V; ++v) group[v] = K == kSharedGate ? (d + v) / per : v;
+      if constexpr (K == kSharedGate && V > 1) split = __any(group[0] != group[V - 1]);
     }
   }
   __device__ __forceinline__ Pack<G, V> load(int64_t t) const {
     Pack<G, V> g;
-    if constexpr (K == kOwnGate) g = load_pack<G, V>(base + t * step);
-    else if constexpr (K == kSharedGate)
+    if constexpr (K == kOwnGate) {
+      g = load_pack<G, V>(base + t * step);
+    } else if constexpr (K == kSharedGate) {
       for (int v = 0; v < V; ++v) g.v[v] = base[t * step + group[v]];
+    }
     return g;
+  }
+  // steps t, t + Way, ..., all of them there
+  template <int Way, int L> __device__ __forceinline__ void load_steps(int64_t t, Pack<G, V> (&gs)[L]) const {
+    if constexpr (K == kSharedGate && L > 1) {
+      if (step == 1 && !split) {
+        const Pack<G, L> line = load_pack<G, L>(base + group[0] + (Way > 0 ? t : t - (L - 1)));
+#pragma unroll
+        for (int j = 0; j < L; ++j)
+          for (int v = 0; v < V; ++v) gs[j].v[v] = line.v[Way > 0 ? j : L - 1 - j];
+        return;
+      }
+    }
+    if (K == kSharedGate && V > 1 && !split) {
+#pragma unroll
+      for (int j = 0; j < L; ++j) gs[j].v[0] = base[(t + Way * j) * step + group[0]];
+#pragma unroll
+      for (int j = 0; j < L; ++j)
+        for (int v = 1; v < V; ++v) gs[j].v[v] = gs[j].v[0];
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < L; ++j) gs[j] = load(t + Way * j);
   }
 };
 
@@ -210,6 +238,20 @@ template <typename T, int V> __device__ __forceinline__ Pack<T, V> constant(floa
   Pack<T, V> p;
   for (int v = 0; v < V; ++v) p.v[v] = (T)x;
   return p;
+}
+
+// Keeps the compiler from carrying the wide values of the first walk over a chunk into the second: the packs as loaded take
+// half the registers or less.
+template <typename T, int V, int L> __device__ __forceinline__ void as_loaded(Pack<T, V> (&p)[L]) {
+  if constexpr (sizeof(T) * V % 4 == 0) {
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+      uint32_t w[sizeof(T) * V / 4];
+      __builtin_memcpy(w, &p[j], sizeof w);
+      for (uint32_t& x : w) asm volatile("" : "+v"(x));
+      __builtin_memcpy(&p[j], w, sizeof w);
+    }
+  }
 }
 
 __device__ __forceinline__ int64_t length_of(int64_t lengths, int64_t b, int64_t steps) {
@@ -234,10 +276,8 @@ __global__ __launch_bounds__(kLanes* kMaxSlots) void scan_kernel(ScanArgs a, Cut
   Pack<G, V> gs[L];
   if (__all(t0 + L <= len)) {
 #pragma unroll
-    for (int j = 0; j < L; ++j) {
-      xs[j] = load_pack<T, V>(x + (t0 + j) * a.x_t);
-      gs[j] = gate.load(t0 + j);
-    }
+    for (int j = 0; j < L; ++j) xs[j] = load_pack<T, V>(x + (t0 + j) * a.x_t);
+    gate.template load_steps<1>(t0, gs);
   } else {
 #pragma unroll
     for (int j = 0; j < L; ++j) {
@@ -270,6 +310,8 @@ __global__ __launch_bounds__(kLanes* kMaxSlots) void scan_kernel(ScanArgs a, Cut
         }
       }
     for (int v = 0; v < V; ++v) own[v].a = kept(own[v].a, least[v] == 0);
+    as_loaded(xs);
+    if constexpr (K != kNoGate) as_loaded(gs);
     carry_in<W, V>(k, (uint64_t*)a.work, tile, row, lane, slot, own, first, h);
   } else {
     for (int v = 0; v < V; ++v) h[v] = first[v];
@@ -346,12 +388,12 @@ __global__ __launch_bounds__(kLanes* kMaxSlots) void scan_grad_kernel(ScanGradAr
 #pragma unroll
     for (int j = 0; j < L; ++j) {
       gs[j] = load_pack<T, V>(dh + (t0 - j) * a.g_t);
-      as[j] = gate.load(t0 - j);
       if constexpr (K != kNoGate) {
         before[j] = load_pack<T, V>(hs + (t0 - j - 1) * a.h_t);
         if (a.mix) xs[j] = load_pack<T, V>(x + (t0 - j) * a.x_t);
       }
     }
+    gate.template load_steps<-1>(t0, as);
   } else {
 #pragma unroll
     for (int j = 0; j < L; ++j) {
@@ -386,6 +428,8 @@ __global__ __launch_bounds__(kLanes* kMaxSlots) void scan_grad_kernel(ScanGradAr
         }
       }
     for (int v = 0; v < V; ++v) own[v].a = kept(own[v].a, least[v] == 0);
+    as_loaded(gs);
+    if constexpr (K != kNoGate) as_loaded(as);
     carry_in<W, V>(k, work, tile, row, lane, slot, own, first, e);
   } else {
     for (int v = 0; v < V; ++v) e[v] = first[v];
@@ -452,7 +496,7 @@ __global__ __launch_bounds__(kLanes* kMaxSlots) void scan_grad_kernel(ScanGradAr
 }
 
 // grad_gate[q][t][g] = sum of the slopes of the sequences and channels that share the gate, in a fixed order: `team` lanes
-// (a wave, or the workgroup where more than kWaveTerms share a gate) side by side, then a tree.
+// (one where a group is one channel, a wave, or the workgroup where more than kWaveTerms share a gate) side by side, then a tree.
 constexpr int64_t kWaveTerms = 2048;
 
 template <typename W, typename G, int kTeam>
@@ -472,7 +516,8 @@ __global__ __launch_bounds__(kThreads) void gate_sum_kernel(const W* __restrict_
         for (int64_t d = lane; d < per; d += kTeam) sum += row[d];
       }
     }
-    for (int s = 32; s; s >>= 1) sum += __shfl_xor(sum, s);
+    if constexpr (kTeam > 1)
+      for (int s = 32; s; s >>= 1) sum += __shfl_xor(sum, s);
     if constexpr (kTeam > 64) {
       if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = sum;
       __syncthreads();
@@ -498,6 +543,10 @@ Cut cut_steps(int64_t batch, int64_t steps, int64_t width, int v, int per_lane, 
   k.tiles = (chunks + k.slots - 1) / k.slots;
   if (k.tiles == 1 && k.slots == 1) k.lanes = k.packs >= kThreads ? kThreads : k.lanes;
   k.pack_rows = (k.packs + k.lanes - 1) / k.lanes;
+  // Close checkpoints leave little to fold, far ones make a short chain of tiles that wait for one another; with many rows
+  // of tiles the chain has time (8 x 4096 x 2560 bf16, 160 rows: 149 us with 8, 157 us with 32; 1 x 65537 x 1024, 8 rows: 123 us
+  // with 8, 116 us with 16).
+  k.checkpoint = k.pack_rows >= 32 ? 8 : k.pack_rows >= 8 ? 16 : 32;
   if (k.tiles * k.pack_rows > 2147483647LL) throw std::runtime_error("gated_scan: the tensor is too large");
   return k;
 }
@@ -641,7 +690,8 @@ void gated_scan_grad(const ScanGradArgs& a) {
           hipLaunchKernelGGL(kernel, dim3((unsigned)std::min<int64_t>((sums * team + kThreads - 1) / kThreads, 1 << 20)), dim3(kThreads), 0, s,
                              (const W*)slopes, (G*)a.grad_gate, rows, a.steps, across, a.groups, a.gate_batch);
         };
-        if (terms <= kWaveTerms) run(gate_sum_kernel<W, G, 64>, 64);
+        if (across == a.groups) run(gate_sum_kernel<W, G, 1>, 1);
+        else if (terms <= kWaveTerms) run(gate_sum_kernel<W, G, 64>, 64);
         else run(gate_sum_kernel<W, G, kThreads>, kThreads);
         LGA_HIP_CHECK(hipGetLastError());
       }

@@ -20,7 +20,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kLanes = 64;          // channel packs of a tile
-constexpr int kScanSteps = 16, kGradSteps = 8;      // steps a lane holds
+constexpr int kScanSteps = 16;      // steps a lane holds
 constexpr int kMaxSlots = 16;       // chunks of a tile
 constexpr uint64_t kEmpty = ~0ull;  // a word nobody has written yet: a NaN that publish() never stores
 
@@ -556,6 +556,11 @@ Cut cut_steps(int64_t batch, int64_t steps, int64_t width, int v, int per_lane, 
 // Up to kMaxSlots chunks are one tile, which needs neither a workspace nor tickets.
 int scan_slots(const ScanArgs& a) { return a.steps > 64 * 8 * kScanSteps || a.steps <= kMaxSlots * kScanSteps ? kMaxSlots : 8; }
 
+// Backwards: values of 16 bits leave room for 16 steps a lane in 128 registers (8 x 4096 x 2560 bf16: 277 us with 16 steps and 8
+// chunks, 299 us with 8 and 16); of fp32 (1 x 423 x 26734: 69 against 109 us) and fp64 they do not.
+constexpr int grad_steps(int64_t type) { return type == kBf16 || type == kF16 ? 16 : 8; }
+constexpr int grad_slots(int64_t type) { return type == kBf16 || type == kF16 ? 8 : kMaxSlots; }
+
 template <typename A> void check_args(const A& a) {
   if (a.batch < 0 || a.steps < 0 || a.width < 0) throw std::runtime_error("gated_scan: a negative size");
   if (a.steps > 2147483647LL) throw std::runtime_error("gated_scan: the tensor is too large");
@@ -600,9 +605,9 @@ template <typename W> void clear_work(const Cut& k, int v, uint64_t* work, hipSt
 
 bool sums_gates(const ScanGradArgs& a) { return a.gate && (a.groups != a.width || a.gate_batch != a.batch); }
 
-// Teams of at least 8 lanes within a gate group (or, with one gate a step for everything, over all lanes) sum up in the
+// Teams of at least 8 lanes, and as many as a lane holds steps, within a gate group (or, with one gate a step for everything, over all lanes) sum up in the
 // backward kernel; a group like 103 channels has none, and its slopes go through memory value by value.
-GateSums gate_sums(const ScanGradArgs& a, const Cut& k, int v) {
+GateSums gate_sums(const ScanGradArgs& a, const Cut& k, int v, int per_lane) {
   GateSums g;
   if (!sums_gates(a) || a.groups == a.width) return g;
   const int64_t per = a.width / a.groups;
@@ -618,7 +623,7 @@ GateSums gate_sums(const ScanGradArgs& a, const Cut& k, int v) {
     g.teams = a.width / v / team;
     g.done = per / v == team && a.gate_batch == a.batch;
   }
-  g.team = team >= 8 ? team : 0;
+  g.team = team >= std::max(8, per_lane) ? team : 0;
   if (!g.team) return GateSums{};
   if (a.groups == 1 && a.gate_batch == 1 && g.teams == 1) g.done = 1;
   return g;
@@ -659,8 +664,9 @@ void gated_scan(const ScanArgs& a) {
 int64_t scan_grad_workspace(const ScanGradArgs& a) {
   check_args(a);
   const int v = two_wide(a) ? 2 : 1;
-  const Cut k = cut_steps(a.batch, a.steps, a.width, v, a.steps <= 1 ? 1 : kGradSteps, kMaxSlots);
-  return 8 * (a.type == kF64 ? work_words<double>(k, v) : work_words<float>(k, v)) + slope_values(a, gate_sums(a, k, v)) * (a.type == kF64 ? 8 : 4);
+  const int steps = a.steps <= 1 ? 1 : grad_steps(a.type);
+  const Cut k = cut_steps(a.batch, a.steps, a.width, v, steps, grad_slots(a.type));
+  return 8 * (a.type == kF64 ? work_words<double>(k, v) : work_words<float>(k, v)) + slope_values(a, gate_sums(a, k, v, steps)) * (a.type == kF64 ? 8 : 4);
 }
 
 void gated_scan_grad(const ScanGradArgs& a) {
@@ -672,12 +678,12 @@ void gated_scan_grad(const ScanGradArgs& a) {
     typedef decltype(gg) G;
     typedef Wide<T> W;
     const hipStream_t s = (hipStream_t)a.stream;
-    by_shape<sizeof(T) < 8, kGradSteps>(a, [&](auto kind, auto v, auto l) {
+    by_shape<sizeof(T) < 8, sizeof(T) == 2 ? grad_steps(kBf16) : grad_steps(kF32)>(a, [&](auto kind, auto v, auto l) {
       constexpr int V = decltype(v)::value, L = decltype(l)::value;
-      const Cut k = cut_steps(a.batch, a.steps, a.width, V, L, kMaxSlots);
+      const Cut k = cut_steps(a.batch, a.steps, a.width, V, L, grad_slots(a.type));
       uint64_t* work = (uint64_t*)a.work;
       clear_work<W>(k, V, work, s);
-      const GateSums g = gate_sums(a, k, V);
+      const GateSums g = gate_sums(a, k, V, L);
       const int64_t slopes = slope_values(a, g) ? (int64_t)(work + work_words<W>(k, V)) : 0;
       hipLaunchKernelGGL((scan_grad_kernel<T, G, (GateKind)decltype(kind)::value, V, L>), dim3((unsigned)(k.tiles * k.pack_rows)), dim3(k.lanes * k.slots),
                          fold_bytes<W>(k, V), s, a, k, work, slopes, g);

@@ -649,8 +649,9 @@ template <typename T> void run_lookup(const LookupArgs& a) {
   LGA_HIP_CHECK(hipGetLastError());
 }
 
-// Up to this many tokens every workgroup looks through all ids for its own rows; above, they are sorted.
-constexpr int64_t kOwnedTokens = 512;
+// Up to this many tokens every workgroup looks through all ids for its own rows (256 tokens, 8192 rows of 512 fp32 values: 11 us,
+// sorted 25 us); above, or for tables of more rows, they are sorted.
+constexpr int64_t kOwnedTokens = 512, kOwnedTable = 131072;
 constexpr int64_t kPrivateLds = 160 * 1024;      // of a wave, for the sums of a column
 
 struct GradPlan {
@@ -696,7 +697,7 @@ GradPlan plan_grad(const LookupGradArgs& a) {
   return p;
 }
 
-bool owned(const LookupGradArgs& a) { return a.n0 * a.n1 <= kOwnedTokens; }
+bool owned(const LookupGradArgs& a) { return a.n0 * a.n1 <= kOwnedTokens && a.rows <= kOwnedTable; }
 
 // Few rows and many tokens: sums of a column of the table in a wave's share of LDS.
 struct PrivatePlan {

@@ -19,7 +19,9 @@ struct Pass {
   const uint32_t* keys_in;      // null: first pass, keys come from the grid
   const void* payload_in;
   int64_t v0, v1;               // first pass: payload (i, j) is at i * v0 + j * v1; payload_in null: the token's number
-  uint8_t* named;               // cleared by the first count, set by the last scatter (null in the other passes)
+  uint8_t* named;               // set by the last scatter (null in the passes before)
+  uint4* clear;                 // its words, where the first kernel of the sort clears them (else null)
+  int64_t clear_words;
   int shift, bits;
   bool few;                     // few tiles: no kernel of its own for the offsets
 };
@@ -52,8 +54,8 @@ __global__ __launch_bounds__(kThreads) void sort_count_kernel(Pass p, uint32_t* 
   const int64_t b = blockIdx.x;
   for (int d = threadIdx.x; d < kBins; d += kThreads) bin[d] = 0;
   __syncthreads();
-  if (!p.keys_in)
-    for (int64_t r = b * kThreads + threadIdx.x; r < p.grid.rows; r += (int64_t)gridDim.x * kThreads) p.named[r] = 0;
+  if (!p.keys_in && p.clear)
+    for (int64_t r = b * kThreads + threadIdx.x; r < p.clear_words; r += (int64_t)gridDim.x * kThreads) p.clear[r] = make_uint4(0, 0, 0, 0);
   const uint32_t mask = (1u << p.bits) - 1;
 #pragma unroll 4
   for (int k = 0; k < kItems; ++k) {
@@ -70,6 +72,10 @@ __global__ __launch_bounds__(kThreads) void sort_count_kernel(Pass p, uint32_t* 
   }
   __syncthreads();
   for (int d = threadIdx.x; d < (1 << p.bits); d += kThreads) counts[(int64_t)d * p.tiles.blocks + b] = bin[d];
+}
+
+__global__ __launch_bounds__(kThreads) void clear_kernel(uint4* __restrict__ p, int64_t words) {
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < words; i += (int64_t)gridDim.x * kThreads) p[i] = make_uint4(0, 0, 0, 0);
 }
 
 // Counts of one digit over the tiles -> where each tile's run of that digit begins among all of that digit; their sum.
@@ -232,7 +238,8 @@ __global__ __launch_bounds__(kOneThreads) void sort_one_kernel(Pass p, int passe
   const uint32_t tokens = (uint32_t)(p.grid.n0 * p.grid.n1);
   uint32_t key[kOneItems], rank[kOneItems];
   P pay[kOneItems];
-  for (int64_t r = t; r < p.grid.rows; r += kOneThreads) p.named[r] = 0;
+  if (p.clear)
+    for (int64_t r = t; r < p.clear_words; r += kOneThreads) p.clear[r] = make_uint4(0, 0, 0, 0);
 #pragma unroll
   for (int k = 0; k < kOneItems; ++k) {
     const uint32_t q = wave * (kSortTile / kOneWaves) + k * 64 + lane;
@@ -380,7 +387,13 @@ SortedTokens token_sort(const TokenGrid& g, const void* values, int64_t v0, int6
   const dim3 grid((unsigned)tiles.blocks), block(kThreads);
   uint32_t *counts = (uint32_t*)(w + l.counts), *totals = (uint32_t*)(w + l.totals);
   uint8_t* named = (uint8_t*)(w + l.named);
-  Pass p{g, tiles, nullptr, values, v0, v1, named, 0, each, small};
+  // the named rows: cleared on the way where that is a few words a lane, else by a kernel of its own
+  const int64_t words = (g.rows + 15) / 16, lanes = one_tile(g) ? kOneThreads : tiles.blocks * kThreads;
+  Pass p{g, tiles, nullptr, values, v0, v1, named, words <= 4 * lanes ? (uint4*)named : nullptr, words, 0, each, small};
+  if (!p.clear) {
+    hipLaunchKernelGGL(clear_kernel, dim3((unsigned)std::min<int64_t>((words + kThreads - 1) / kThreads, 4096)), block, 0, s, (uint4*)named, words);
+    LGA_HIP_CHECK(hipGetLastError());
+  }
   if (one_tile(g)) {
     uint32_t* keys = (uint32_t*)(w + l.keys[0]);
     void* pay = w + l.payload[0];

@@ -45,13 +45,13 @@ def embedding(table, ids, scale: float = 1.0):
     rows, width = table.shape
     if width > 1 and table.stride(1) != 1 or table.stride(0) < 0:
         table = table.contiguous()
-    view = two_dims(ids.shape, ids.stride())
-    if view is None:
-        ids = ids.contiguous()
-        view = two_dims(ids.shape, ids.stride())
-    (n0, n1), ((s0, s1),) = view
     out = torch.empty((*ids.shape, width), dtype=table.dtype, device=table.device)
     if out.numel():
+        view = two_dims(ids.shape, ids.stride())
+        if view is None:
+            ids = ids.contiguous()
+            view = two_dims(ids.shape, ids.stride())
+        (n0, n1), ((s0, s1),) = view
         run(lib.lga_hip_embedding,
             lambda work: _LOOKUP.pack(table.data_ptr(), ids.data_ptr(), out.data_ptr(), stream_of(device), device, rows, width, table.stride(0),
                                       n0, n1, s0, s1, code, wide_ids, float(scale)), table.device)
@@ -83,6 +83,8 @@ def embedding_grad(grad, ids, num_rows: int, scale: float = 1.0, dtype=None):
     width = grad.shape[-1]
     if width > 1 and grad.stride(-1) != 1:
         grad = grad.contiguous()
+    if not ids.numel():
+        ids, grad = ids.reshape(0), grad.reshape(0, width)
     view = two_dims(ids.shape, ids.stride(), grad.stride()[:-1])
     if view is None:
         ids, grad = ids.contiguous(), grad.contiguous()

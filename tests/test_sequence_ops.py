@@ -222,6 +222,35 @@ def test_lookup_gradient_is_the_sum_over_the_tokens_of_a_row(shape, rows, width,
 
 
 @gpu
+@pytest.mark.parametrize("tokens,rows,width,name", [((40, 20000), 32000, 1, "f32"), ((37, 9001), 18100, 1, "f64"), ((70001,), 4001, 3, "f32"),
+                                                    ((300, 1700), 9300, 7, "f64"), ((100, 31), 150, 2, "bf16"), ((3100, 100), 400, 1, "f16")])
+def test_lookup_gradient_of_few_rows(tokens, rows, width, name):
+    """Sums of a column in LDS: tables up to a CU's LDS, lanes that share rows, lines shorter than a step."""
+    g = rng(rows)
+    grad = normal(g, (*tokens, width), TYPES[name])
+    for kind, ids in (("uniform", make_ids(g, tokens, rows, torch.int32, 0.05)), ("few", make_ids(g, tokens, rows, torch.int64, 0.0, "few"))):
+        for view, like in ((ids, grad), (ids.transpose(0, -1), grad.transpose(0, -2))):
+            got = ops.embedding_grad(_on_gpu(like), _on_gpu(view), rows, scale=0.5, dtype=torch.float32 if name in ("bf16", "f16") else None)
+            want, mag, n = lookup_grad_oracle(like, view, rows, 0.5)
+            within(got, want, (n + 4).reshape(-1, 1) * u(wide(TYPES[name])) * mag, got.dtype)
+
+
+@gpu
+@pytest.mark.parametrize("tokens,rows,width", [(300, 3000001, 1), (3000, 2000003, 3), (20000, 700001, 40), (5, 400000, 17), (600, 20000000, 1)])
+def test_lookup_gradient_of_large_tables(tokens, rows, width):
+    g = rng(tokens)
+    grad, ids = normal(g, (tokens, width), torch.float32), make_ids(g, (tokens,), rows, torch.int64)
+    got = ops.embedding_grad(grad.cuda(), ids.cuda(), rows)
+    named = torch.unique(ids[(ids >= 0) & (ids < rows)])
+    at = torch.searchsorted(named, ids.clamp(0, rows - 1))
+    inner = torch.where((ids >= 0) & (ids < rows), at, torch.full_like(at, -1))
+    want, mag, n = lookup_grad_oracle(grad, inner, len(named), 1.0)
+    within(got[named.cuda()], want, (n + 4).reshape(-1, 1) * u(torch.float32) * mag, torch.float32)
+    got[named.cuda()] = 0
+    assert not got.any()
+
+
+@gpu
 def test_lookup_gradient_reads_expanded_and_strided_gradients_in_place():
     g = rng(11)
     ids = make_ids(g, (500, 60), 400, torch.int32)
@@ -297,7 +326,17 @@ SCANS = [(1, 1, 1, "f32", "f32", 1, 1, False, False, False),
          (2, 4097, 66, "f16", "f16", 66, 2, False, False, True),
          (1, 20000, 40, "f32", "f32", 40, 1, True, True, False),
          (65, 40, 24, "bf16", "bf16", 24, 1, False, True, True),
-         (3, 700, 128, "f64", "f64", 4, 3, True, True, True)]
+         (3, 700, 128, "f64", "f64", 4, 3, True, True, True),
+         # gates shared by whole teams of lanes, by all channels of an odd width, by the batch
+         (3, 70, 512, "bf16", "f32", 8, 3, False, True, True),
+         (2, 90, 192, "f32", "f32", 2, 1, True, True, False),
+         (4, 33, 1536, "f16", "f16", 16, 4, True, False, True),
+         (1, 40, 1021, "f32", "f32", 1, 1, True, True, True),
+         (6, 300, 64, "f16", "f16", 1, 1, False, True, True),
+         (5, 260, 33, "bf16", "bf16", 1, 1, True, False, False),
+         (6, 140, 35, "f16", "f32", 35, 1, True, True, True),
+         (2, 1, 256, "bf16", "f32", 4, 2, True, True, False),
+         (7, 1, 1030, "f32", "f32", 1, 7, False, True, True)]
 
 
 @gpu
@@ -458,7 +497,13 @@ def _everything(seed, t=300, d=96):
 
 
 def _chain(ids, table, gate, dh):
-    """Lookup, recurrence and both gradients, as a training step runs them."""
+    """Lookup, recurrence and both gradients, as a training step runs them, and the gradient of a forest's leaves."""
+    leaves = (ids.reshape(-1, 1) * 31 + torch.arange(200, device="cuda")) % 20001
+    grad_leaves = ops.embedding_grad(gate.reshape(-1)[:len(leaves)].reshape(-1, 1, 1).expand(-1, 200, 1), leaves, 20001)
+    return (*_step(ids, table, gate, dh), grad_leaves)
+
+
+def _step(ids, table, gate, dh):
     x = ops.embedding(table, ids, scale=2.0)
     states, last = ops.gated_scan(x, gate, mix=True)
     grad_x, grad_state, grad_gate = ops.gated_scan_grad(dh, states, gate, x=x, mix=True)
@@ -470,7 +515,7 @@ def _chain(ids, table, gate, dh):
 @pytest.mark.parametrize("t,d", [(1, 64), (60, 96), (300, 96), (2500, 130)])
 def test_a_training_step_of_all_four_follows_the_formulas(t, d):
     ids, table, gate, dh = _everything(t, t, d)
-    x, states, last, grad_x, grad_state, grad_gate, grad_table = _chain(ids, table, gate, dh)
+    x, states, last, grad_x, grad_state, grad_gate, grad_table = _step(ids, table, gate, dh)
     want = lookup_oracle(table, ids, 2.0)
     assert torch.equal(x.double().cpu(), want)
     want, want_last, bound, bound_last = scan_oracle(x, gate, None, True, None)
@@ -552,6 +597,10 @@ def test_empty_tensors():
     state = torch.full((2, 5), 3.0, device=dev)
     states, last = ops.gated_scan(torch.ones((2, 0, 5), device=dev), torch.ones((2, 0, 5), device=dev), state)
     assert states.shape == (2, 0, 5) and torch.equal(last, state)
+    for shape in ((2, 0, 3, 0), (0, 2, 3), (2, 3, 0), (0,)):
+        none = torch.zeros(shape, dtype=torch.int32, device=dev)
+        assert ops.embedding(torch.ones((3, 2), device=dev), none).shape == (*shape, 2)
+        assert not ops.embedding_grad(torch.ones((*shape, 2), device=dev), none, 4).any()
     gx, gs, gg = ops.gated_scan_grad(states, states, torch.ones((2, 0, 5), device=dev), state, grad_last=2 * state)
     assert gx.shape == (2, 0, 5) and torch.equal(gs, 2 * state) and gg.shape == (2, 0, 5)
     for shape in ((0, 7, 5), (2, 7, 0)):

@@ -728,7 +728,10 @@ PrivatePlan plan_private(const LookupGradArgs& a) {
   p.whole = !p.items_along0 && a.width == 1 && p.g1 == 1;
   p.lds = (int)((lds + 15) / 16 * 16);
   const int64_t fit = 256 * std::min<int64_t>(8, std::max<int64_t>(1, 163840 / p.lds));
-  p.waves = (int)std::max<int64_t>(1, std::min({fit / a.width, p.steps, tokens / std::max<int64_t>(1024, a.rows)}));
+  // as many tokens a wave as the table has rows, so that the waves' sums are no more than the tokens; fewer where that
+  // would leave CUs idle (557 k tokens of 3 values, 23478 rows: 69 waves 88 us, 255 waves MID us)
+  const int64_t chunks = std::max(tokens / std::max<int64_t>(1024, a.rows), std::min(256 / a.width, tokens / std::max<int64_t>(1024, a.rows / 4)));
+  p.waves = (int)std::max<int64_t>(1, std::min({fit / a.width, p.steps, chunks}));
   return p;
 }
 

@@ -25,7 +25,7 @@ struct Pass {
   int shift, bits;
   bool few;                     // few tiles: no kernel of its own for the offsets
 };
-constexpr int64_t kFewTiles = 128;
+constexpr int64_t kFewTiles = 128, kSmallTiles = 4096;
 
 __device__ __forceinline__ uint32_t grid_key(const TokenGrid& g, int64_t i, int64_t j) {
   if (i >= g.n0 || j >= g.n1) return (uint32_t)g.rows;
@@ -359,7 +359,7 @@ TokenTiles token_tiles(const TokenGrid& g, int bits) {
   return t;
 }
 
-// Small tiles where tiles of 4096 would leave most of the chip idle.
+// Small tiles where tiles of 4096 would leave most of the chip idle (500 k tokens in 127500 rows: 122 of them).
 TokenTiles sort_tiles(const TokenGrid& g) {
   if (one_tile(g)) {
     TokenTiles t;
@@ -368,9 +368,8 @@ TokenTiles sort_tiles(const TokenGrid& g) {
     t.count = kSortTile;
     return t;
   }
-  const TokenTiles small = token_tiles(g, 10);
-  if (small.blocks > kFewTiles) return token_tiles(g);
-  TokenTiles t = small;
+  TokenTiles t = token_tiles(g, 10);
+  if (t.blocks > kSmallTiles) return token_tiles(g);
   t.blocks = (t.blocks + 3) / 4 * 4;      // whole multiples of kSortTile
   t.count = t.blocks << 10;
   return t;
@@ -389,7 +388,7 @@ SortedTokens token_sort(const TokenGrid& g, const void* values, int64_t v0, int6
   uint8_t* named = (uint8_t*)(w + l.named);
   // the named rows: cleared on the way where that is a few words a lane, else by a kernel of its own
   const int64_t words = (g.rows + 15) / 16, lanes = one_tile(g) ? kOneThreads : tiles.blocks * kThreads;
-  Pass p{g, tiles, nullptr, values, v0, v1, named, words <= 4 * lanes ? (uint4*)named : nullptr, words, 0, each, small};
+  Pass p{g, tiles, nullptr, values, v0, v1, named, words <= 4 * lanes ? (uint4*)named : nullptr, words, 0, each, tiles.blocks <= kFewTiles && small};
   if (!p.clear) {
     hipLaunchKernelGGL(clear_kernel, dim3((unsigned)std::min<int64_t>((words + kThreads - 1) / kThreads, 4096)), block, 0, s, (uint4*)named, words);
     LGA_HIP_CHECK(hipGetLastError());

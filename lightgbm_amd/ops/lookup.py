@@ -43,7 +43,7 @@ def embedding(table, ids, scale: float = 1.0):
     device = need_device("embedding", table, ids)
     lib = core()
     rows, width = table.shape
-    if width > 1 and table.stride(1) != 1 or table.stride(0) < 0:
+    if width > 1 and table.stride(1) != 1:
         table = table.contiguous()
     out = torch.empty((*ids.shape, width), dtype=table.dtype, device=table.device)
     if out.numel():

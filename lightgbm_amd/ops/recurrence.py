@@ -25,7 +25,7 @@ def _wide(t):
 
 def _rows(t):
     """``t`` with a sequence step's channels next to each other."""
-    return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 def _check(op: str, x, code: int, gate, lengths, ends):
@@ -67,7 +67,8 @@ def _gate_steps(gate, batch: int):
     """Elements between the gates of neighbouring sequences and steps."""
     if gate is None:
         return 0, 0
-    return (gate.stride(0) if gate.shape[0] == batch else 0), gate.stride(1)
+    gate_b, gate_t, _ = gate.stride()
+    return (gate_b if gate.shape[0] == batch else 0), gate_t
 
 
 def gated_scan(x, gate=None, state=None, *, mix: bool = False, lengths=None):
@@ -78,7 +79,8 @@ def gated_scan(x, gate=None, state=None, *, mix: bool = False, lengths=None):
     the state before the first step (zeros if not given).  ``lengths``: int32 [batch]; behind a sequence's length (clamped to
     0 .. steps) the states are zero, ``last`` is the state after its last step, and what stands in ``x`` and ``gate`` there
     is not used.  States are carried in float32 (float64 for fp64), which is also the type of ``state`` and ``last``: feeding
-    ``last`` back in continues a sequence, step by step or in pieces.
+    ``last`` back in continues a sequence, step by step or in pieces.  Gates are meant to lie in -1 .. 1: outside, the product
+    of a long run of them may overflow, and then so do states that single steps would have kept finite.
     """
     need_tensor("gated_scan", "x", x)
     code = need_type("gated_scan", "x", x)
@@ -91,14 +93,16 @@ def gated_scan(x, gate=None, state=None, *, mix: bool = False, lengths=None):
     lib = core()
     x, state, lengths = _rows(x), _contiguous(state), _contiguous(lengths)
     b, t, d = x.shape
-    states = torch.empty((b, t, d), dtype=x.dtype, device=x.device)
-    last = torch.empty((b, d), dtype=_wide(x), device=x.device)
-    if last.numel():
+    where = x.device
+    states = torch.empty((b, t, d), dtype=x.dtype, device=where)
+    last = torch.empty((b, d), dtype=_wide(x), device=where)
+    if b and d:
         gate_b, gate_t = _gate_steps(gate, b)
+        x_b, x_t, _ = x.stride()
+        stream = stream_of(device)
         run(lib.lga_hip_gated_scan,
             lambda work: _SCAN.pack(x.data_ptr(), _address(gate) if t else 0, _address(state), _address(lengths), states.data_ptr(), last.data_ptr(),
-                                    work, stream_of(device), device, b, t, d, x.stride(0), x.stride(1), gate_b, gate_t, groups, code, gate_code,
-                                    bool(mix)), x.device)
+                                    work, stream, device, b, t, d, x_b, x_t, gate_b, gate_t, groups, code, gate_code, bool(mix)), where)
     return states, last
 
 
@@ -129,18 +133,20 @@ def gated_scan_grad(grad_states, states, gate=None, state=None, *, x=None, grad_
     grad_states, states, x = _rows(grad_states), _rows(states), _rows(x) if mix else None
     state, grad_last, lengths = _contiguous(state), _contiguous(grad_last), _contiguous(lengths)
     b, t, d = states.shape
-    grad_x = torch.empty((b, t, d), dtype=states.dtype, device=states.device)
-    grad_state = torch.empty((b, d), dtype=_wide(states), device=states.device)
-    grad_gate = None if gate is None else torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
-    if grad_state.numel():
+    where = states.device
+    grad_x = torch.empty((b, t, d), dtype=states.dtype, device=where)
+    grad_state = torch.empty((b, d), dtype=_wide(states), device=where)
+    grad_gate = None if gate is None else torch.empty(gate.shape, dtype=gate.dtype, device=where)
+    if b and d:
         gate_b, gate_t = _gate_steps(gate, b)
-        x_b, x_t = (x.stride(0), x.stride(1)) if mix else (0, 0)
+        (g_b, g_t, _), (h_b, h_t, _), (x_b, x_t, _) = grad_states.stride(), states.stride(), x.stride() if mix else (0, 0, 0)
+        stream = stream_of(device)
         gates = 0 if gate is None else gate.shape[0]
         run(lib.lga_hip_gated_scan_grad,
             lambda work: _SCAN_GRAD.pack(grad_states.data_ptr(), states.data_ptr(), _address(gate) if t else 0, _address(state), _address(x),
                                          _address(grad_last), _address(lengths), grad_x.data_ptr(), grad_state.data_ptr(), _address(grad_gate), work,
-                                         stream_of(device), device, b, t, d, grad_states.stride(0), grad_states.stride(1), states.stride(0),
-                                         states.stride(1), x_b, x_t, gate_b, gate_t, groups, gates, code, gate_code, bool(mix)), states.device)
+                                         stream, device, b, t, d, g_b, g_t, h_b, h_t, x_b, x_t, gate_b, gate_t, groups, gates, code, gate_code,
+                                         bool(mix)), where)
     elif grad_gate is not None:
         grad_gate.zero_()
     return grad_x, grad_state, grad_gate

@@ -503,7 +503,7 @@ constexpr int kNarrowItems = 8, kNarrowPiece = kThreads * kNarrowItems;
 
 // Rows of up to kNarrow values: a workgroup takes a piece, a lane 8 neighbouring tokens; a segmented scan over the lanes
 // carries a run's sum on.  kValues: the payload is the gradient itself (rows of one value).
-template <typename T, typename O, bool kValues>
+template <typename T, typename O, bool kValues, int C>
 __global__ __launch_bounds__(kThreads) void lookup_grad_narrow_kernel(Runs r, const T* __restrict__ grad, O* __restrict__ out, Wide<T>* __restrict__ head,
                                                                       Wide<T>* __restrict__ tail, int zero_blocks, Wide<T> scale) {
   typedef Wide<T> W;
@@ -513,7 +513,7 @@ __global__ __launch_bounds__(kThreads) void lookup_grad_narrow_kernel(Runs r, co
       for (int64_t c = 0; c < r.width; ++c) out[row * r.width + c] = (O)0.f;
     return;
   }
-  __shared__ W wave_sum[kThreads / 64];
+  __shared__ W wave_sum[kThreads / 64][C];
   __shared__ int wave_break[kThreads / 64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t piece = (int64_t)blockIdx.x - zero_blocks, begin = piece * kNarrowPiece, at = begin + threadIdx.x * kNarrowItems;
@@ -542,55 +542,65 @@ __global__ __launch_bounds__(kThreads) void lookup_grad_narrow_kernel(Runs r, co
       from[u] = grad + i * r.g0 + j * r.g1;
     }
   }
-  T next[kNarrowItems];               // of the next column
-  auto load = [&](int64_t c) {
+  // C columns at a time; the last ones may be some of those before once more, with the same sums
+  for (int64_t base = 0; base < r.width; base += C) {
+    const int64_t c0 = min(base, r.width - C);
+    Pack<T, C> x[kNarrowItems];
+    if constexpr (!kValues) {
 #pragma unroll
-    for (int u = 0; u < kNarrowItems; ++u) next[u] = kValues ? (T)0.f : from[u][c];
-  };
-  load(0);
-  for (int64_t c = 0; c < r.width; ++c) {
-    W v[kNarrowItems], open = 0;      // open: the sum since the last beginning
-#pragma unroll
-    for (int u = 0; u < kNarrowItems; ++u) {
-      if constexpr (kValues) v[u] = (W)values.v[u];
-      else v[u] = key[u + 1] < rows ? (W)next[u] : (W)0;
+      for (int u = 0; u < kNarrowItems; ++u) x[u] = load_pack<T, C>(from[u] + c0);
     }
-    if (c + 1 < r.width) load(c + 1);
-#pragma unroll
-    for (int u = 0; u < kNarrowItems; ++u) open = key[u] != key[u + 1] ? v[u] : open + v[u];
-    // inclusive segmented scan over the wave, then over the waves
-    W sum = open;
-    bool broken = breaks;
-    for (int d = 1; d < 64; d <<= 1) {
-      const W s = __shfl_up(sum, d);
-      const bool b = __shfl_up((int)broken, d);
-      if (lane >= d) {
-        if (!broken) sum = s + sum;
-        broken |= b;
-      }
-    }
-    if (lane == 63) wave_sum[wave] = sum, wave_break[wave] = broken;
-    W carry = __shfl_up(sum, 1);
-    const bool cut = __shfl_up((int)broken, 1);
-    __syncthreads();
-    W from_waves = 0;
-    for (int w = 0; w < wave; ++w) from_waves = wave_break[w] ? wave_sum[w] : from_waves + wave_sum[w];
-    if (lane == 0) carry = from_waves;
-    else if (!cut) carry = from_waves + carry;
-    auto close = [&](uint32_t row, W total) {
-      if (row >= rows) return;
-      if (row == before_piece) head[piece * r.width + c] = total;
-      else out[(int64_t)row * r.width + c] = (O)(total * scale);
+    auto value = [&](int u, int e) -> W {
+      if constexpr (kValues) return (W)values.v[u];
+      else return key[u + 1] < rows ? (W)x[u].v[e] : (W)0;
     };
+    W carry[C];
+    bool broken = breaks;
 #pragma unroll
-    for (int u = 0; u < kNarrowItems; ++u) {
-      if (key[u] != key[u + 1] && at + u > begin) close(key[u], carry);
-      carry = key[u] != key[u + 1] ? v[u] : carry + v[u];
+    for (int e = 0; e < C; ++e) {     // the sum since the lane's last beginning
+      carry[e] = 0;
+#pragma unroll
+      for (int u = 0; u < kNarrowItems; ++u) carry[e] = key[u] != key[u + 1] ? value(u, e) : carry[e] + value(u, e);
     }
-    if (threadIdx.x == kThreads - 1 && key[kNarrowItems] < rows) {
-      const uint32_t last = key[kNarrowItems];
-      if (last != behind) close(last, carry);
-      else (last == before_piece ? head : tail)[piece * r.width + c] = carry;
+    // inclusive segmented scan over the wave, then over the waves
+    for (int d = 1; d < 64; d <<= 1) {
+      const bool b = __shfl_up((int)broken, d);
+#pragma unroll
+      for (int e = 0; e < C; ++e) {
+        const W s = __shfl_up(carry[e], d);
+        if (lane >= d && !broken) carry[e] = s + carry[e];
+      }
+      if (lane >= d) broken |= b;
+    }
+    if (lane == 63) {
+      for (int e = 0; e < C; ++e) wave_sum[wave][e] = carry[e];
+      wave_break[wave] = broken;
+    }
+    const bool cut = __shfl_up((int)broken, 1);
+#pragma unroll
+    for (int e = 0; e < C; ++e) carry[e] = __shfl_up(carry[e], 1);
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < C; ++e) {
+      const int64_t c = c0 + e;
+      W from_waves = 0;
+      for (int w = 0; w < wave; ++w) from_waves = wave_break[w] ? wave_sum[w][e] : from_waves + wave_sum[w][e];
+      W sum = lane == 0 ? from_waves : cut ? carry[e] : from_waves + carry[e];
+      auto close = [&](uint32_t row, W total) {
+        if (row >= rows) return;
+        if (row == before_piece) head[piece * r.width + c] = total;
+        else out[(int64_t)row * r.width + c] = (O)(total * scale);
+      };
+#pragma unroll
+      for (int u = 0; u < kNarrowItems; ++u) {
+        if (key[u] != key[u + 1] && at + u > begin) close(key[u], sum);
+        sum = key[u] != key[u + 1] ? value(u, e) : sum + value(u, e);
+      }
+      if (threadIdx.x == kThreads - 1 && key[kNarrowItems] < rows) {
+        const uint32_t last = key[kNarrowItems];
+        if (last != behind) close(last, sum);
+        else (last == before_piece ? head : tail)[piece * r.width + c] = sum;
+      }
     }
     __syncthreads();
   }
@@ -803,12 +813,18 @@ template <typename T, typename O> void run_lookup_grad(const LookupGradArgs& a) 
   if (a.width <= kNarrow) {
     const int zero_blocks = (int)((a.rows + kThreads - 1) / kThreads);
     const dim3 grid((unsigned)(zero_blocks + p.pieces));
+    auto run = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, r, (const T*)a.grad, (O*)a.out, head, tail, zero_blocks, (W)a.scale);
+    };
     if constexpr (sizeof(T) >= 4) {
-      if (p.values)
-        hipLaunchKernelGGL((lookup_grad_narrow_kernel<T, O, true>), grid, dim3(kThreads), 0, s, r, (const T*)a.grad, (O*)a.out, head, tail, zero_blocks, (W)a.scale);
+      if (p.values) run(lookup_grad_narrow_kernel<T, O, true, 1>);
     }
-    if (!p.values)
-      hipLaunchKernelGGL((lookup_grad_narrow_kernel<T, O, false>), grid, dim3(kThreads), 0, s, r, (const T*)a.grad, (O*)a.out, head, tail, zero_blocks, (W)a.scale);
+    if (!p.values) {
+      if (a.width == 1) run(lookup_grad_narrow_kernel<T, O, false, 1>);
+      else if (a.width == 2) run(lookup_grad_narrow_kernel<T, O, false, 2>);
+      else if (a.width == 3) run(lookup_grad_narrow_kernel<T, O, false, 3>);
+      else run(lookup_grad_narrow_kernel<T, O, false, 4>);
+    }
   } else {
     launch_runs<T, O, kPack<T>>(a, p, r, head, tail);
   }

@@ -33,10 +33,12 @@ def fail(what: str):
 
 
 def need_tensor(op: str, name: str, t):
+    """``t`` as its memory has to be read: a lazily negated view (``z.conj().imag``) is written out."""
     if not isinstance(t, torch.Tensor):
         fail(f"{op}: {name} has to be a torch tensor, got {type(t).__name__}")
     if t.requires_grad and torch.is_grad_enabled():
         fail(f"{op}: {name} requires grad, and nothing is recorded here: call it under torch.no_grad() and take the gradient from {op}_grad")
+    return t.resolve_neg() if t.is_neg() else t
 
 
 def need_type(op: str, name: str, t) -> int:

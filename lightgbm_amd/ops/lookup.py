@@ -18,13 +18,13 @@ _LOOKUP_GRAD = struct.Struct("17qd")
 _MAX_TOKENS = 2**31 - 1
 
 
-def _check_ids(op: str, ids) -> int:
-    need_tensor(op, "ids", ids)
+def _check_ids(op: str, ids):
+    ids = need_tensor(op, "ids", ids)
     if ids.dtype not in (torch.int32, torch.int64):
         fail(f"{op}: ids have to be int32 or int64, got {ids.dtype}")
     if ids.numel() > _MAX_TOKENS:
         fail(f"{op}: {ids.numel()} ids; at most 2^31 - 1 in one call")
-    return int(ids.dtype == torch.int64)
+    return ids, int(ids.dtype == torch.int64)
 
 
 def embedding(table, ids, scale: float = 1.0):
@@ -35,11 +35,11 @@ def embedding(table, ids, scale: float = 1.0):
     fp64) and rounded once.  Strided tables and ids are read in place as long as a row's values are neighbours and the
     ids' dimensions merge to two; otherwise they are copied first.
     """
-    need_tensor("embedding", "table", table)
+    table = need_tensor("embedding", "table", table)
     code = need_type("embedding", "table", table)
     if table.dim() != 2:
         fail(f"embedding: the table has to be [rows, width], got {tuple(table.shape)}")
-    wide_ids = _check_ids("embedding", ids)
+    ids, wide_ids = _check_ids("embedding", ids)
     device = need_device("embedding", table, ids)
     lib = core()
     rows, width = table.shape
@@ -66,9 +66,9 @@ def embedding_grad(grad, ids, num_rows: int, scale: float = 1.0, dtype=None):
     or float32; the sums are held in 32 bits (64 for fp64).  The tokens are sorted, so every row is added up in the order
     of its tokens and the result does not depend on timing.
     """
-    need_tensor("embedding_grad", "grad", grad)
+    grad = need_tensor("embedding_grad", "grad", grad)
     code = need_type("embedding_grad", "grad", grad)
-    wide_ids = _check_ids("embedding_grad", ids)
+    ids, wide_ids = _check_ids("embedding_grad", ids)
     if grad.dim() != ids.dim() + 1 or grad.shape[:-1] != ids.shape:
         fail(f"embedding_grad: grad has to be [*ids.shape, width], got {tuple(grad.shape)} for ids {tuple(ids.shape)}")
     if isinstance(num_rows, bool) or int(num_rows) != num_rows or not 0 <= num_rows < 2**31 - 1:

@@ -29,11 +29,11 @@ def _rows(t):
 
 
 def _check(op: str, x, code: int, gate, lengths, ends):
-    """Checks what forward and backward share; returns (gate, gate type code, groups)."""
+    """Checks what forward and backward share; returns (gate, gate type code, groups, the states at the ends, lengths)."""
     b, t, d = x.shape
     gate_code = groups = 0
     if gate is not None:
-        need_tensor(op, "gate", gate)
+        gate = need_tensor(op, "gate", gate)
         gate_code = need_type(op, "gate", gate)
         if gate_code != code and not (gate_code == 2 and code < 2):
             fail(f"{op}: a gate of {gate.dtype} for values of {x.dtype}; it has to be of that type or, for 16-bit values, float32")
@@ -43,24 +43,24 @@ def _check(op: str, x, code: int, gate, lengths, ends):
         if d and (groups < 1 or d % groups):
             fail(f"{op}: the width {d} is not a multiple of the gate's {groups} groups")
         gate = _rows(gate)
+    checked = []
     for name, end in ends:
         if end is not None:
-            need_tensor(op, name, end)
+            end = need_tensor(op, name, end)
             if end.dtype != _wide(x) or end.shape != (b, d):
                 fail(f"{op}: {name} has to be {_wide(x)} [{b}, {d}], got {end.dtype} {tuple(end.shape)}")
+            end = end.contiguous()
+        checked.append(end)
     if lengths is not None:
-        need_tensor(op, "lengths", lengths)
+        lengths = need_tensor(op, "lengths", lengths)
         if lengths.dtype != torch.int32 or lengths.shape != (b,):
             fail(f"{op}: lengths have to be int32 [{b}], got {lengths.dtype} {tuple(lengths.shape)}")
-    return gate, gate_code, groups
+        lengths = lengths.contiguous()
+    return gate, gate_code, groups, checked, lengths
 
 
 def _address(t) -> int:
     return 0 if t is None else t.data_ptr()
-
-
-def _contiguous(t):
-    return None if t is None else t.contiguous()
 
 
 def _gate_steps(gate, batch: int):
@@ -82,16 +82,16 @@ def gated_scan(x, gate=None, state=None, *, mix: bool = False, lengths=None):
     ``last`` back in continues a sequence, step by step or in pieces.  Gates are meant to lie in -1 .. 1: outside, the product
     of a long run of them may overflow, and then so do states that single steps would have kept finite.
     """
-    need_tensor("gated_scan", "x", x)
+    x = need_tensor("gated_scan", "x", x)
     code = need_type("gated_scan", "x", x)
     if x.dim() != 3:
         fail(f"gated_scan: x has to be [batch, steps, width], got {tuple(x.shape)}")
-    gate, gate_code, groups = _check("gated_scan", x, code, gate, lengths, (("state", state),))
+    gate, gate_code, groups, (state,), lengths = _check("gated_scan", x, code, gate, lengths, (("state", state),))
     if mix and gate is None:
         fail("gated_scan: the mixed form needs a gate")
     device = need_device("gated_scan", x, gate, state, lengths)
     lib = core()
-    x, state, lengths = _rows(x), _contiguous(state), _contiguous(lengths)
+    x = _rows(x)
     b, t, d = x.shape
     where = x.device
     states = torch.empty((b, t, d), dtype=x.dtype, device=where)
@@ -115,23 +115,21 @@ def gated_scan_grad(grad_states, states, gate=None, state=None, *, x=None, grad_
     type and shape - summed over the channels and sequences that shared a gate - and is ``None`` without one.  Behind a
     sequence's length all of them are zero.
     """
-    need_tensor("gated_scan_grad", "grad_states", grad_states)
-    need_tensor("gated_scan_grad", "states", states)
+    grad_states = need_tensor("gated_scan_grad", "grad_states", grad_states)
+    states = need_tensor("gated_scan_grad", "states", states)
+    x = None if x is None else need_tensor("gated_scan_grad", "x", x)
     code = need_type("gated_scan_grad", "states", states)
     if states.dim() != 3:
         fail(f"gated_scan_grad: states have to be [batch, steps, width], got {tuple(states.shape)}")
     for name, like in (("grad_states", grad_states), ("x", x)):
-        if like is not None:
-            need_tensor("gated_scan_grad", name, like)
-            if like.dtype != states.dtype or like.shape != states.shape:
-                fail(f"gated_scan_grad: {name} has to be {states.dtype} {tuple(states.shape)} as the states, got {like.dtype} {tuple(like.shape)}")
-    gate, gate_code, groups = _check("gated_scan_grad", states, code, gate, lengths, (("state", state), ("grad_last", grad_last)))
+        if like is not None and (like.dtype != states.dtype or like.shape != states.shape):
+            fail(f"gated_scan_grad: {name} has to be {states.dtype} {tuple(states.shape)} as the states, got {like.dtype} {tuple(like.shape)}")
+    gate, gate_code, groups, (state, grad_last), lengths = _check("gated_scan_grad", states, code, gate, lengths, (("state", state), ("grad_last", grad_last)))
     if mix and (gate is None or x is None):
         fail("gated_scan_grad: the mixed form needs the gate and x")
     device = need_device("gated_scan_grad", states, grad_states, x, gate, state, grad_last, lengths)
     lib = core()
     grad_states, states, x = _rows(grad_states), _rows(states), _rows(x) if mix else None
-    state, grad_last, lengths = _contiguous(state), _contiguous(grad_last), _contiguous(lengths)
     b, t, d = states.shape
     where = states.device
     grad_x = torch.empty((b, t, d), dtype=states.dtype, device=where)

@@ -666,3 +666,40 @@ def test_tensors_of_different_devices_are_refused():
         ops.embedding(torch.ones((2, 3)).cuda(), _I)
     with pytest.raises(LightGBMError, match="tensors on"):
         ops.gated_scan(_X.cuda(), torch.ones((2, 3, 4)))
+
+
+# -- views whose memory is not what they say --------------------------------------------------------------------------
+
+def _negated(t):
+    """Equal to ``t``, with -t in memory and torch's negative bit set."""
+    view = torch.complex(torch.zeros_like(t), -t).conj().imag
+    assert view.is_neg() and torch.equal(view, t)
+    return view
+
+
+def test_arguments_are_taken_as_their_memory_has_to_be_read():
+    from lightgbm_amd.ops import _args
+    v = torch.arange(1.0, 4.0).reshape(3, 1)
+    got = _args.need_tensor("op", "x", _negated(v))
+    assert not got.is_neg() and torch.equal(got, v)
+    assert _args.need_tensor("op", "x", v) is v
+
+
+@gpu
+@pytest.mark.parametrize("width", [1, 6])
+@pytest.mark.parametrize("name", ["f32", "f64"])
+def test_negated_views_are_read_with_their_sign(name, width):
+    g = rng(width)
+    ids = make_ids(g, (3, 20), 30).cuda()
+    table, grad, x, dh, state, dlast = (normal(g, shape, TYPES[name]).cuda()
+                                        for shape in ((30, width), (3, 20, width), (3, 20, width), (3, 20, width), (3, width), (3, width)))
+    gate = torch.sigmoid(normal(g, (3, 20, 1), TYPES[name])).cuda()
+    assert torch.equal(ops.embedding(_negated(table), ids), ops.embedding(table, ids))
+    assert torch.equal(ops.embedding_grad(_negated(grad), ids, 30), ops.embedding_grad(grad, ids, 30))
+    want = ops.gated_scan(x, gate, state, mix=True)
+    got = ops.gated_scan(_negated(x), _negated(gate), _negated(state), mix=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    states = want[0]
+    want = ops.gated_scan_grad(dh, states, gate, state, x=x, grad_last=dlast, mix=True)
+    got = ops.gated_scan_grad(_negated(dh), _negated(states), _negated(gate), _negated(state), x=_negated(x), grad_last=_negated(dlast), mix=True)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))

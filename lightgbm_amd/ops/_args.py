@@ -4,6 +4,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 from .._lib import LightGBMError
@@ -38,6 +39,8 @@ def need_tensor(op: str, name: str, t):
         fail(f"{op}: {name} has to be a torch tensor, got {type(t).__name__}")
     if t.requires_grad and torch.is_grad_enabled():
         fail(f"{op}: {name} requires grad, and nothing is recorded here: call it under torch.no_grad() and take the gradient from {op}_grad")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        fail(f"{op}: {name} is a dual tensor, and its tangent would be lost here: pass its primal value")
     return t.resolve_neg() if t.is_neg() else t
 
 

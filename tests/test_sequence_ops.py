@@ -703,3 +703,28 @@ def test_negated_views_are_read_with_their_sign(name, width):
     want = ops.gated_scan_grad(dh, states, gate, state, x=x, grad_last=dlast, mix=True)
     got = ops.gated_scan_grad(_negated(dh), _negated(states), _negated(gate), _negated(state), x=_negated(x), grad_last=_negated(dlast), mix=True)
     assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+DUALS = {
+    "table": lambda d: ops.embedding(d(30, 4), _I),
+    "grad": lambda d: ops.embedding_grad(d(3, 4), _I, 5),
+    "x": lambda d: ops.gated_scan(d(2, 3, 4)),
+    "gate": lambda d: ops.gated_scan(_X, d(2, 3, 4)),
+    "state": lambda d: ops.gated_scan(_X, None, d(2, 4)),
+    "grad_states": lambda d: ops.gated_scan_grad(d(2, 3, 4), _X),
+    "states": lambda d: ops.gated_scan_grad(_X, d(2, 3, 4)),
+    "x of the gradient": lambda d: ops.gated_scan_grad(_X, _X, torch.ones((2, 3, 4)), x=d(2, 3, 4), mix=True),
+    "grad_last": lambda d: ops.gated_scan_grad(_X, _X, grad_last=d(2, 4)),
+}
+
+
+@pytest.mark.parametrize("what", DUALS)
+def test_dual_tensors_are_refused(what):
+    """Their tangents would be dropped without a word; under no_grad() too, which leaves forward mode on."""
+    from torch.autograd import forward_ad
+    for grad_mode in (torch.enable_grad, torch.no_grad):
+        with forward_ad.dual_level(), grad_mode():
+            with pytest.raises(LightGBMError, match="dual"):
+                DUALS[what](lambda *shape: forward_ad.make_dual(torch.ones(shape), torch.ones(shape)))
+            with pytest.raises(LightGBMError, match="GPU"):          # others are taken inside a level too
+                DUALS[what](lambda *shape: torch.ones(shape))

@@ -38,25 +38,41 @@ struct GateSums {
   int64_t rows = 1, teams = 1;
 };
 
-__device__ __forceinline__ float smallest(float) { return 1.40129846e-45f; }
-__device__ __forceinline__ double smallest(double) { return 4.9406564584124654e-324; }
 __device__ __forceinline__ float abs_of(float x) { return __builtin_fabsf(x); }
 __device__ __forceinline__ double abs_of(double x) { return __builtin_fabs(x); }
-__device__ __forceinline__ float sign_of(float m, float s) { return __builtin_copysignf(m, s); }
-__device__ __forceinline__ double sign_of(double m, double s) { return __builtin_copysign(m, s); }
+__device__ __forceinline__ float mantissa(float x) { return __builtin_amdgcn_frexp_mantf(x); }
+__device__ __forceinline__ double mantissa(double x) { return __builtin_amdgcn_frexp_mant(x); }
+__device__ __forceinline__ int exponent(float x) { return __builtin_amdgcn_frexp_expf(x); }
+__device__ __forceinline__ int exponent(double x) { return __builtin_amdgcn_frexp_exp(x); }
+__device__ __forceinline__ float times_power(float x, int e) { return __builtin_ldexpf(x, e); }
+__device__ __forceinline__ double times_power(double x, int e) { return __builtin_ldexp(x, e); }
 
-// A product of gates that has underflowed although none of them is zero stays just above zero: an infinite state must
-// come out of it as infinite as out of the single steps, not as 0 * inf = NaN.
-template <typename W> __device__ __forceinline__ W kept(W product, bool any_zero) {
-  return product == 0 && !any_zero ? sign_of(smallest(product), product) : product;
+// The map of a run of steps, x -> (product of its gates) x + h.  The product is m 2^e and is right whatever its size: a hundred
+// gates of a half leave the range of fp32, but what they leave of a state of 1e30 does not, a state of zero stays zero
+// under gates above one, and an infinite state is no 0 * inf.  No product runs over more steps than lie between two
+// checkpoints, so e stays far from its ends.
+template <typename W, bool kGates> struct Map { W m; int e; W h; };
+template <typename W> struct Map<W, false> { W h; };      // without gates the product is one
+template <typename W, bool kGates> __device__ __forceinline__ Map<W, kGates> no_steps() {
+  if constexpr (kGates) return {1, 0, 0};
+  else return {0};
 }
 
-template <typename W> struct Map { W a, h; };
-
-// `later` after `first`
-template <typename W> __device__ __forceinline__ Map<W> after(const Map<W>& later, const Map<W>& first) {
-  return {kept(later.a * first.a, later.a == 0 || first.a == 0), fma_wide(later.a, first.h, later.h)};
+// 1 <= |m| < 2, or infinite, NaN, or zero (and then e too: it may hold large gates around the gate of zero)
+template <typename W> __device__ __forceinline__ Map<W, true> normal(const Map<W, true>& f) {
+  return {2 * mantissa(f.m), f.m == 0 ? 0 : f.e + exponent(f.m) - 1, f.h};
 }
+template <typename W> __device__ __forceinline__ Map<W, false> normal(const Map<W, false>& f) { return f; }
+
+// f normal
+template <typename W> __device__ __forceinline__ W apply(const Map<W, true>& f, W x) { return fma_wide(times_power(x, f.e), f.m, f.h); }
+template <typename W> __device__ __forceinline__ W apply(const Map<W, false>& f, W x) { return x + f.h; }
+
+// `later` (normal) after `first`; a fold of n normal maps has 1 <= |m| < 2^n
+template <typename W> __device__ __forceinline__ Map<W, true> after(const Map<W, true>& later, const Map<W, true>& first) {
+  return {later.m * first.m, later.e + first.e, apply(later, first.h)};
+}
+template <typename W> __device__ __forceinline__ Map<W, false> after(const Map<W, false>& later, const Map<W, false>& first) { return {first.h + later.h}; }
 
 // Words that tiles hand to one another.  Each is written once, whole, and read with agent scope until it is there: the
 // value itself is the flag.
@@ -79,21 +95,56 @@ template <int N> __device__ __forceinline__ void wait_words(const uint64_t* p, u
     load_words(p, w);
   }
 }
-// fp32: one word (a low, h high).  A NaN pair that reads as kEmpty becomes another NaN pair.
-__device__ __forceinline__ void publish(uint64_t* p, const Map<float>& m) {
-  const uint64_t v = (uint64_t)__float_as_uint(m.a) | (uint64_t)__float_as_uint(m.h) << 32;
-  __hip_atomic_store(p, v == kEmpty ? 0x7fc000007fc00000ull : v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// The product of a normal map in as many bits as m: the field of m's exponent and two bits of its fraction hold e, up to 2^509
+// (2^4093 for fp64), beyond which the product makes zero or infinity of any state of the type.  What the two bits round is four
+// roundings of W, where the gates of a tile have at least 128 (a word of its own for e: 145 against 121 us at 1 x 65537 x 1024 bf16).
+template <typename W> struct Bits;
+template <> struct Bits<float> { typedef uint32_t U; static constexpr int fraction = 23, exponent = 8; };
+template <> struct Bits<double> { typedef uint64_t U; static constexpr int fraction = 52, exponent = 11; };
+
+template <typename W> __device__ __forceinline__ typename Bits<W>::U packed(W m, int e) {
+  typedef typename Bits<W>::U U;
+  constexpr int F = Bits<W>::fraction, X = Bits<W>::exponent, kMiddle = 1 << (X + 1);
+  constexpr U kSign = (U)1 << (F + X), kOnes = ((U)4 << X) - 1;     // of e: 0 for zero, all ones for what is not finite
+  U bits;
+  __builtin_memcpy(&bits, &m, sizeof m);
+  const U scale = (U)(min(max(e, 1 - kMiddle), kMiddle - 3) + kMiddle);
+  U p = (scale << (F - 2)) + (((bits & (((U)1 << F) - 1)) + 2) >> 2);      // a fraction rounded up to one goes into e
+  if (m == 0) p = 0;
+  if (!(abs_of(m) < 2)) p = kOnes << (F - 2) | (m != m);
+  return p | (bits & kSign);
 }
-__device__ __forceinline__ Map<float> read_map(const uint64_t* w, float) { return {__uint_as_float((uint32_t)*w), __uint_as_float((uint32_t)(*w >> 32))}; }
+template <typename W> __device__ __forceinline__ void unpack(typename Bits<W>::U p, W& m, int& e) {
+  typedef typename Bits<W>::U U;
+  constexpr int F = Bits<W>::fraction, X = Bits<W>::exponent, kMiddle = 1 << (X + 1);
+  constexpr U kSign = (U)1 << (F + X), kOnes = ((U)4 << X) - 1;
+  const U scale = p >> (F - 2) & kOnes;
+  e = (int)scale - kMiddle;
+  const U field = scale == 0 ? 0 : scale == kOnes ? ((U)1 << X) - 1 : ((U)1 << (X - 1)) - 1;
+  const U bits = (p & kSign) | field << F | (p << 2 & (((U)1 << F) - 1));
+  __builtin_memcpy(&m, &bits, sizeof m);
+}
+// fp32: one word; never kEmpty, whose product is none that packed() gives
+__device__ __forceinline__ void publish(uint64_t* p, const Map<float, true>& f) { put_word(p, (uint64_t)packed(f.m, f.e) << 32 | __float_as_uint(f.h)); }
+__device__ __forceinline__ void read_map(const uint64_t* w, Map<float, true>& f) {
+  unpack((uint32_t)(*w >> 32), f.m, f.e);
+  f.h = __uint_as_float((uint32_t)*w);
+}
 // fp64: two words
-__device__ __forceinline__ void publish(uint64_t* p, const Map<double>& m) {
-  put_word(p, (uint64_t)__double_as_longlong(m.a));
-  put_word(p + 1, (uint64_t)__double_as_longlong(m.h));
+__device__ __forceinline__ void publish(uint64_t* p, const Map<double, true>& f) {
+  put_word(p, packed(f.m, f.e));
+  put_word(p + 1, (uint64_t)__double_as_longlong(f.h));
 }
-__device__ __forceinline__ Map<double> read_map(const uint64_t* w, double) {
-  return {__longlong_as_double((int64_t)w[0]), __longlong_as_double((int64_t)w[1])};
+__device__ __forceinline__ void read_map(const uint64_t* w, Map<double, true>& f) {
+  unpack(w[0], f.m, f.e);
+  f.h = __longlong_as_double((int64_t)w[1]);
 }
-template <typename W> constexpr int kMapWords = sizeof(W) / 4;
+// states, and maps without gates
+__device__ __forceinline__ void publish(uint64_t* p, const Map<float, false>& f) { put_word(p, __float_as_uint(f.h)); }
+__device__ __forceinline__ void read_map(const uint64_t* w, Map<float, false>& f) { f = {__uint_as_float((uint32_t)*w)}; }
+__device__ __forceinline__ void publish(uint64_t* p, const Map<double, false>& f) { put_word(p, (uint64_t)__double_as_longlong(f.h)); }
+__device__ __forceinline__ void read_map(const uint64_t* w, Map<double, false>& f) { f = {__longlong_as_double((int64_t)*w)}; }
+template <typename W, bool kGates> constexpr int kMapWords = kGates ? sizeof(W) / 4 : 1;
 
 __global__ __launch_bounds__(kThreads) void fill_words_kernel(uint4* __restrict__ p, int64_t n) {
   for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) p[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
@@ -109,9 +160,9 @@ struct Cut {
 };
 
 // Workspace of a cut into several tiles, in words: [0] tickets, then the tiles' maps, then the checkpoints' states.
-template <typename W> __host__ __device__ inline int64_t map_words(const Cut& k, int v) { return k.tiles * k.pack_rows * k.lanes * v * kMapWords<W>; }
-template <typename W> inline int64_t work_words(const Cut& k, int v) {
-  const int64_t n = 8 + map_words<W>(k, v) + (k.tiles / k.checkpoint + 1) * k.pack_rows * k.lanes * v * kMapWords<W>;
+template <typename W> inline int64_t work_words(const Cut& k, int v, bool gates) {
+  const int64_t channels = k.pack_rows * k.lanes * v, map = gates ? kMapWords<W, true> : kMapWords<W, false>;
+  const int64_t n = 8 + k.tiles * channels * map + (k.tiles / k.checkpoint + 1) * channels;
   return k.tiles < 2 ? 0 : (n + 1) / 2 * 2;
 }
 
@@ -131,58 +182,63 @@ __device__ __forceinline__ void take_tile(const Cut& k, uint64_t* work, int64_t&
 
 // The state before this lane's chunk, given the chunk's own map.  `first`: the state before the first tile.
 // Returns it in `carry`.
-template <typename W, int V>
-__device__ __forceinline__ void carry_in(const Cut& k, uint64_t* work, int64_t tile, int64_t row, int lane, int slot, const Map<W> (&own)[V], const W (&first)[V],
-                                         W (&carry)[V]) {
+template <typename W, int V, bool kGates>
+__device__ __forceinline__ void carry_in(const Cut& k, uint64_t* work, int64_t tile, int64_t row, int lane, int slot, const Map<W, kGates> (&own)[V],
+                                         const W (&first)[V], W (&carry)[V]) {
+  typedef Map<W, kGates> M;
+  constexpr int kWords = kMapWords<W, kGates>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  Map<W>(*maps)[V] = (Map<W>(*)[V])lds;                       // [slots][lanes]
-  Map<W>(*parts)[V] = maps + k.slots * k.lanes;               // partial folds of the tiles before this one
+  M(*maps)[V] = (M(*)[V])lds;                                 // [slots][lanes]
+  M(*parts)[V] = maps + k.slots * k.lanes;                    // partial folds of the tiles before this one
   const int at = slot * k.lanes + lane;
   for (int v = 0; v < V; ++v) maps[at][v] = own[v];
   __syncthreads();
-  Map<W> mine[V];                                             // the chunks of this tile before this one
-  for (int v = 0; v < V; ++v) mine[v] = {1, 0};
+  M mine[V];                                                  // the chunks of this tile before this one
+  for (int v = 0; v < V; ++v) mine[v] = no_steps<W, kGates>();
   for (int s = 0; s < slot; ++s)
     for (int v = 0; v < V; ++v) mine[v] = after(maps[s * k.lanes + lane][v], mine[v]);
   for (int v = 0; v < V; ++v) carry[v] = first[v];
+  const int64_t channels = k.pack_rows * k.lanes * V, channel = (row * k.lanes + lane) * V;
   if (k.tiles > 1) {
-    const int64_t stride = k.pack_rows * k.lanes * V * kMapWords<W>;
-    uint64_t* tile_maps = work + 8 + (row * k.lanes + lane) * V * kMapWords<W>;
-    uint64_t* checkpoints = tile_maps + k.tiles * stride;
+    uint64_t* tile_maps = work + 8 + channel * kWords;        // channels * kWords of them a tile
     if (slot == k.slots - 1 && tile + 1 < k.tiles)
-      for (int v = 0; v < V; ++v) publish(tile_maps + tile * stride + v * kMapWords<W>, after(own[v], mine[v]));
+      for (int v = 0; v < V; ++v) publish(tile_maps + tile * channels * kWords + v * kWords, normal(after(own[v], mine[v])));
     const int64_t from = tile / k.checkpoint * k.checkpoint;    // first tile behind the last checkpoint
     const int before = (int)(tile - from), share = (before + k.slots - 1) / k.slots;
-    const uint64_t* checkpoint = checkpoints + (from / k.checkpoint - 1) * stride;
-    uint64_t words[V * kMapWords<W>], state[V * kMapWords<W>];
+    const uint64_t* checkpoint = work + 8 + k.tiles * channels * kWords + (from / k.checkpoint - 1) * channels + channel;
+    uint64_t words[V * kWords], state[V];
     if (from > 0) load_words(checkpoint, state);              // on its way while the maps are waited for
-    Map<W> part[V];
-    for (int v = 0; v < V; ++v) part[v] = {1, 0};
+    M part[V];
+    for (int v = 0; v < V; ++v) part[v] = no_steps<W, kGates>();
     for (int p = slot * share; p < min(before, (slot + 1) * share); ++p) {
-      const uint64_t* const map = tile_maps + (from + p) * stride;
+      const uint64_t* const map = tile_maps + (from + p) * channels * kWords;
       load_words(map, words);
       wait_words(map, words);
-      for (int v = 0; v < V; ++v) part[v] = after(read_map(words + v * kMapWords<W>, (W)0), part[v]);
+      for (int v = 0; v < V; ++v) {
+        M m;
+        read_map(words + v * kWords, m);
+        part[v] = after(m, part[v]);
+      }
     }
-    for (int v = 0; v < V; ++v) parts[at][v] = part[v];
+    for (int v = 0; v < V; ++v) parts[at][v] = normal(part[v]);
     if (from > 0) {
       wait_words(checkpoint, state);
-      for (int v = 0; v < V; ++v) carry[v] = read_map(state + v * kMapWords<W>, (W)0).h;
+      for (int v = 0; v < V; ++v) {
+        Map<W, false> c;
+        read_map(state + v, c);
+        carry[v] = c.h;
+      }
     }
     __syncthreads();
     if (before)
       for (int s = 0; s * share < before; ++s)
-        for (int v = 0; v < V; ++v) {
-          const Map<W> m = parts[s * k.lanes + lane][v];
-          carry[v] = fma_wide(m.a, carry[v], m.h);
-        }
-    if (slot == k.slots - 1 && (tile + 1) % k.checkpoint == 0 && tile + 1 < k.tiles)
-      for (int v = 0; v < V; ++v) {
-        const Map<W> m = after(own[v], mine[v]);
-        publish(checkpoints + tile / k.checkpoint * stride + v * kMapWords<W>, Map<W>{0, fma_wide(m.a, carry[v], m.h)});
-      }
+        for (int v = 0; v < V; ++v) carry[v] = apply(parts[s * k.lanes + lane][v], carry[v]);
   }
-  for (int v = 0; v < V; ++v) carry[v] = fma_wide(mine[v].a, carry[v], mine[v].h);
+  for (int v = 0; v < V; ++v) carry[v] = apply(normal(mine[v]), carry[v]);
+  if (slot == k.slots - 1 && (tile + 1) % k.checkpoint == 0 && tile + 1 < k.tiles) {
+    uint64_t* checkpoint = work + 8 + k.tiles * channels * kWords + tile / k.checkpoint * channels + channel;
+    for (int v = 0; v < V; ++v) publish(checkpoint + v, Map<W, false>{apply(maps[at][v], carry[v])});
+  }
 }
 
 // The channels of a pack: d .. d + V - 1 of sequence b.  The last pack of a width that V does not divide starts earlier; its
@@ -305,9 +361,8 @@ __global__ __launch_bounds__(kLanes* kMaxSlots) void scan_kernel(ScanArgs a, Cut
   W h[V], first[V];
   for (int v = 0; v < V; ++v) first[v] = a.state && live ? ((const W*)a.state)[c + v] : (W)0;
   if (k.tiles > 1 || k.slots > 1) {
-    Map<W> own[V];
-    W least[V];
-    for (int v = 0; v < V; ++v) own[v] = {1, 0}, least[v] = 1;
+    Map<W, K != kNoGate> own[V];
+    for (int v = 0; v < V; ++v) own[v] = no_steps<W, K != kNoGate>();
 #pragma unroll
     for (int j = 0; j < L; ++j)
       for (int v = 0; v < V; ++v) {
@@ -318,14 +373,14 @@ __global__ __launch_bounds__(kLanes* kMaxSlots) void scan_kernel(ScanArgs a, Cut
           const W g = (W)gs[j].v[v];
           if (a.mix) in *= (W)1 - g;
           own[v].h = fma_wide(g, own[v].h, in);
-          own[v].a *= g;
-          least[v] = min(least[v], abs_of(g));
+          own[v].m *= mantissa(g);
+          own[v].e += exponent(g);
         }
       }
-    for (int v = 0; v < V; ++v) own[v].a = kept(own[v].a, least[v] == 0);
+    for (int v = 0; v < V; ++v) own[v] = normal(own[v]);
     as_loaded(xs);
     if constexpr (K != kNoGate) as_loaded(gs);
-    carry_in<W, V>(k, (uint64_t*)a.work, tile, row, lane, slot, own, first, h);
+    carry_in<W, V, K != kNoGate>(k, (uint64_t*)a.work, tile, row, lane, slot, own, first, h);
   } else {
     for (int v = 0; v < V; ++v) h[v] = first[v];
   }
@@ -426,9 +481,8 @@ __global__ __launch_bounds__(kLanes* kMaxSlots) void scan_grad_kernel(ScanGradAr
   W e[V], first[V];
   for (int v = 0; v < V; ++v) first[v] = a.grad_last && live ? ((const W*)a.grad_last)[c + v] : (W)0;
   if (k.tiles > 1 || k.slots > 1) {
-    Map<W> own[V];
-    W least[V];
-    for (int v = 0; v < V; ++v) own[v] = {1, 0}, least[v] = 1;
+    Map<W, K != kNoGate> own[V];
+    for (int v = 0; v < V; ++v) own[v] = no_steps<W, K != kNoGate>();
 #pragma unroll
     for (int j = 0; j < L; ++j)
       for (int v = 0; v < V; ++v) {
@@ -436,14 +490,14 @@ __global__ __launch_bounds__(kLanes* kMaxSlots) void scan_grad_kernel(ScanGradAr
         if constexpr (K != kNoGate) {
           const W g = (W)as[j].v[v];
           own[v].h *= g;
-          own[v].a *= g;
-          least[v] = min(least[v], abs_of(g));
+          own[v].m *= mantissa(g);
+          own[v].e += exponent(g);
         }
       }
-    for (int v = 0; v < V; ++v) own[v].a = kept(own[v].a, least[v] == 0);
+    for (int v = 0; v < V; ++v) own[v] = normal(own[v]);
     as_loaded(gs);
     if constexpr (K != kNoGate) as_loaded(as);
-    carry_in<W, V>(k, work, tile, row, lane, slot, own, first, e);
+    carry_in<W, V, K != kNoGate>(k, work, tile, row, lane, slot, own, first, e);
   } else {
     for (int v = 0; v < V; ++v) e[v] = first[v];
   }
@@ -608,10 +662,12 @@ template <bool Two, int Steps, typename A, typename F> void by_shape(const A& a,
   else with_kind(Const<kSharedGate>());
 }
 
-template <typename W> size_t fold_bytes(const Cut& k, int v) { return k.tiles * k.slots == 1 ? 0 : 2 * k.slots * k.lanes * v * sizeof(Map<W>); }
+template <typename W> size_t fold_bytes(const Cut& k, int v, bool gates) {
+  return k.tiles * k.slots == 1 ? 0 : 2 * k.slots * k.lanes * v * (gates ? sizeof(Map<W, true>) : sizeof(Map<W, false>));
+}
 
-template <typename W> void clear_work(const Cut& k, int v, uint64_t* work, hipStream_t s) {
-  const int64_t n = work_words<W>(k, v);
+template <typename W> void clear_work(const Cut& k, int v, bool gates, uint64_t* work, hipStream_t s) {
+  const int64_t n = work_words<W>(k, v, gates);
   if (!n) return;
   hipLaunchKernelGGL(fill_words_kernel, dim3((unsigned)std::min<int64_t>((n / 2 + kThreads - 1) / kThreads, 2048)), dim3(kThreads), 0, s, (uint4*)work, n / 2);
   LGA_HIP_CHECK(hipGetLastError());
@@ -654,7 +710,7 @@ int64_t scan_workspace(const ScanArgs& a) {
   check_args(a);
   const int v = two_wide(a) ? 2 : 1;
   const Cut k = cut_steps(a.batch, a.steps, a.width, v, a.steps <= 1 ? 1 : kScanSteps, scan_slots(a));
-  return 8 * (a.type == kF64 ? work_words<double>(k, v) : work_words<float>(k, v));
+  return 8 * (a.type == kF64 ? work_words<double>(k, v, a.gate != 0) : work_words<float>(k, v, a.gate != 0));
 }
 
 void gated_scan(const ScanArgs& a) {
@@ -667,9 +723,9 @@ void gated_scan(const ScanArgs& a) {
     by_shape<sizeof(T) < 8, kScanSteps>(a, [&](auto kind, auto v, auto l) {
       constexpr int V = decltype(v)::value, L = decltype(l)::value;
       const Cut k = cut_steps(a.batch, a.steps, a.width, V, L, scan_slots(a));
-      clear_work<Wide<T>>(k, V, (uint64_t*)a.work, (hipStream_t)a.stream);
+      clear_work<Wide<T>>(k, V, a.gate != 0, (uint64_t*)a.work, (hipStream_t)a.stream);
       hipLaunchKernelGGL((scan_kernel<T, G, (GateKind)decltype(kind)::value, V, L>), dim3((unsigned)(k.tiles * k.pack_rows)), dim3(k.lanes * k.slots),
-                         fold_bytes<Wide<T>>(k, V), (hipStream_t)a.stream, a, k);
+                         fold_bytes<Wide<T>>(k, V, a.gate != 0), (hipStream_t)a.stream, a, k);
       LGA_HIP_CHECK(hipGetLastError());
     });
   });
@@ -680,7 +736,7 @@ int64_t scan_grad_workspace(const ScanGradArgs& a) {
   const int v = two_wide(a) ? 2 : 1;
   const int steps = a.steps <= 1 ? 1 : grad_steps(a.type);
   const Cut k = cut_steps(a.batch, a.steps, a.width, v, steps, grad_slots(a.type));
-  return 8 * (a.type == kF64 ? work_words<double>(k, v) : work_words<float>(k, v)) + slope_values(a, gate_sums(a, k, v, steps)) * (a.type == kF64 ? 8 : 4);
+  return 8 * (a.type == kF64 ? work_words<double>(k, v, a.gate != 0) : work_words<float>(k, v, a.gate != 0)) + slope_values(a, gate_sums(a, k, v, steps)) * (a.type == kF64 ? 8 : 4);
 }
 
 void gated_scan_grad(const ScanGradArgs& a) {
@@ -696,11 +752,11 @@ void gated_scan_grad(const ScanGradArgs& a) {
       constexpr int V = decltype(v)::value, L = decltype(l)::value;
       const Cut k = cut_steps(a.batch, a.steps, a.width, V, L, grad_slots(a.type));
       uint64_t* work = (uint64_t*)a.work;
-      clear_work<W>(k, V, work, s);
+      clear_work<W>(k, V, a.gate != 0, work, s);
       const GateSums g = gate_sums(a, k, V, L);
-      const int64_t slopes = slope_values(a, g) ? (int64_t)(work + work_words<W>(k, V)) : 0;
+      const int64_t slopes = slope_values(a, g) ? (int64_t)(work + work_words<W>(k, V, a.gate != 0)) : 0;
       hipLaunchKernelGGL((scan_grad_kernel<T, G, (GateKind)decltype(kind)::value, V, L>), dim3((unsigned)(k.tiles * k.pack_rows)), dim3(k.lanes * k.slots),
-                         fold_bytes<W>(k, V), s, a, k, work, slopes, g);
+                         fold_bytes<W>(k, V, a.gate != 0), s, a, k, work, slopes, g);
       LGA_HIP_CHECK(hipGetLastError());
       if (slopes) {
         // the slopes, or the teams' sums of them: [rows][steps][across]

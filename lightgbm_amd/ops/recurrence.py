@@ -79,8 +79,8 @@ def gated_scan(x, gate=None, state=None, *, mix: bool = False, lengths=None):
     the state before the first step (zeros if not given).  ``lengths``: int32 [batch]; behind a sequence's length (clamped to
     0 .. steps) the states are zero, ``last`` is the state after its last step, and what stands in ``x`` and ``gate`` there
     is not used.  States are carried in float32 (float64 for fp64), which is also the type of ``state`` and ``last``: feeding
-    ``last`` back in continues a sequence, step by step or in pieces.  Gates are meant to lie in -1 .. 1: outside, the product
-    of a long run of them may overflow, and then so do states that single steps would have kept finite.
+    ``last`` back in continues a sequence, step by step or in pieces.  The product of a run of gates may
+    leave the type's range either way; results are finite wherever the recurrence over absolute values is.
     """
     x = need_tensor("gated_scan", "x", x)
     code = need_type("gated_scan", "x", x)

@@ -728,3 +728,74 @@ def test_dual_tensors_are_refused(what):
                 DUALS[what](lambda *shape: forward_ad.make_dual(torch.ones(shape), torch.ones(shape)))
             with pytest.raises(LightGBMError, match="GPU"):          # others are taken inside a level too
                 DUALS[what](lambda *shape: torch.ones(shape))
+
+
+# -- products of gates beyond the type's range --------------------------------------------------------------------------
+
+#         type  steps state     gate
+FADING = [("f32", 300, 1e30, 0.5), ("f32", 3000, 1e30, -0.5), ("f32", 1000, 1.2e30, 0.9), ("f32", 700, 3e38, 0.8), ("f32", 40, 1e30, 2.0**-20),
+          ("f32", 2100, 1e30, 2.0**-140), ("bf16", 700, 1e30, 0.5), ("f64", 3000, 1e300, 0.5), ("f64", 5000, 1e300, -0.81), ("f64", 300, 1e300, 2.0**-60),
+          # products above the range too, of states that stay within it
+          ("f32", 200, 2.0**-120, 2.0), ("f32", 600, 0.0, 4.0), ("f64", 1200, 2.0**-1000, 2.0), ("f64", 700, 0.0, 2.0**9)]
+
+
+@gpu
+@pytest.mark.parametrize("groups", [1, 24])
+@pytest.mark.parametrize("name,t,start,factor", FADING)
+def test_products_of_gates_leave_the_range_and_states_do_not(name, t, start, factor, groups):
+    """What is left of a state is the product of many gates times a large (small, no) number, whatever the product alone is."""
+    g = rng(t)
+    b, d = 2, 24
+    x, w = torch.zeros((b, t, d), dtype=TYPES[name]), wide(TYPES[name])
+    x[:, -1] = 1.0
+    gate = torch.full((b, t, groups), factor, dtype=w)
+    gate[1, t // 2:] = gate[1, t // 2:].abs().clamp(max=1.0)
+    state = start * (1 + 0.1 * torch.rand((b, d), generator=g, dtype=w))
+    states, last = ops.gated_scan(x.cuda(), gate.cuda(), state.cuda())
+    want, want_last, bound, bound_last = scan_oracle(x, gate, state, False, None)
+    within(states, want, bound, x.dtype)
+    within(last, want_last, bound_last, w)
+
+    x, gate = x.flip(1), gate.flip(1)                       # backwards the gradient of the last state fades
+    before = torch.zeros_like(x)
+    got = ops.gated_scan_grad(x.cuda(), before.cuda(), gate.cuda(), grad_last=state.cuda())
+    for value, oracle, dtype in zip(got, scan_grad_oracle(x, before, gate, None, None, state, False, None), (x.dtype, w, w)):
+        within(value, *oracle, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("name,factor", [("f32", 2.0**-30), ("f32", -0.5), ("f64", 2.0**-300), ("f64", -0.5)])
+def test_infinite_states_stay_infinite_under_gates_that_are_not_zero(name, factor):
+    t = 2501
+    w = TYPES[name]
+    state = torch.tensor([[float("inf"), -float("inf"), 1.0, 0.0]], dtype=w)
+    zero = torch.zeros((1, t, 4), dtype=w)
+    gate = torch.full((1, t, 1), factor, dtype=w)
+    sign = torch.sign(torch.tensor(factor, dtype=w)) ** torch.arange(1, t + 1, dtype=w)
+    _, last = ops.gated_scan(zero.cuda(), gate.cuda(), state.cuda())
+    assert last.cpu().tolist() == [[sign[-1].item() * float("inf"), -sign[-1].item() * float("inf"), 0.0, 0.0]]
+    gate[0, 1700] = 0.0                                      # 0 * inf, as step by step
+    states, last = ops.gated_scan(zero.cuda(), gate.cuda(), state.cuda())
+    states = states.cpu()
+    assert torch.equal(states[0, :1700, 0], sign[:1700] * float("inf")) and states[0, 1700:, :2].isnan().all() and states[0, 1700:, 2:].eq(0).all()
+    _, grad_state, _ = ops.gated_scan_grad(zero.cuda(), zero.cuda(), gate.abs().clamp(min=0.25).cuda(), grad_last=state.cuda())
+    assert grad_state.cpu().tolist() == [[float("inf"), -float("inf"), 0.0, 0.0]]
+
+
+@gpu
+@pytest.mark.parametrize("name,power", [("f32", 9), ("f64", 80)])
+def test_a_gate_of_zero_between_large_gates_leaves_nothing(name, power):
+    """The product of a run is zero, and so is what it leaves of a state, however large the gates around the zero are."""
+    t, w = 700, TYPES[name]
+    gate = torch.full((1, t, 1), 2.0**power, dtype=w)
+    zeros = [5, 300, 301]
+    gate[0, zeros] = 0.0
+    x = torch.zeros((1, t, 8), dtype=w)
+    state = torch.linspace(-1.0, 1.0, 8, dtype=w).reshape(1, 8)
+    states, last = ops.gated_scan(x.cuda(), gate.cuda(), state.cuda())
+    assert not states[0, 5:].any() and not last.any()
+    want = torch.ldexp(state.double(), power * torch.arange(1, 6).reshape(1, 5, 1))
+    assert torch.equal(states[:, :5].cpu().double(), want)               # powers of two: exact
+    _, grad_state, grad_gate = ops.gated_scan_grad(x.cuda(), states, gate.flip(1).cuda(), grad_last=state.cuda())
+    assert not grad_state.any()
+    assert torch.isfinite(grad_gate).all()

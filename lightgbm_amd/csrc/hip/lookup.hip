@@ -68,7 +68,7 @@ __global__ __launch_bounds__(kThreads) void lookup_tile_kernel(const T* __restri
   const bool along0 = grid.s0 < grid.s1;
   const int live1 = (int)min((int64_t)side1, grid.n1 - j0), live0 = (int)min((int64_t)1 << shift0, grid.n0 - i0);
   // A lane's items are kThreads apart, which is a fixed way in both walks unless an axis is longer than that and not all.
-  const bool whole = live0 == 1 << shift0 && live1 == side1 && (shift1 <= 8 || shift1 == kBits);
+  const bool whole = live0 == 1 << shift0 && live1 == side1 && (shift1 <= 8 || shift1 == kBits) && (!along0 || shift0 <= 8);
   const int t = threadIdx.x;
   if (whole) {
     const int i = along0 ? t & ((1 << shift0) - 1) : t >> shift1, j = along0 ? t >> shift0 : t & (side1 - 1);

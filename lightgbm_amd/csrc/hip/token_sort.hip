@@ -359,11 +359,14 @@ Layout layout(const TokenTiles& t, int payload, int64_t rows) {
 
 TokenTiles token_tiles(const TokenGrid& g, int bits) {
   TokenTiles t;
-  // sides: as many tokens along axis 0 as there are, up to 64 (256 bytes of int32 ids where they are neighbours)
-  int shift0 = 0;
+  // sides: as many tokens along axis 0 as there are, up to 64 (256 bytes of int32 ids where they are neighbours), or more where
+  // axis 1 does not fill the rest: a tile is more than half full, and 2^31 - 1 tokens have places of 32 bits
+  int shift0 = 0, shift1 = 0;
   while (shift0 < 6 && (1LL << shift0) < g.n0) ++shift0;
+  while (shift1 < bits - shift0 && (1LL << shift1) < g.n1) ++shift1;
+  shift0 = bits - shift1;
   t.bits = bits;
-  t.shift1 = bits - shift0;
+  t.shift1 = shift1;
   t.across = (g.n1 + (1LL << t.shift1) - 1) >> t.shift1;
   t.blocks = ((g.n0 + (1LL << shift0) - 1) >> shift0) * t.across;
   t.count = t.blocks << bits;

@@ -799,3 +799,57 @@ def test_a_gate_of_zero_between_large_gates_leaves_nothing(name, power):
     _, grad_state, grad_gate = ops.gated_scan_grad(x.cuda(), states, gate.flip(1).cuda(), grad_last=state.cuda())
     assert not grad_state.any()
     assert torch.isfinite(grad_gate).all()
+
+
+# -- token grids with a short axis ---------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("n0,n1", [(1000000, 2), (1000000, 3), (90001, 33), (50001, 65), (3000, 1001), (65, 50001), (33, 90001), (3, 1000000),
+                                   (2**30 - 1, 2), (715827882, 3), (65075262, 33), (33038209, 65), (16519104, 130), (46340, 46341), (65, 33038209),
+                                   (33, 65075262), (2, 2**30 - 1), (1, 2**31 - 1)])
+def test_sorted_token_grids_are_filled_up_to_less_than_twice_their_size(n0, n1):
+    """The core sizes its workspace on the host: 16 bytes of ids and token numbers a slot, up to 2 of counts, a few thousandths of
+    partial sums, 1 a table row; a slot belongs to a token or fills up a tile of at most 4096, and there are less than two a
+    token and some tiles at the edges (at most one row of tiles of 64 and one column, or 2 MB)."""
+    import ctypes
+    from lightgbm_amd import _lib, build
+    from lightgbm_amd.ops import lookup
+    lib, hip = _lib.load()
+    if not hip:
+        path = build.PKG / "_lga_hip.so"
+        if not path.exists():
+            pytest.skip("the HIP core is not built")
+        lib = ctypes.CDLL(str(path))
+        lib.lga_hip_embedding_grad.argtypes = [ctypes.c_char_p, ctypes.POINTER(ctypes.c_int64)]
+        lib.lga_last_error.restype = ctypes.c_char_p
+    rows, tokens = 200000, n0 * n1
+    for ids_stride in ((n1 + 1, 1), (1, n0 + 1)):
+        for grad_stride in ((n1 + 1, 1), (1, n0 + 1)):
+            need = ctypes.c_int64()
+            words = lookup._LOOKUP_GRAD.pack(1, 1, 1, 0, 0, 0, rows, 1, n0, n1, *ids_stride, *grad_stride, 2, 2, 0, 1.0)      # no workspace: only its size
+            assert lib.lga_hip_embedding_grad(words, need) == 0, lib.lga_last_error()
+            assert tokens * 16 <= need.value <= 2 * 18.1 * tokens + rows + 2**21
+
+
+SHORT_AXIS = [((300001, 2), 70001, 1, "f32"), ((2, 300001), 70001, 1, "f64"), ((40001, 3), 70001, 2, "bf16"), ((30007, 3), 300, 1, "f64"),
+              ((9001, 5), 20000, 40, "f32"), ((2049, 33), 60000, 3, "f16"), ((2049, 65), 60000, 1, "f64"), ((300, 129), 60000, 7, "f32"), ((5000001, 2), 500, 1, "bf16")]
+
+
+@gpu
+@pytest.mark.parametrize("shape,rows,width,name", SHORT_AXIS)
+def test_token_grids_with_a_short_axis(shape, rows, width, name):
+    """Ids that cannot merge to one axis, either one's neighbours next to each other: lookup and gradient."""
+    g = rng(rows + shape[0])
+    whole = make_ids(g, (shape[0], shape[1] + 1), rows, torch.int32, 0.05)
+    table, grad = normal(g, (rows, width), TYPES[name]), normal(g, (*shape, width), TYPES[name])
+    table_g, grad_g = table.cuda(), grad.cuda()
+    ids = whole[:, 1:]
+    looked = lookup_oracle(table, ids, 0.3)
+    want, mag, n = lookup_grad_oracle(grad, ids, rows, 0.3)
+    # all of 1e7 tokens to 500 rows in 16 bits: the count of a row's tokens times u(fp32) stays far below one
+    for view in (whole.cuda()[:, 1:], whole.t().contiguous().cuda().t()[:, 1:]):
+        assert torch.equal(view.cpu(), ids) and not view.is_contiguous()
+        within(ops.embedding(table_g, view, 0.3), looked, 3 * u(wide(TYPES[name])) * looked.abs(), TYPES[name])
+        got = ops.embedding_grad(grad_g, view, rows, scale=0.3, dtype=torch.float32 if name in ("bf16", "f16") else None)
+        within(got, want, (n + 4).reshape(-1, 1) * u(wide(TYPES[name])) * mag, got.dtype)
+        got = ops.embedding_grad(grad_g.transpose(0, 1), view.t(), rows, scale=0.3, dtype=got.dtype)
+        within(got, want, (n + 4).reshape(-1, 1) * u(wide(TYPES[name])) * mag, got.dtype)

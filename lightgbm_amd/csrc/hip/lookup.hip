@@ -788,7 +788,8 @@ template <typename T, typename O> void run_lookup_grad(const LookupGradArgs& a) 
     int bits = 1;
     while (a.rows >> bits) ++bits;
     auto run = [&](auto kernel) {
-      if (few.lds > 65536) LGA_HIP_CHECK(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, few.lds));
+      // the limit belongs to the process: always the same one, or a call from another thread could lower it before this launch
+      if (few.lds > 65536) LGA_HIP_CHECK(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kPrivateLds));
       hipLaunchKernelGGL(kernel, dim3(few.waves, (unsigned)a.width), dim3(64), few.lds, s, (const T*)a.grad, few.grid, few.g0, few.g1, (int)a.width, bits,
                          (int)few.lines, (int)few.steps, (int)((few.steps + few.waves - 1) / few.waves), parts);
     };

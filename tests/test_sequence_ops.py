@@ -853,3 +853,36 @@ def test_token_grids_with_a_short_axis(shape, rows, width, name):
         within(got, want, (n + 4).reshape(-1, 1) * u(wide(TYPES[name])) * mag, got.dtype)
         got = ops.embedding_grad(grad_g.transpose(0, 1), view.t(), rows, scale=0.3, dtype=got.dtype)
         within(got, want, (n + 4).reshape(-1, 1) * u(wide(TYPES[name])) * mag, got.dtype)
+
+
+@gpu
+def test_threads_with_tables_of_different_lds_sizes():
+    """Sums of few rows take 66 to 160 KB of LDS a wave here; the launch limit is one of the process, set by every thread."""
+    import threading
+    g = rng(77)
+    steps = []
+    for rows in (18000, 7400, 12000, 9000):
+        grad = normal(g, (20 * rows, 1), torch.float64).cuda()
+        steps.append((grad, make_ids(g, (20 * rows,), rows, torch.int32).cuda(), rows))
+    want = [ops.embedding_grad(*s) for s in steps]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(k):
+        stream = torch.cuda.Stream()
+        try:
+            with torch.cuda.stream(stream):
+                got = [ops.embedding_grad(*steps[k]) for _ in range(40)]
+            stream.synchronize()
+            wrong.extend(k for v in got if not torch.equal(v, want[k]))
+        except Exception as e:                     # noqa: BLE001 - of any kind, for the assertion below
+            wrong.append(e)
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(len(steps))]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not wrong
+    for (grad, ids, rows), got in zip(steps, want):
+        expect, mag, n = lookup_grad_oracle(grad, ids, rows, 1.0)
+        within(got, expect, (n + 4).reshape(-1, 1) * u(torch.float64) * mag, torch.float64)

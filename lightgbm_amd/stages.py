@@ -181,12 +181,14 @@ def refit_stages(booster, data, label, weight=None, num_steps: int = 20, learnin
         raise LightGBMError(f"refit_stages: num_steps has to be a whole number >= 0, got {num_steps!r}")
     if not 0.0 < learning_rate <= 2.0:
         raise LightGBMError(f"refit_stages: learning_rate has to be in (0, 2], got {learning_rate!r}")
-    if not lambda_l2 >= 0.0:
-        raise LightGBMError(f"refit_stages: lambda_l2 has to be >= 0, got {lambda_l2!r}")
+    if not 0.0 <= lambda_l2 < np.inf:
+        raise LightGBMError(f"refit_stages: lambda_l2 has to be a number >= 0, got {lambda_l2!r}")
     y = _to_1d(label, np.float64)
     w = np.ones(rows) if weight is None else _to_1d(weight, np.float64)
     if len(y) != rows or len(w) != rows:
         raise LightGBMError("refit_stages: the label's or the weights' length differs from the number of rows")
+    if not np.isfinite(y).all():          # one NaN would reach every leaf that shares a row with its own
+        raise LightGBMError("refit_stages: the labels have to be finite")
     if kind == "binary":
         y = (y > 0).astype(np.float64)
     target = y.reshape(-1, 1)
@@ -198,8 +200,8 @@ def refit_stages(booster, data, label, weight=None, num_steps: int = 20, learnin
     if rows == 0 or forest.count == 0 or num_steps == 0:
         return out
     total = float(w.sum())
-    if not (w >= 0).all() or not total > 0:
-        raise LightGBMError("refit_stages: weights have to be >= 0 and not all zero")
+    if not (w >= 0).all() or not 0 < total < np.inf:
+        raise LightGBMError("refit_stages: weights have to be finite, with a finite sum, >= 0 and not all zero")
     run = _RefitGpu if _on_gpu(device, rows * len(forest.offsets[:-1])) else _RefitCpu
     values = run(forest, mat, target, w / total, stages).descend(int(num_steps), float(learning_rate), float(lambda_l2))
     lib, _ = _lib.load()

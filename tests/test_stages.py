@@ -170,6 +170,18 @@ def test_refit_stages_refusals():
         multi.refit_stages(Xm, ym + 3)
 
 
+@pytest.mark.parametrize("kind", ["regression", "binary", "multiclass"])
+@pytest.mark.parametrize("odd", [np.nan, np.inf, -np.inf])
+def test_refit_stages_refuses_what_is_not_finite(kind, odd):
+    booster, X, y, w = make(kind, rows=200)
+    label, weight = y.copy(), w.copy()
+    label[3], weight[3] = odd, odd
+    for kw in ({"label": label}, {"label": label, "num_steps": 0}, {"label": label, "weight": np.where(np.arange(200) == 3, 0.0, 1.0)},
+               {"label": y, "weight": weight}, {"label": y, "weight": np.full(200, 1e308)}, {"label": y, "lambda_l2": odd}):
+        with pytest.raises(LightGBMError):
+            booster.refit_stages(X, device="cpu", **kw)
+
+
 def test_the_gpu_is_refused_where_there_is_none():
     from lightgbm_amd import _lib
     if _lib.load()[1]:

@@ -41,6 +41,8 @@ def need_tensor(op: str, name: str, t):
         fail(f"{op}: {name} requires grad, and nothing is recorded here: call it under torch.no_grad() and take the gradient from {op}_grad")
     if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
         fail(f"{op}: {name} is a dual tensor, and its tangent would be lost here: pass its primal value")
+    if not t.data_ptr() and t.numel():
+        fail(f"{op}: {name} has no memory (its storage was released)")
     return t.resolve_neg() if t.is_neg() else t
 
 

@@ -886,3 +886,41 @@ def test_threads_with_tables_of_different_lds_sizes():
     for (grad, ids, rows), got in zip(steps, want):
         expect, mag, n = lookup_grad_oracle(grad, ids, rows, 1.0)
         within(got, expect, (n + 4).reshape(-1, 1) * u(torch.float64) * mag, torch.float64)
+
+
+RELEASED = {
+    "table": lambda d, x: ops.embedding(d(30, 4), _I.to(x.device)),
+    "strided table": lambda d, x: ops.embedding(d(4, 30, columns=True), _I.to(x.device)),
+    "ids": lambda d, x: ops.embedding(x[0], d(3).view(torch.int32)),
+    "grad": lambda d, x: ops.embedding_grad(d(3, 4), _I.to(x.device), 5),
+    "x": lambda d, x: ops.gated_scan(d(2, 3, 4)),
+    "gate": lambda d, x: ops.gated_scan(x, d(2, 3, 4)),
+    "state": lambda d, x: ops.gated_scan(x, None, d(2, 4)),
+    "lengths": lambda d, x: ops.gated_scan(x, lengths=d(2).view(torch.int32)),
+    "grad_states": lambda d, x: ops.gated_scan_grad(d(2, 3, 4), x),
+    "states": lambda d, x: ops.gated_scan_grad(x, d(2, 3, 4)),
+    "x of the gradient": lambda d, x: ops.gated_scan_grad(x, x, torch.ones_like(x), x=d(2, 3, 4), mix=True),
+    "grad_last": lambda d, x: ops.gated_scan_grad(x, x, grad_last=d(2, 4)),
+}
+
+
+def _released(what, device):
+    """Parameters whose storage a sharding wrapper has taken back keep their shape and have the address 0."""
+    def make(*shape, columns=False):
+        t = torch.ones(shape, device=device)
+        t = t.t() if columns else t
+        t.untyped_storage().resize_(0)
+        return t
+    with pytest.raises(LightGBMError, match="no memory"):
+        RELEASED[what](make, _X.to(device))
+
+
+@pytest.mark.parametrize("what", RELEASED)
+def test_tensors_without_memory_are_refused(what):
+    _released(what, "cpu")
+
+
+@gpu
+@pytest.mark.parametrize("what", RELEASED)
+def test_gpu_tensors_without_memory_are_refused(what):
+    _released(what, "cuda")

@@ -924,3 +924,86 @@ def test_tensors_without_memory_are_refused(what):
 @pytest.mark.parametrize("what", RELEASED)
 def test_gpu_tensors_without_memory_are_refused(what):
     _released(what, "cuda")
+
+
+# -- every variant of the lookup's gradient ------------------------------------------------------------------------------
+
+#         tokens shape    rows  width type  transposed
+PATHS = [((3000,), 3000, 1, "f64", False),             # sorted by one workgroup, 8 bytes carried
+         ((60000,), 70000, 1, "f64", False),           # few small tiles, 8 bytes
+         ((190000,), 60000, 1, "f64", False),          # offsets by a kernel of their own, 8 bytes
+         ((210007,), 90000, 1, "f32", False), ((71, 3001), 60000, 2, "bf16", True),
+         ((300, 16411), 400000, 1, "f64", True),       # tiles of 4096, 8 bytes; ids the other way round, ragged edges
+         ((16411, 300), 400000, 1, "f32", True),       # 4 bytes, values carried
+         ((67, 70003), 300000, 3, "f32", False), ((4400000,), 280000, 1, "f16", False),      # 4 bytes, token numbers carried
+         ((1300000,), 82000, 17, "bf16", False),       # strips of 64 tokens and more
+         ((2200, 1000), 140000, 24, "f32", True), ((1400001,), 90000, 40, "f16", False),
+         ((8400001,), 530000, 17, "bf16", False)]
+
+
+@gpu
+@pytest.mark.parametrize("shape,rows,width,name,transposed", PATHS)
+def test_lookup_gradient_of_many_tokens(shape, rows, width, name, transposed):
+    """Sizes that reach the sorts of 4 and 8 bytes by one workgroup, by small and by large tiles, with and without a kernel of its
+    own for the offsets, and the longer strips.  The oracle sums on the GPU in 64 bits, with torch."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    ids = (torch.rand(shape, generator=g, device="cuda", dtype=torch.float64) ** 2 * (rows + 3)).to(torch.int32) - 1
+    grad = torch.randn((*shape, width), generator=g, device="cuda", dtype=wide(TYPES[name])).to(TYPES[name])
+    if transposed:
+        ids = ids.t().contiguous().t()
+    got = ops.embedding_grad(grad, ids, rows, scale=0.5, dtype=torch.float32 if name in ("bf16", "f16") else None)
+    assert torch.equal(got, ops.embedding_grad(grad, ids, rows, scale=0.5, dtype=got.dtype))
+    i = ids.reshape(-1).long()
+    i = torch.where((i >= 0) & (i < rows), i, torch.full_like(i, rows))
+    want, mag = torch.zeros((2, rows + 1, width), dtype=torch.float64, device="cuda")
+    g64 = grad.reshape(-1, width).double()
+    # atomic additions in 64 bits: their order costs n u(fp64), which for fp64 the bound counts twice
+    want.index_add_(0, i, g64)
+    mag.index_add_(0, i, g64.abs())
+    n = torch.bincount(i, minlength=rows + 1).double()
+    want, mag, n = (0.5 * want[:rows]).cpu(), (0.5 * mag[:rows]).cpu(), n[:rows].cpu()
+    within(got, want, (2 * n + 4).reshape(-1, 1) * u(wide(TYPES[name])) * mag, got.dtype)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["f64", "f32", "bf16"])
+@pytest.mark.parametrize("width", [1, 2])
+def test_lookup_of_many_narrow_rows(name, width):
+    """More tokens than small tiles are taken for, ids the other way round, edges that fill no tile."""
+    g = torch.Generator(device="cuda").manual_seed(width)
+    ids = torch.randint(-1, 38102, (15013, 301), generator=g, device="cuda", dtype=torch.int32)
+    table = torch.randn((38101, width), generator=g, device="cuda", dtype=torch.float64).to(TYPES[name])
+    padded = torch.cat([table, torch.zeros((1, width), dtype=table.dtype, device="cuda")])
+    for view in (ids, ids.t(), ids[1:, 3:], ids.t()[2:, 5:], ids.long().t()):
+        want = padded[torch.where((view >= 0) & (view < 38101), view, torch.full_like(view, 38101)).long()]
+        assert torch.equal(ops.embedding(table, view), want)
+
+
+#        tokens rows width type: sums in one workgroup's list, sums in LDS, sorted by one workgroup, by tiles, wide rows
+ODD = [(300, 50, 3, "f32"), (40000, 500, 1, "f32"), (40000, 500, 2, "bf16"), (3000, 3000, 1, "f64"), (3000, 3000, 2, "f16"), (90000, 40000, 1, "f64"),
+       (90000, 40000, 5, "f32"), (3000, 2000, 40, "bf16"), (50000, 20000, 24, "f64")]
+
+
+@gpu
+@pytest.mark.parametrize("tokens,rows,width,name", ODD)
+def test_infinite_and_nan_gradients_reach_their_own_rows_only(tokens, rows, width, name):
+    g = rng(tokens + width)
+    ids = make_ids(g, (tokens,), rows, torch.int32, 0.1)
+    grad = normal(g, (tokens, width), TYPES[name])
+    clean = ops.embedding_grad(grad.cuda(), ids.cuda(), rows).cpu()
+    inside = (ids >= 0) & (ids < rows)
+    used = torch.nonzero(inside).reshape(-1)
+    named = torch.unique(ids[inside])
+    for tok in torch.nonzero(~inside).reshape(-1)[:20].tolist():          # padding: whatever it holds
+        grad[tok] = float("nan")
+    plus, nan, both = named[1].item(), named[len(named) // 2].item(), named[-1].item()
+    first = {r: used[ids[used] == r][0].item() for r in (plus, nan, both)}
+    grad[first[plus], 0], grad[first[nan], width - 1], grad[first[both], 0] = float("inf"), float("nan"), -float("inf")
+    if int((ids == both).sum()) > 1:
+        grad[used[ids[used] == both][-1], 0] = float("inf")               # inf - inf
+    got = ops.embedding_grad(grad.cuda(), ids.cuda(), rows).cpu()
+    want, _, _ = lookup_grad_oracle(torch.where(torch.isfinite(grad), torch.zeros_like(grad), grad), ids, rows, 1.0)
+    odd = ~torch.isfinite(want)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isinf(got), torch.isinf(want))
+    assert torch.equal(got[odd & torch.isinf(want)].double(), want[odd & torch.isinf(want)])
+    assert torch.equal(got[~odd], clean[~odd])                            # and no other value changes by a bit

@@ -55,13 +55,13 @@ def need_type(op: str, name: str, t) -> int:
 
 def need_device(op: str, first, *others) -> int:
     """All tensors on one GPU; returns its index."""
-    device = first.device
+    device = first.get_device()            # -1 on the CPU; the device object's words are only looked at for a message
     for t in others:
-        if t is not None and t.device != device:
-            fail(f"{op}: tensors on {device} and {t.device}")
-    if device.type != "cuda":
-        fail(f"{op}: needs tensors on the GPU, got {device}")
-    return device.index
+        if t is not None and t.get_device() != device:
+            fail(f"{op}: tensors on {first.device} and {t.device}")
+    if not first.is_cuda:
+        fail(f"{op}: needs tensors on the GPU, got {first.device}")
+    return device
 
 
 # The current stream's handle without a Python Stream object around it (2 us less a call), where torch offers that.

@@ -5,6 +5,7 @@
 #include "seq_types.hpp"
 #include "token_sort.hpp"
 #include <algorithm>
+#include <cmath>
 
 namespace lga {
 
@@ -857,6 +858,8 @@ void lookup(const LookupArgs& a) {
 
 int64_t lookup_grad_workspace(const LookupGradArgs& a) {
   check_sizes(a.rows, a.width, a.n0, a.n1);
+  // rows that no id names are zero, which no other factor leaves a sum of nothing
+  if (!std::isfinite(a.type == kF64 ? a.scale : (float)a.scale)) throw std::runtime_error("embedding_grad: the scale has to be finite");
   if (owned(a)) return 0;
   const PrivatePlan few = plan_private(a);
   if (few.waves) return few.waves * a.rows * a.width * (a.type == kF64 ? 8 : 4);

@@ -63,7 +63,7 @@ def embedding_grad(grad, ids, num_rows: int, scale: float = 1.0, dtype=None):
     ``[num_rows, width]``; rows that no id names are zero, ids outside the table are left out.
 
     ``grad``: ``[*ids.shape, width]`` (an expanded tensor is read in place).  ``dtype``: the result's type, ``grad``'s own
-    or float32; the sums are held in 32 bits (64 for fp64).  The tokens are sorted, so every row is added up in the order
+    or float32; the sums are held in 32 bits (64 for fp64); ``scale`` has to be finite.  The tokens are sorted, so every row is added up in the order
     of its tokens and the result does not depend on timing.
     """
     grad = need_tensor("embedding_grad", "grad", grad)

@@ -1007,3 +1007,16 @@ def test_infinite_and_nan_gradients_reach_their_own_rows_only(tokens, rows, widt
     assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isinf(got), torch.isinf(want))
     assert torch.equal(got[odd & torch.isinf(want)].double(), want[odd & torch.isinf(want)])
     assert torch.equal(got[~odd], clean[~odd])                            # and no other value changes by a bit
+
+
+@gpu
+@pytest.mark.parametrize("tokens,rows,width", [(300, 50, 3), (40000, 500, 1), (3000, 3000, 2), (50000, 20000, 24)])
+def test_scales_that_are_not_finite_are_refused_by_every_variant(tokens, rows, width):
+    """Times infinity a row that no id names would be NaN, not zero."""
+    grad, ids = torch.ones((tokens, width), device="cuda"), torch.zeros(tokens, dtype=torch.int32, device="cuda")
+    for scale in (float("inf"), -float("inf"), float("nan"), 1e39):          # the last one in fp32
+        with pytest.raises(LightGBMError, match="finite"):
+            ops.embedding_grad(grad, ids, rows, scale=scale)
+    got = ops.embedding_grad(grad.double(), ids, rows, scale=1e39)
+    assert got[0].eq(tokens * 1e39).all() or (got[0] / (tokens * 1e39) - 1).abs().max() < 1e-12
+    assert not got[1:].any()

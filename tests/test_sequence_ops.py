@@ -1020,3 +1020,62 @@ def test_scales_that_are_not_finite_are_refused_by_every_variant(tokens, rows, w
     got = ops.embedding_grad(grad.double(), ids, rows, scale=1e39)
     assert got[0].eq(tokens * 1e39).all() or (got[0] / (tokens * 1e39) - 1).abs().max() < 1e-12
     assert not got[1:].any()
+
+
+#            ids' shape   rows  width type: one list, LDS sums of up to 64 KB and above, sorted by one workgroup, by small and large tiles
+CAPTURED = [((300,), 50, 3, "f32"), ((70, 300), 900, 1, "f32"), ((40, 8000), 15000, 1, "f64"), ((3000,), 3000, 2, "f16"), ((60000,), 70000, 1, "f64"),
+            ((300, 16411), 400000, 1, "f32"), ((50000,), 20000, 24, "bf16")]
+
+
+@gpu
+@pytest.mark.parametrize("shape,rows,width,name", CAPTURED)
+def test_every_variant_of_the_gradient_can_be_captured(shape, rows, width, name):
+    g = rng(rows)
+    sets = [(make_ids(g, shape, rows, torch.int32, 0.05).cuda(), normal(g, (*shape, width), TYPES[name]).cuda()) for _ in range(2)]
+    want = [ops.embedding_grad(grad, ids, rows) for ids, grad in sets]
+    ids, grad = (torch.zeros_like(v) for v in sets[0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.embedding_grad(grad, ids, rows)
+    for replay in range(4):
+        ids.copy_(sets[replay % 2][0])
+        grad.copy_(sets[replay % 2][1])
+        graph.replay()
+        eager = ops.embedding_grad(*sets[1 - replay % 2][::-1], rows)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[replay % 2]) and torch.equal(eager, want[1 - replay % 2])
+        out.zero_()
+
+
+@gpu
+@pytest.mark.parametrize("case", [(2, 1, 64, "bf16", "f32", 64), (1, 3000, 40, "f64", "f64", 1), (3, 700, 515, "f32", "f32", 5), (2, 900, 96, "f16", "f16", 0),
+                                  (1, 9000, 70, "bf16", "bf16", 70)], ids=lambda c: "-".join(map(str, c)))
+def test_recurrences_of_every_kind_of_gate_can_be_captured(case):
+    b, t, d, name, gate_name, groups = case
+    g = rng(t)
+    sets = []
+    for _ in range(2):
+        x, gate, state, _ = make_scan(g, b, t, d, name, gate_name, groups, b, True, False)
+        sets.append([v if v is None else v.cuda() for v in (x, gate, state, normal(g, (b, t, d), TYPES[name]))])
+
+    def run(x, gate, state, dh):
+        states, last = ops.gated_scan(x, gate, state)
+        return [v for v in (states, last, *ops.gated_scan_grad(dh, states, gate, state)) if v is not None]
+    want = [run(*s) for s in sets]
+    still = [v if v is None else torch.zeros_like(v) for v in sets[0]]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(*still)
+    for replay in range(4):
+        for dst, src in zip(still, sets[replay % 2]):
+            if dst is not None:
+                dst.copy_(src)
+        graph.replay()
+        eager = run(*sets[1 - replay % 2])
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, want[replay % 2]))
+        assert all(torch.equal(p, q) for p, q in zip(eager, want[1 - replay % 2]))
+        for v in out:
+            v.zero_()

@@ -612,17 +612,23 @@ Cut cut_steps(int64_t batch, int64_t steps, int64_t width, int v, int per_lane, 
   if (k.tiles == 1 && k.slots == 1) k.lanes = k.packs >= kThreads ? kThreads : k.lanes;
   k.pack_rows = (k.packs + k.lanes - 1) / k.lanes;
   // Close checkpoints leave little to fold, far ones make a short chain of tiles that wait for one another; with many rows
-  // of tiles the chain has time (8 x 4096 x 2560 bf16, 160 rows: 149 us with 8, 157 us with 32; 1 x 65537 x 1024, 8 rows: 123 us
-  // with 8, 116 us with 16).
-  k.checkpoint = k.pack_rows >= 32 ? 8 : k.pack_rows >= 8 ? 16 : 32;
+  // of tiles the chain has time.  bf16, every 8 against every 32 tiles, forward and backward: 1 row of 65537 steps 111 / 145 against
+  // 47 / 58 us, 8 x 48828 99 / 151 against 86 / 126, 16 x 24414 84 / 124 against 83 / 115, 31 x 12600 82 / 112 against 84 / 111,
+  // 64 x 6103 76 / 106 against 79 / 111, 160 x 2441 72 / 106 against 76 / 110.
+  k.checkpoint = k.pack_rows >= 32 ? 8 : 32;
   if (k.tiles * k.pack_rows * k.lanes * k.slots > 4294967295LL) throw std::runtime_error("gated_scan: the tensor is too large");
   return k;
 }
 
-// Two workgroups of 8 chunks a CU overlap loads with sums better than one of 16 (8 x 4096 x 2560 bf16: 156 against 161 us),
-// but a long sequence has fewer maps to fold in larger tiles (1 x 65537 x 1024 bf16: 116 against 128 us).
-// Up to kMaxSlots chunks are one tile, which needs neither a workspace nor tickets.
-int scan_slots(const ScanArgs& a) { return a.steps > 64 * 8 * kScanSteps || a.steps <= kMaxSlots * kScanSteps ? kMaxSlots : 8; }
+// Chunks of a tile forwards.  Two workgroups of 8 chunks a CU overlap loads with sums better than one of 16 where there are many
+// rows of tiles; few rows rather have fewer maps to fold, unless there are few steps in all (bf16, 8 against 16 chunks: 8 rows of 16384
+// steps 44 against 38 us, 32 x 4096 37 against 33, 128 x 1024 34 against 31, 64 x 16384 184 against 192, 160 x 4096 112 against 125,
+// 24 x 1024 16.5 against 18.0; with fp32 gates, in fp32 and in fp64 the two change places at the same sizes or, for fp32 gates, at
+// 48 rows).  Up to kMaxSlots chunks are one tile, which needs neither a workspace nor tickets.
+int scan_slots(const ScanArgs& a, int v) {
+  const int64_t rows = (a.batch * ((a.width + v - 1) / v) + kLanes - 1) / kLanes;
+  return a.steps > kMaxSlots * kScanSteps && (rows >= 160 || (rows >= 64 && a.steps >= 4096) || rows * a.steps <= 32768) ? 8 : kMaxSlots;
+}
 
 // Backwards: values of 16 bits leave room for 16 steps a lane in 128 registers (8 x 4096 x 2560 bf16: 277 us with 16 steps and 8
 // chunks, 299 us with 8 and 16); of fp32 (1 x 423 x 26734: 69 against 109 us) and fp64 they do not.
@@ -709,7 +715,7 @@ int64_t slope_values(const ScanGradArgs& a, const GateSums& g) {
 int64_t scan_workspace(const ScanArgs& a) {
   check_args(a);
   const int v = two_wide(a) ? 2 : 1;
-  const Cut k = cut_steps(a.batch, a.steps, a.width, v, a.steps <= 1 ? 1 : kScanSteps, scan_slots(a));
+  const Cut k = cut_steps(a.batch, a.steps, a.width, v, a.steps <= 1 ? 1 : kScanSteps, scan_slots(a, v));
   return 8 * (a.type == kF64 ? work_words<double>(k, v, a.gate != 0) : work_words<float>(k, v, a.gate != 0));
 }
 
@@ -722,7 +728,7 @@ void gated_scan(const ScanArgs& a) {
     typedef decltype(gg) G;
     by_shape<sizeof(T) < 8, kScanSteps>(a, [&](auto kind, auto v, auto l) {
       constexpr int V = decltype(v)::value, L = decltype(l)::value;
-      const Cut k = cut_steps(a.batch, a.steps, a.width, V, L, scan_slots(a));
+      const Cut k = cut_steps(a.batch, a.steps, a.width, V, L, scan_slots(a, V));
       clear_work<Wide<T>>(k, V, a.gate != 0, (uint64_t*)a.work, (hipStream_t)a.stream);
       hipLaunchKernelGGL((scan_kernel<T, G, (GateKind)decltype(kind)::value, V, L>), dim3((unsigned)(k.tiles * k.pack_rows)), dim3(k.lanes * k.slots),
                          fold_bytes<Wide<T>>(k, V, a.gate != 0), (hipStream_t)a.stream, a, k);

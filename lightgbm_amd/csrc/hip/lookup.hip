@@ -18,7 +18,10 @@ __device__ __forceinline__ int64_t load_id(const void* ids, int64_t at, int ids6
   return ids64 ? reinterpret_cast<const int64_t*>(ids)[at] : (int64_t)reinterpret_cast<const int32_t*>(ids)[at];
 }
 
-constexpr int kNarrow = 16;      // rows of up to this many values go through a tile of tokens
+// Rows of up to this many values go through a tile of tokens, wider ones are copied and summed by groups of lanes (1 M tokens of
+// 70000 rows, tile against groups: 12 bf16 values 22 against 12 us, their gradient 102 against 78; 9 fp32 values 22 against 17 and 109
+// against 76; below eight 16-bit values a row is shorter than a pack).
+constexpr int kNarrow = 8;
 
 // Rows of more than kNarrow values: `group` lanes copy a row in packs of V, four in flight.  Bound by HBM: 32768 rows of 4096
 // bf16 values, 85 us (one lane per value took 366).
@@ -656,8 +659,10 @@ template <typename T> void run_lookup(const LookupArgs& a) {
     grid.ids64 = (int)a.ids64;
     grid.n0 = a.n0, grid.n1 = a.n1, grid.s0 = a.s0, grid.s1 = a.s1;
     grid.rows = a.rows;
-    TokenTiles tiles = token_tiles(grid, 10);      // small tiles until there are enough for every CU
-    if (tiles.blocks > 4096) tiles = token_tiles(grid);
+    // Small tiles until there are enough for every CU: 300 trees of fp64 leaf values, tiles of 1024 against 4096: 10000 rows (3125 small
+    // tiles) 13.6 against 17.7 us, 20000 rows (6250) 27 against 29, 45800 rows (14315) 70 against 58.
+    TokenTiles tiles = token_tiles(grid, 10);
+    if (tiles.blocks > 8192) tiles = token_tiles(grid);
     auto run = [&](auto kernel, auto* ids) {
       hipLaunchKernelGGL(kernel, dim3((unsigned)tiles.blocks), dim3(kThreads), 0, (hipStream_t)a.stream, (const T*)a.table, ids, (T*)a.out, a.rows,
                          (int)a.width, a.table_stride, grid, tiles, (Wide<T>)a.scale);
@@ -679,10 +684,16 @@ template <typename T> void run_lookup(const LookupArgs& a) {
   LGA_HIP_CHECK(hipGetLastError());
 }
 
-// Up to this many tokens every workgroup looks through all ids for its own rows (256 tokens, 8192 rows of 512 fp32 values: 11 us,
-// sorted 25 us); above, or for tables of more rows, they are sorted.
+// Up to this many tokens every workgroup looks through all ids for its own rows; above, or for tables of more rows, they are sorted
+// (256 tokens, 8192 rows of 512 fp32 values: 11 against 23 us; 512 tokens: 8192 x 512 13 against 23, 131072 x 512 53 against 69,
+// 100000 x 3 19 against 20, but 32000 x 4096 148 against 131; 1024 tokens: 131072 x 512 78 against 70, 8192 x 512 16 against 24).
 constexpr int64_t kOwnedTokens = 512, kOwnedTable = 131072;
-constexpr int64_t kPrivateLds = 160 * 1024;      // of a wave, for the sums of a column
+// Sums in a wave's LDS where the table fits and tokens outnumber its rows.  That is a bet on leaf tokens, whose lanes meet seldom:
+// against sorting, 13 M of them in 300 trees of 31 leaves 61 against 289 us (fp32), 1 M 31 against 48, 100 trees of 127 leaves 86 against
+// 339; but 3 trees, whose lanes are mostly idle, 296 against 199, and ids drawn from the whole table, where lanes meet in most
+// groups, 14 M of 3000 rows 164 against 280, of 9300 rows 324 against 296, of 18000 rows 745 against 300.
+constexpr int64_t kPrivateLds = 160 * 1024, kPrivateRatio = 16;
+constexpr int kPrivateWidth = 16;
 
 struct GradPlan {
   TokenGrid grid;
@@ -740,7 +751,7 @@ struct PrivatePlan {
 PrivatePlan plan_private(const LookupGradArgs& a) {
   PrivatePlan p;
   const int64_t wide = a.type == kF64 ? 8 : 4, tokens = a.n0 * a.n1, lds = (a.rows + 1) * (wide + 1);
-  if (a.width > kNarrow || lds > kPrivateLds || tokens < 16 * a.rows) return p;
+  if (a.width > kPrivateWidth || lds > kPrivateLds || tokens < kPrivateRatio * a.rows) return p;
   p.grid.ids = (const void*)a.ids;
   p.grid.ids64 = (int)a.ids64;
   p.grid.rows = a.rows;

@@ -27,6 +27,11 @@ struct Pass {
   int shift, bits;
   bool few;                     // few tiles: no kernel of its own for the offsets
 };
+// Up to kFewTiles tiles a scatter adds up the counts of its digits itself, above a kernel of its own does (by itself against
+// with that kernel: 50000 rows of 1024 bf16 values, 68 tiles, 85 against 88 us; 70000 rows, 6 tiles 29 against 36, 59 tiles 33 against 34,
+// 98 tiles 37 against 34, 293 tiles 60 against 39).
+// Up to kSmallTiles small tiles they stay small (1 M tokens, 977 small tiles: 56 against 72 us with tiles of 4096; 3 M in two passes 100
+// against 90, in three 101 against 106; 6 M 170 against 146 and 159 against 171).
 constexpr int64_t kFewTiles = 128, kSmallTiles = 4096;
 
 __device__ __forceinline__ uint32_t grid_key(const TokenGrid& g, int64_t i, int64_t j) {

@@ -1079,3 +1079,21 @@ def test_recurrences_of_every_kind_of_gate_can_be_captured(case):
         assert all(torch.equal(p, q) for p, q in zip(eager, want[1 - replay % 2]))
         for v in out:
             v.zero_()
+
+
+@gpu
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("width", [8, 9, 11, 15, 16, 17])
+def test_widths_around_a_pack(width, name):
+    """Rows of a pack or two: tiles of tokens up to eight values, groups of lanes whose last pack starts earlier above."""
+    g = rng(width)
+    for shape, rows in (((700,), 900), ((20011,), 30000), ((9, 1300), 9000), ((3000, 7), 20000)):
+        table, ids = normal(g, (rows, width), TYPES[name]), make_ids(g, shape, rows, torch.int32)
+        got = ops.embedding(table.cuda(), ids.cuda(), 0.3)
+        want = lookup_oracle(table, ids, 0.3)
+        within(got, want, 3 * u(wide(TYPES[name])) * want.abs(), TYPES[name])
+        grad = normal(g, (*shape, width), TYPES[name])
+        for to, ids_to in ((grad.cuda(), ids.cuda()), (_on_gpu(grad.transpose(0, -2)), _on_gpu(ids.transpose(0, -1)))):
+            got = ops.embedding_grad(to, ids_to, rows, scale=2.0, dtype=torch.float32 if name in ("bf16", "f16") else None)
+            want, mag, n = lookup_grad_oracle(grad, ids, rows, 2.0)
+            within(got, want, (n + 4).reshape(-1, 1) * u(wide(TYPES[name])) * mag, got.dtype)

@@ -60,8 +60,8 @@ __global__ __launch_bounds__(kThreads) void lookup_rows_kernel(const T* __restri
 }
 
 // Narrow rows: a workgroup takes a tile of tokens, reads its ids along the axis on which they are neighbours, and writes
-// along the axis on which the results are.  300 trees x 45800 rows of one fp64 value, ids by row: 57 us (2.9 TB/s; ids come in
-// pieces of 256 bytes), 198 us with one lane per value.
+// along the axis on which the results are.  300 trees x 45800 rows of one fp64 value, ids by row: 57 us (2.9 TB/s; what bounds it has
+// not been taken apart: ids come in pieces of 256 bytes, and a tile gathers from 64 trees' values), 198 us with one lane per value.
 template <typename T, typename I, int kBits>
 __global__ __launch_bounds__(kThreads) void lookup_tile_kernel(const T* __restrict__ table, const I* __restrict__ ids, T* __restrict__ out, int64_t rows,
                                                                int width, int64_t table_stride, TokenGrid grid, TokenTiles tiles, Wide<T> scale) {
@@ -660,9 +660,10 @@ template <typename T> void run_lookup(const LookupArgs& a) {
     grid.n0 = a.n0, grid.n1 = a.n1, grid.s0 = a.s0, grid.s1 = a.s1;
     grid.rows = a.rows;
     // Small tiles until there are enough for every CU: 300 trees of fp64 leaf values, tiles of 1024 against 4096: 10000 rows (3125 small
-    // tiles) 13.6 against 17.7 us, 20000 rows (6250) 27 against 29, 45800 rows (14315) 70 against 58.
+    // tiles) 13.6 against 17.7 us, 20000 rows (6250) 27 against 29, 45800 rows (14315) 70 against 58; 100 trees x 45800 rows of three fp32
+    // values (5728) 32 against 31.
     TokenTiles tiles = token_tiles(grid, 10);
-    if (tiles.blocks > 8192) tiles = token_tiles(grid);
+    if (tiles.blocks > 4096) tiles = token_tiles(grid);
     auto run = [&](auto kernel, auto* ids) {
       hipLaunchKernelGGL(kernel, dim3((unsigned)tiles.blocks), dim3(kThreads), 0, (hipStream_t)a.stream, (const T*)a.table, ids, (T*)a.out, a.rows,
                          (int)a.width, a.table_stride, grid, tiles, (Wide<T>)a.scale);

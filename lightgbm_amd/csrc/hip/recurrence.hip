@@ -10,9 +10,9 @@
 // through memory, folds the maps before it, and then walks its chunks again from the exact state before each: every
 // value is read once and written once.  All folds run in the order of the steps, so results do not depend on timing.
 //
-// Bound by HBM where there are enough rows of tiles: 8 x 4096 x 2560 bf16 with fp32 gates, mixed, 143 us forward (4.7 TB/s) and
-// 278 us backward (4.8 TB/s) where a copy reaches 4.9; 500 x 45800 fp64 with one gate a step 96 us (3.8 TB/s).  One sequence of
-// 65537 x 1024 bf16 takes 118 us (3.4 TB/s): its eight rows of tiles leave a CU one workgroup, which loads, folds and stores in
+// Bound by HBM where there are enough rows of tiles: 8 x 4096 x 2560 bf16 with fp32 gates, mixed, 141 us forward (4.8 TB/s) and
+// 269 us backward (5.0 TB/s) where a copy reaches 4.9; 500 x 45800 fp64 with one gate a step 94 us (3.9 TB/s).  One sequence of
+// 65537 x 1024 bf16 takes 115 us (3.5 TB/s): its eight rows of tiles leave a CU one workgroup, which loads, folds and stores in
 // turn.  One lane walking a channel through all steps took 1877 us, 61.6 ms, 265 us and 30.7 ms.
 #include "recurrence.hpp"
 #include "device.hpp"

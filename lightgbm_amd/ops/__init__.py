@@ -12,7 +12,7 @@ plain NumPy / PyTorch reference in isolation:
 
 and the operators that the prediction and refitting of whole ensembles are made of, for use on any tensors:
 
-* :func:`embedding`, :func:`embedding_grad`   - row lookup by token with scaling, its gradient by sorted tokens
+* :func:`embedding`, :func:`embedding_grad`   - row lookup by token with scaling, its gradient summed by token
 * :func:`gated_scan`, :func:`gated_scan_grad` - gated linear recurrence over long sequences and its gradients
 
 Without a GPU every function raises ``LightGBMError``.

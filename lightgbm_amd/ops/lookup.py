@@ -1,9 +1,9 @@
-"""Row lookup by token and its gradient by sorted tokens (``csrc/hip/lookup.hip``).
+"""Row lookup by token and its gradient (``csrc/hip/lookup.hip``).
 
 A tree ensemble's raw score is a sum of looked-up leaf values (tokens: leaf indices, table: one row per leaf), and the
 gradient of a leaf value is the sum of the gradients of the rows in the leaf; an embedding layer does the same with
 words.  Both run on torch's current stream of the tensors' device, can be captured into a HIP graph, and give the same
-bits every time.
+bits every time for the same sizes, strides and values.
 """
 from __future__ import annotations
 
@@ -63,8 +63,9 @@ def embedding_grad(grad, ids, num_rows: int, scale: float = 1.0, dtype=None):
     ``[num_rows, width]``; rows that no id names are zero, ids outside the table are left out.
 
     ``grad``: ``[*ids.shape, width]`` (an expanded tensor is read in place).  ``dtype``: the result's type, ``grad``'s own
-    or float32; the sums are held in 32 bits (64 for fp64); ``scale`` has to be finite.  The tokens are sorted, so every row is added up in the order
-    of its tokens and the result does not depend on timing.
+    or float32; the sums are held in 32 bits (64 for fp64); ``scale`` has to be finite.  A row's gradients are added up in
+    an order that the sizes, strides and ids determine, never the timing: sorted and strip by strip, or in partial sums of
+    waves where the tokens are few or outnumber the rows.
     """
     grad = need_tensor("embedding_grad", "grad", grad)
     code = need_type("embedding_grad", "grad", grad)

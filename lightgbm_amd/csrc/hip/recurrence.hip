@@ -144,6 +144,14 @@ __device__ __forceinline__ void publish(uint64_t* p, const Map<float, false>& f)
 __device__ __forceinline__ void read_map(const uint64_t* w, Map<float, false>& f) { f = {__uint_as_float((uint32_t)*w)}; }
 __device__ __forceinline__ void publish(uint64_t* p, const Map<double, false>& f) { put_word(p, (uint64_t)__double_as_longlong(f.h)); }
 __device__ __forceinline__ void read_map(const uint64_t* w, Map<double, false>& f) { f = {__longlong_as_double((int64_t)*w)}; }
+// after() for maps that were packed: a product whose e may have been cut has made zero or infinity of every state but zero, which
+// later gates do not bring back.
+template <typename W> __device__ __forceinline__ Map<W, true> behind(const Map<W, true>& later, const Map<W, true>& first) {
+  Map<W, true> f = after(later, first);
+  if (abs(first.e) >= (2 << Bits<W>::exponent) - 3) f.e = first.e;
+  return f;
+}
+template <typename W> __device__ __forceinline__ Map<W, false> behind(const Map<W, false>& later, const Map<W, false>& first) { return after(later, first); }
 template <typename W, bool kGates> constexpr int kMapWords = kGates ? sizeof(W) / 4 : 1;
 
 __global__ __launch_bounds__(kThreads) void fill_words_kernel(uint4* __restrict__ p, int64_t n) {
@@ -217,7 +225,7 @@ __device__ __forceinline__ void carry_in(const Cut& k, uint64_t* work, int64_t t
       for (int v = 0; v < V; ++v) {
         M m;
         read_map(words + v * kWords, m);
-        part[v] = after(m, part[v]);
+        part[v] = behind(m, part[v]);
       }
     }
     for (int v = 0; v < V; ++v) parts[at][v] = normal(part[v]);

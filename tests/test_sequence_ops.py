@@ -1097,3 +1097,23 @@ def test_widths_around_a_pack(width, name):
             got = ops.embedding_grad(to, ids_to, rows, scale=2.0, dtype=torch.float32 if name in ("bf16", "f16") else None)
             want, mag, n = lookup_grad_oracle(grad, ids, rows, 2.0)
             within(got, want, (n + 4).reshape(-1, 1) * u(wide(TYPES[name])) * mag, got.dtype)
+
+
+@gpu
+@pytest.mark.parametrize("name,power", [("f32", 9), ("f64", 90)])
+@pytest.mark.parametrize("fade,grow", [(512, 512), (700, 400), (100, 100), (2000, 2000), (513, 1500)])
+def test_a_state_that_faded_for_good_is_not_brought_back_as_another(name, power, fade, grow):
+    """Gates below one, then their inverses: single steps lose the state on the way, the product of all gates may keep it.  What is
+    left is nothing or the exact power of two times the state, never anything between - and nothing infinite for a state of zero."""
+    w, t = TYPES[name], 4200
+    gate = torch.ones((1, t, 1), dtype=w)
+    gate[:, :fade], gate[:, fade:fade + grow] = 2.0**-power, 2.0**power
+    gate = torch.cat([gate, gate.roll(7, 1)])
+    state = torch.tensor([[1.0, -1.5, 0.0, 3.0]], dtype=w).expand(2, 4).contiguous()
+    x = torch.zeros((2, t, 4), dtype=w)
+    exact = torch.ldexp(state.double(), torch.tensor(power * (grow - fade)))
+    _, last = ops.gated_scan(x.cuda(), gate.cuda(), state.cuda())
+    _, grad_state, _ = ops.gated_scan_grad(x.cuda(), x.cuda(), gate.flip(1).cuda(), grad_last=state.cuda())
+    for got in (last.cpu().double(), grad_state.cpu().double()):
+        assert (got.eq(0) | got.eq(exact) | (exact.abs() > torch.finfo(w).max) & (got.abs() >= torch.finfo(w).max)).all(), got
+        assert got[:, 2].eq(0).all()

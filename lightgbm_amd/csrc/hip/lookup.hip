@@ -692,9 +692,9 @@ constexpr int64_t kOwnedTokens = 512, kOwnedTable = 131072;
 // Sums in a wave's LDS where the table fits and tokens outnumber its rows.  That is a bet on leaf tokens, whose lanes meet seldom:
 // against sorting, 13 M of them in 300 trees of 31 leaves 61 against 289 us (fp32), 1 M 31 against 48, 100 trees of 127 leaves 86 against
 // 339; but 3 trees, whose lanes are mostly idle, 296 against 199, and ids drawn from the whole table, where lanes meet in most
-// groups, 14 M of 3000 rows 164 against 280, of 9300 rows 324 against 296, of 18000 rows 745 against 300.
+// groups, 14 M of 3000 rows 164 against 280, of 9300 rows 324 against 296, of 18000 rows 745 against 300.  Wider rows than
+// narrow ones are not worth it: 3 M leaf tokens (100 trees of 31 leaves) of 8 fp32 values 122 against 173 us, of 9 values 234 against 169.
 constexpr int64_t kPrivateLds = 160 * 1024, kPrivateRatio = 16;
-constexpr int kPrivateWidth = 16;
 
 struct GradPlan {
   TokenGrid grid;
@@ -752,7 +752,7 @@ struct PrivatePlan {
 PrivatePlan plan_private(const LookupGradArgs& a) {
   PrivatePlan p;
   const int64_t wide = a.type == kF64 ? 8 : 4, tokens = a.n0 * a.n1, lds = (a.rows + 1) * (wide + 1);
-  if (a.width > kPrivateWidth || lds > kPrivateLds || tokens < kPrivateRatio * a.rows) return p;
+  if (a.width > kNarrow || lds > kPrivateLds || tokens < kPrivateRatio * a.rows) return p;
   p.grid.ids = (const void*)a.ids;
   p.grid.ids64 = (int)a.ids64;
   p.grid.rows = a.rows;
